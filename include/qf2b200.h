@@ -105,6 +105,25 @@ int qf2_rope_scatter(const void* x, const int64_t* x_strides, const float* f, in
                      void* y, const int64_t* y_strides, int64_t B, int64_t N, int64_t M, int64_t H, int64_t D,
                      int dtype, void* workspace, qf2_stream_t stream);
 
+/* Rotary positions from token positions and frequencies (no counterpart in the reference,
+ * whose rope_apply takes a table of complex factors): pair p < rotary_dim / 2 of a head row
+ * at position t turns by theta = t * inv_freq[p],
+ *   a' = gain (a cos - b sin), b' = gain (b cos + a sin)    (inverse != 0: sin -> -sin)
+ * with (a, b) = (x[p], x[p + rotary_dim / 2]) for QF2_ROTARY_HALF or (x[2p], x[2p + 1]) for
+ * QF2_ROTARY_INTERLEAVED; channels from rotary_dim on are copied.  Angles in 64 bits, the
+ * rotation in fp32, one rounding.  positions int32 or int64 (pos_is_i64) on the device,
+ * strides {batch, seq} (0 broadcasts); inv_freq fp64 on the device.  Tensors as
+ * qf2_rope_apply: strides {batch, seq, head} in elements, contiguous last dim, xk may be
+ * absent (Hk = 0), out may be the input itself.  D <= 1024, rotary_dim even, <= D.  Rows
+ * that are not 16-byte aligned take single-element accesses. */
+#define QF2_ROTARY_HALF 0
+#define QF2_ROTARY_INTERLEAVED 1
+int qf2_rotary_apply(const void* xq, void* xq_out, int64_t Hq, const int64_t* xq_strides,
+                     const int64_t* xq_out_strides, const void* xk, void* xk_out, int64_t Hk,
+                     const int64_t* xk_strides, const int64_t* xk_out_strides, const void* positions,
+                     const int64_t* pos_strides, int pos_is_i64, const double* inv_freq, int64_t rotary_dim, int layout,
+                     float gain, int inverse, int64_t B, int64_t S, int64_t D, int dtype, qf2_stream_t stream);
+
 /* ------------------------------------------------------------- RMSNorm --
  * Replaces rmsnorm_apply (src/kernels/__init__.py:73-80) and the Triton
  * apply_rmsnorm (src/kernels/triton/rmsnorm.py:72-95).
@@ -229,6 +248,57 @@ int qf2_blocksparse_attn(const void* q, const int64_t* q_strides, const void* k,
                          const void* v, const int64_t* v_strides, void* out, const int64_t* out_strides, int64_t B,
                          int64_t Hq, int64_t Hkv, int64_t S, int64_t D, const int32_t* idx, int64_t keep,
                          float sm_scale, int dtype, void* workspace, int64_t workspace_bytes, qf2_stream_t stream);
+
+/* ------------------------------------- masked, capped and biased attention --
+ * 16-bit attention with masks (the reference's flash / SDPA branches take key padding only,
+ * src/models/common/attn.py:92-130; its text encoders come from a third-party package):
+ *   s(i, j) = sm_scale q_i . k_j;  softcap > 0: s = softcap tanh(s / softcap);
+ *   slopes: s -= slopes[h] |t_i - j|;  bias_table: s += bias_table[h][clamp(j - t_i, -R, R) + R]
+ *   out_i = sum e^s(i, j) v_j / sum e^s(i, j) over the keys j that i sees, 0 if it sees none
+ * with t_i = q_offset + i the query's position (const, per batch element, or END: the
+ * queries are the last Sq positions of the sequence's kv_lens keys; offsets beyond 2^29 are
+ * taken as 2^29).  The query sees key j if
+ *   j < kv_lens[b] (clamped to [0, Skv]; NULL: Skv)  and
+ *   j < prefix_lens[b]  or  (left < 0 or j >= t_i - left) and (right < 0 or j <= t_i + right)
+ *   and, with ids, q_ids[b][i] == k_ids[b][j] >= 0 (ids of documents; negative = padding).
+ * Causal attention is right = 0.  A key hidden from every row is not read into the result,
+ * whatever its bits; a NaN or infinite value that some rows see may reach the others of
+ * its 128-row tile (0 * NaN), as it does in a plain product.
+ * prefix_k / prefix_v [P, Hkv, D] (strides {-, head, seq}): keys and values that all batch
+ * elements share at positions 0 .. P - 1, read once for the rows of many batch elements;
+ * the own key j, the queries and kv_lens then count from position P.  Not with ids.
+ * q/k/v/out strides = {batch, head, seq} in elements, multiples of 8, rows 16-byte aligned;
+ * QF2_BF16 or QF2_F16; D = 64, 96, 128 or 256; Hq % Hkv == 0; Sq, Skv, P up to 2^20 with at
+ * most 8192 key tiles of 128; R <= 1024.  Arrays on the device, contiguous.  Scores, sums
+ * and outputs are fp32, probabilities are rounded to the operand type.
+ * A bounded wait that gave up is reported by qf2_masked_attn_status (synchronizes the
+ * stream, clears the word; one word per device for all calls). */
+#define QF2_OFFSET_CONST 0
+#define QF2_OFFSET_ARRAY 1
+#define QF2_OFFSET_END 2
+typedef struct qf2_attn_mask {
+  int64_t left, right;        /* band around the query's position, < 0: open           */
+  const int32_t* kv_lens;     /* [B] or NULL                                           */
+  const int32_t* prefix_lens; /* [B] or NULL                                           */
+  const int32_t* q_offsets;   /* [B], for QF2_OFFSET_ARRAY                             */
+  int64_t q_offset;           /* for QF2_OFFSET_CONST                                  */
+  int64_t q_offset_mode;
+  const int32_t* q_ids;       /* [B, Sq] or NULL                                       */
+  const int32_t* k_ids;       /* [B, Skv] or NULL, with q_ids                          */
+  const float* slopes;        /* [Hq] or NULL                                          */
+  const float* bias_table;    /* [Hq, 2 * bias_reach + 1] or NULL, not with slopes     */
+  int64_t bias_reach;
+  float softcap;              /* 0: none                                               */
+} qf2_attn_mask;
+int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P,
+                                        int64_t D, int with_ids);
+int qf2_masked_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
+                    const int64_t* v_strides, void* out, const int64_t* out_strides, int64_t B, int64_t Hq,
+                    int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D, const void* prefix_k,
+                    const int64_t* prefix_k_strides, const void* prefix_v, const int64_t* prefix_v_strides, int64_t P,
+                    const qf2_attn_mask* mask, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
+                    qf2_stream_t stream);
+int qf2_masked_attn_status(qf2_stream_t stream);
 
 /* ------------------------------------------------------ quantized linears --
  * Replace the torchao weight subclasses the reference swaps into nn.Linear.weight

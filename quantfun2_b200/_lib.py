@@ -6,6 +6,7 @@ an sm_100 part, every op raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 from ctypes import c_float, c_int, c_int64, c_void_p, POINTER
@@ -19,9 +20,22 @@ QF2_OK = 0
 QF2_F32, QF2_F16, QF2_BF16, QF2_I8, QF2_E4M3, QF2_I32 = range(6)
 QF2_ROPE_FP16_TRIG = 1
 QF2_RMS_EAGER, QF2_RMS_FUSED = 0, 1
+QF2_ROTARY_HALF, QF2_ROTARY_INTERLEAVED = 0, 1
+QF2_OFFSET_CONST, QF2_OFFSET_ARRAY, QF2_OFFSET_END = 0, 1, 2
 
 _P64 = POINTER(c_int64)
 _P32 = POINTER(ctypes.c_int32)
+
+
+
+class AttnMask(ctypes.Structure):
+    """qf2_attn_mask of include/qf2b200.h."""
+
+    _fields_ = [("left", c_int64), ("right", c_int64), ("kv_lens", c_void_p), ("prefix_lens", c_void_p),
+                ("q_offsets", c_void_p), ("q_offset", c_int64), ("q_offset_mode", c_int64), ("q_ids", c_void_p),
+                ("k_ids", c_void_p), ("slopes", c_void_p), ("bias_table", c_void_p), ("bias_reach", c_int64),
+                ("softcap", c_float)]
+
 
 # name -> (restype, argtypes); mirrors include/qf2b200.h
 SIGNATURES = {
@@ -86,6 +100,20 @@ SIGNATURES = {
         [c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_int64, c_int64, c_int64, c_int64,
          c_int64, c_void_p, c_int64, c_float, c_int, c_void_p, c_int64, c_void_p],
     ),
+    "qf2_rotary_apply": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, _P64, _P64, c_void_p, c_void_p, c_int64, _P64, _P64, c_void_p, _P64, c_int,
+         c_void_p, c_int64, c_int, c_float, c_int, c_int64, c_int64, c_int64, c_int, c_void_p],
+    ),
+    "qf2_masked_attn_workspace_bytes": (
+        c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
+    "qf2_masked_attn": (
+        c_int,
+        [c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_int64, c_int64, c_int64, c_int64, c_int64,
+         c_int64, c_void_p, _P64, c_void_p, _P64, c_int64, POINTER(AttnMask), c_float, c_int, c_void_p, c_int64,
+         c_void_p],
+    ),
+    "qf2_masked_attn_status": (c_int, [c_void_p]),
     "qf2_quantize_rows": (
         c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p]),
     "qf2_codes_to_bf16": (c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p]),
@@ -191,6 +219,18 @@ def require_device(t) -> None:
         _device_ok[idx] = ok
     if not ok:
         raise QF2Error(f"device {idx} is not compute capability 10.0 (B200); sm_100a kernels only")
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which `device` is current (the library launches on the current device)."""
+    import torch
+
+    if device.index is None or device.index == torch.cuda.current_device():
+        return _NO_GUARD
+    return torch.cuda.device(device)
 
 
 def stream_ptr(device=None) -> c_void_p:

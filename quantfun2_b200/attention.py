@@ -20,10 +20,11 @@ import math
 import torch
 
 from . import _lib
-from ._lib import QF2Error, check, i64, ptr32, require_device, stream_ptr
+from ._lib import AttnMask, QF2Error, check, i64, on_device, ptr32, require_device, stream_ptr
 
 __all__ = ["sageattn", "sageattn_varlen", "sage_quantize", "sage_workspace_layout", "block_topk_select",
-           "blocksparse_attn", "flash_attn", "do_attn", "unpad_tokens", "pad_tokens", "ATTN"]
+           "blocksparse_attn", "flash_attn", "masked_attn", "shared_prefix_attn", "masked_attn_status", "do_attn",
+           "unpad_tokens", "pad_tokens", "ATTN"]
 
 
 def _dt(t: torch.Tensor) -> int:
@@ -238,9 +239,184 @@ def blocksparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, idx: tor
     return out
 
 
+# ------------------------------------------- masked, capped, biased attention --
+def _rows16(t: torch.Tensor) -> torch.Tensor:
+    # rows a tensor map can read: contiguous channels, 16-byte aligned, no dimension on itself
+    if t.stride(-1) != 1 or t.data_ptr() % 16 or \
+            any(n > 1 and (s % 8 or s <= 0) for s, n in zip(t.stride()[:-1], t.shape)):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+    return t
+
+
+def _int32(t: torch.Tensor, shape, what: str, device) -> torch.Tensor:
+    if t.device != device or tuple(t.shape) != tuple(shape) or t.dtype not in (torch.int32, torch.int64):
+        raise QF2Error(f"{what} must be int32 (or int64) of shape {tuple(shape)} on {device}")
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _float32(t: torch.Tensor, what: str, device) -> torch.Tensor:
+    if t.device != device or t.dtype != torch.float32:
+        raise QF2Error(f"{what} must be fp32 on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_lens, q_offset, softcap, slopes,
+            bias_table, sm_scale, tensor_layout, out):
+    require_device(q)
+    dev = q.device
+    for t, what in ((k, "k"), (v, "v"), (prefix_k, "prefix_k"), (prefix_v, "prefix_v")):
+        if t is not None and (t.dtype != q.dtype or t.device != dev):
+            raise QF2Error(f"{what} must have q's dtype and device")
+    if q.dim() != 4 or k.dim() != 4:
+        raise QF2Error("q, k and v must have four dimensions")
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (q, k, v, prefix_k, prefix_v, slopes, bias_table)):
+        raise QF2Error("masked attention is an inference op: its inputs must not require a gradient")
+    dt = _dt(q)
+    B, Hq, Sq, D, _ = _hnd(q, tensor_layout)
+    Bk, Hkv, Skv, Dk, _ = _hnd(k, tensor_layout)
+    if v.shape != k.shape or Bk != B or Dk != D or Hkv == 0 or Hq % Hkv:
+        raise QF2Error("k and v must be alike, with q's batch and head dim and a number of heads that divides q's")
+    P = 0
+    if prefix_k is not None:
+        if prefix_v is None or prefix_k.dim() != 3 or prefix_v.shape != prefix_k.shape or prefix_k.shape[2] != D:
+            raise QF2Error("prefix_k and prefix_v must be alike, three-dimensional, with q's head dim")
+        ph, P = (prefix_k.shape[0], prefix_k.shape[1]) if tensor_layout == "HND" else \
+            (prefix_k.shape[1], prefix_k.shape[0])
+        if ph != Hkv:
+            raise QF2Error("the prefix must have the own keys' heads")
+    if out is None:
+        out = torch.empty_like(q)
+        if out.stride(-1) != 1 or any(s % 8 for s in out.stride()[:-1]):
+            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1 or \
+            any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise QF2Error("out must match q's shape, dtype and device, with a contiguous last dim")
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    if P:
+        prefix_k, prefix_v = _rows16(prefix_k), _rows16(prefix_v)
+
+    m = AttnMask()
+    left, right = (-1, -1) if window is None else (int(window[0]), int(window[1]))
+    m.left, m.right = max(left, -1), max(right, -1)
+    keep = []  # converted arrays stay referenced until the launch is queued
+
+    def dev_ptr(t):
+        keep.append(t)
+        return t.data_ptr()
+
+    if kv_lens is not None:
+        m.kv_lens = dev_ptr(_int32(kv_lens, (B,), "kv_lens", dev))
+    if prefix_lens is not None:
+        m.prefix_lens = dev_ptr(_int32(prefix_lens, (B,), "prefix_lens", dev))
+    if segment_ids is not None:
+        qi, ki = segment_ids if isinstance(segment_ids, (tuple, list)) else (segment_ids, segment_ids)
+        m.q_ids = dev_ptr(_int32(qi, (B, Sq), "segment_ids of the queries", dev))
+        m.k_ids = dev_ptr(_int32(ki, (B, Skv), "segment_ids of the keys", dev))
+    if q_offset is None:
+        if kv_lens is not None and (left >= 0 or right >= 0 or slopes is not None or bias_table is not None):
+            raise QF2Error("with kv_lens, give q_offset: 0 for right-padded prompts, 'end' for the last tokens of a "
+                           "cache, or the first query's position")
+        m.q_offset = Skv - Sq
+    elif isinstance(q_offset, str):
+        if q_offset != "end":
+            raise QF2Error(f"unknown q_offset {q_offset!r}")
+        m.q_offset_mode = _lib.QF2_OFFSET_END
+    elif isinstance(q_offset, torch.Tensor):
+        m.q_offsets = dev_ptr(_int32(q_offset, (B,), "q_offset", dev))
+        m.q_offset_mode = _lib.QF2_OFFSET_ARRAY
+    else:
+        m.q_offset = int(q_offset)
+    if slopes is not None:
+        if bias_table is not None:
+            raise QF2Error("give slopes or bias_table, not both")
+        if tuple(slopes.shape) != (Hq,):
+            raise QF2Error(f"slopes must be [{Hq}]")
+        m.slopes = dev_ptr(_float32(slopes, "slopes", dev))
+    if bias_table is not None:
+        if bias_table.dim() != 2 or bias_table.shape[0] != Hq or bias_table.shape[1] % 2 == 0:
+            raise QF2Error(f"bias_table must be [{Hq}, 2 R + 1]")
+        m.bias_table = dev_ptr(_float32(bias_table, "bias_table", dev))
+        m.bias_reach = bias_table.shape[1] // 2
+    m.softcap = float(softcap or 0.0)
+    if sm_scale is None:
+        sm_scale = 1.0 / math.sqrt(D)
+    lib = _lib.load()
+    nbytes = int(lib.qf2_masked_attn_workspace_bytes(B, Hq, Hkv, Sq, Skv, P, D, int(segment_ids is not None)))
+    if nbytes < 0:
+        check(nbytes, "qf2_masked_attn_workspace_bytes")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    st = lambda t: i64(*_hnd(t, tensor_layout)[4])  # noqa: E731
+    pst = lambda t: i64(0, t.stride(0), t.stride(1)) if tensor_layout == "HND" else i64(0, t.stride(1), t.stride(0))  # noqa: E731
+    with on_device(dev):
+        check(lib.qf2_masked_attn(
+            q.data_ptr(), st(q), k.data_ptr(), st(k), v.data_ptr(), st(v), out.data_ptr(), st(out), B, Hq, Hkv, Sq,
+            Skv, D, prefix_k.data_ptr() if P else None, pst(prefix_k) if P else None,
+            prefix_v.data_ptr() if P else None, pst(prefix_v) if P else None, P, m, float(sm_scale), dt,
+            ws.data_ptr() if nbytes else None, nbytes, stream_ptr(dev)), "qf2_masked_attn")
+    return out
+
+
+def masked_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: tuple[int, int] | None = None,
+                prefix_lens: torch.Tensor | None = None, segment_ids=None, kv_lens: torch.Tensor | None = None,
+                q_offset=None, softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                bias_table: torch.Tensor | None = None, sm_scale: float | None = None, tensor_layout: str = "HND",
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """16-bit attention with masks, capped scores and a bias by distance, on the tensor cores
+    (tcgen05 kind::f16, fp32 scores, sums and outputs).  q [B, Hq, Sq, D] (HND) or
+    [B, Sq, Hq, D] (NHD); k, v with Hkv heads (Hq % Hkv == 0) and any length, 0 included;
+    D = 64, 96, 128 or 256; bf16 or fp16.  From prompts of one token to long ones, and for
+    single tokens on a cache.
+
+    Query i stands at position t = q_offset + i, key j at j.  q_offset: an int, int32 [B],
+    "end" (the queries are the last Sq of the sequence's keys), or None for Skv - Sq (with
+    kv_lens it must be given where positions matter).  A query sees a key if
+      j < kv_lens[b]                       (int32 [B]; None: all keys)
+      and (j < prefix_lens[b]              (int32 [B]; None: no prefix)
+           or t - left <= j <= t + right)  (window = (left, right), -1 open; causal: (-1, 0))
+      and their segment_ids are equal and not negative ([B, S], or a pair for queries and
+                                            keys; documents, and -1 for padding).
+    A row that sees no key is zero.  What lies in keys that no row sees is not read into the
+    result, whatever its bits.  Scores: s = sm_scale q.k (default D ** -0.5), then softcap > 0:
+    softcap * tanh(s / softcap), then minus slopes[h] * |t - j| (fp32 [Hq]) or plus
+    bias_table[h, clamp(j - t, -R, R) + R] (fp32 [Hq, 2 R + 1], R <= 1024).  Inference only.
+    `out` may be any strided view of q's shape with 16-byte aligned rows."""
+    return _masked(q, None, None, k, v, window, prefix_lens, segment_ids, kv_lens, q_offset, softcap, slopes,
+                   bias_table, sm_scale, tensor_layout, out)
+
+
+def shared_prefix_attn(q: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor, k: torch.Tensor,
+                       v: torch.Tensor, window: tuple[int, int] | None = None, kv_lens: torch.Tensor | None = None,
+                       q_offset=None, softcap: float = 0.0, slopes: torch.Tensor | None = None,
+                       bias_table: torch.Tensor | None = None, sm_scale: float | None = None,
+                       tensor_layout: str = "HND", out: torch.Tensor | None = None) -> torch.Tensor:
+    """masked_attn of a batch whose sequences begin with the same P tokens: their keys and
+    values are given once, prefix_k / prefix_v [Hkv, P, D] (HND) or [P, Hkv, D] (NHD), and
+    single tokens of many batch elements read them once.  k, v hold each element's own keys
+    behind the prefix: own key j stands at position P + j; kv_lens and q_offset count own
+    tokens.  Everything else as masked_attn."""
+    if prefix_k is None or prefix_v is None:
+        raise QF2Error("shared_prefix_attn needs prefix_k and prefix_v")
+    return _masked(q, prefix_k, prefix_v, k, v, window, None, None, kv_lens, q_offset, softcap, slopes, bias_table,
+                   sm_scale, tensor_layout, out)
+
+
+def masked_attn_status(device=None) -> None:
+    """Waits for the current stream of `device` and raises QF2Error if a masked_attn or
+    shared_prefix_attn call on it gave up a bounded wait since the last check."""
+    dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with on_device(dev):
+        check(_lib.load().qf2_masked_attn_status(stream_ptr(dev)), "masked attention")
+
+
 # ------------------------------------------------ the attention processor seam --
 # Backend of do_attn, as the reference's module global ATTN (src/models/common/attn.py:15):
-# "b200" / "sage" -> Sage INT8/FP8 attention, "flash" / "sdpa" -> bf16 tcgen05 attention.
+# "b200" / "sage" -> Sage INT8/FP8 attention, "flash" / "sdpa" -> bf16 tcgen05 attention,
+# "masked" -> 16-bit attention of masked_attn (padded batches, D up to 256).
 ATTN = "b200"
 
 
@@ -289,7 +465,8 @@ def do_attn(attn, xq: torch.Tensor, xk: torch.Tensor, xv: torch.Tensor, attn_mas
     (True = token, None = all tokens) -> [B, S, Hq, D].  ATTN "b200" / "sage": Sage INT8/FP8
     attention, through the varlen kernel on the unpadded tokens when the mask pads (no
     host sync, padded rows of the output are zero); "flash" / "sdpa": bf16 attention on the
-    tensor cores (unpadded batches).  `attn`, `apply_fn`, `batch` and `seq_len` are
+    tensor cores (unpadded batches); "masked": 16-bit attention of padded batches too, padded
+    rows zero.  `attn`, `apply_fn`, `batch` and `seq_len` are
     accepted for signature parity (the reference builds the SDPA mask with apply_fn)."""
     D = xq.shape[-1]
     if softmax_scale is None:
@@ -298,6 +475,9 @@ def do_attn(attn, xq: torch.Tensor, xk: torch.Tensor, xv: torch.Tensor, attn_mas
         if attn_mask is not None:
             raise QF2Error("the bf16 attention path takes unpadded batches; use ATTN='b200' for padded ones")
         return flash_attn(xq, xk, xv, softmax_scale, tensor_layout="NHD")
+    if ATTN == "masked":
+        ids = None if attn_mask is None else attn_mask.to(torch.int32) - 1
+        return masked_attn(xq, xk, xv, segment_ids=ids, sm_scale=softmax_scale, tensor_layout="NHD")
     if ATTN not in ("b200", "sage"):
         raise QF2Error(f"unknown ATTN backend {ATTN!r}")
     if attn_mask is None:

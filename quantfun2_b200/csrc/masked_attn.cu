@@ -1,0 +1,358 @@
+// Masked, capped and biased 16-bit attention and its shared-prefix form: entry points,
+// work split, the id ranges of key tiles and the merge of split rows.  The attention kernel
+// is in masked_attn.cuh.
+#include "masked_attn.cuh"
+
+#include <algorithm>
+
+namespace qf2 {
+namespace mattn {
+
+// Set by a kernel whose bounded wait gave up; read and cleared by qf2_masked_attn_status.
+// It lives in the module, zero when loaded, so that a call needs no launch to clear one.
+__device__ int g_status;
+
+// ------------------------------------------------------------- key ids --
+// Padded copy of a batch element's key ids (tiles of 128, pad -2) and the least and
+// greatest id of each tile: a tile is skipped where its range meets none of the rows' ids.
+// grid (nto, B), 128 threads.
+__global__ void __launch_bounds__(128) mattn_ids_kernel(const int32_t* __restrict__ ids, int Skv, int nto,
+                                                        int32_t* __restrict__ out, int2* __restrict__ rng) {
+  const int t = blockIdx.x, b = blockIdx.y, i = threadIdx.x;
+  const int j = t * kBlk + i;
+  const int v = j < Skv ? ids[(int64_t)b * Skv + j] : -2;
+  out[((int64_t)b * nto + t) * kBlk + i] = v;
+  __shared__ int2 part[4];
+  const int mn = __reduce_min_sync(0xffffffffu, v), mx = __reduce_max_sync(0xffffffffu, v);
+  if ((i & 31) == 0) part[i >> 5] = make_int2(mn, mx);
+  __syncthreads();
+  if (i == 0)
+    rng[(int64_t)b * nto + t] = make_int2(min(min(part[0].x, part[1].x), min(part[2].x, part[3].x)),
+                                          max(max(part[0].y, part[1].y), max(part[2].y, part[3].y)));
+}
+
+// ----------------------------------------------------------- merge splits --
+// out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits of one row (a split
+// that saw nothing has m = -inf and is not read).  One CTA per (batch, token, head) row:
+// D / 4 threads cover the row in 16-byte pieces, 128 / (D / 4) such groups take every
+// second, fifth, ... split, and the groups are added in a fixed order.
+template <int D, bool F16>
+__global__ void __launch_bounds__(128) mattn_merge_kernel(const float* __restrict__ part_o,
+                                                          const float2* __restrict__ part_ml, int ns, int64_t R,
+                                                          uint8_t* __restrict__ out, S3 os, int Sq, int Hq) {
+  constexpr int C = D / 4, NG = 128 / C;
+  __shared__ float wgt[kMaxSplits];
+  __shared__ float4 acc[NG][C];
+  __shared__ float redm[4], redl[4];
+  const int64_t r = blockIdx.x;
+  const int tid = threadIdx.x;
+  float m = -INFINITY;
+  for (int s = tid; s < ns; s += 128) m = fmaxf(m, part_ml[s * R + r].x);
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+  if ((tid & 31) == 0) redm[tid >> 5] = m;
+  __syncthreads();
+  const float M = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
+  float l = 0.f;
+  for (int s = tid; s < ns; s += 128) {
+    const float2 ml = part_ml[s * R + r];
+    // a NaN sum (its maximum may be -inf: NaN scores leave it) goes on to the output
+    const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
+    wgt[s] = w;
+    l += w * ml.y;
+  }
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+  if ((tid & 31) == 0) redl[tid >> 5] = l;
+  __syncthreads();
+  l = (redl[0] + redl[1]) + (redl[2] + redl[3]);
+  const int g = tid / C, c = tid % C;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (g < NG) {
+#pragma unroll 4
+    for (int s = g; s < ns; s += NG) {
+      const float w = wgt[s];
+      if (w != 0.f) {
+        const float4 o = *reinterpret_cast<const float4*>(part_o + ((int64_t)s * R + r) * D + 4 * c);
+        a.x = fmaf(w, o.x, a.x); a.y = fmaf(w, o.y, a.y); a.z = fmaf(w, o.z, a.z); a.w = fmaf(w, o.w, a.w);
+      }
+    }
+    acc[g][c] = a;
+  }
+  __syncthreads();
+  if (tid < C) {
+    for (int k = 1; k < NG; ++k) {
+      const float4 o = acc[k][tid];
+      a.x += o.x; a.y += o.y; a.z += o.z; a.w += o.w;
+    }
+    const bool zero = l == 0.f;
+    const float inv = zero ? 0.f : 1.0f / l;
+    const int h = (int)(r % Hq);
+    const int64_t bt = r / Hq;
+    const int64_t tok = bt % Sq, b = bt / Sq;
+    uint2 w;
+    w.x = zero ? 0u : pack16<F16>(a.x * inv, a.y * inv);
+    w.y = zero ? 0u : pack16<F16>(a.z * inv, a.w * inv);
+    *reinterpret_cast<uint2*>(out + 2 * (b * os.b + (int64_t)h * os.h + tok * os.s + 4 * tid)) = w;
+  }
+}
+
+// ------------------------------------------------------------------- plan --
+struct Plan {
+  int nt, G, T, Nb[2], qtiles[2], splits[2], ntp, nto, merged;
+  int64_t items[2];  // CTAs of own and prefix items, splits counted
+  int64_t ids_off, rng_off, ml_off, o_off, bytes;
+};
+
+static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P, int64_t D,
+                     bool ids) {
+  if (D != 64 && D != 96 && D != 128 && D != 256) return QF2_ERR_SHAPE;
+  if (B < 0 || Sq < 0 || Skv < 0 || P < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return QF2_ERR_SHAPE;
+  if (B > 65535 || Hq > 65535 || Sq > (1 << 20)) return QF2_ERR_SHAPE;
+  const int64_t ntp = (P + kBlk - 1) / kBlk, nto = (Skv + kBlk - 1) / kBlk;
+  if (P > (1 << 20) || Skv > (1 << 20) || ntp + nto > kMaxTiles) return QF2_ERR_SHAPE;
+  *p = Plan{};
+  p->ntp = (int)ntp;
+  p->nto = (int)nto;
+  const int64_t group = Hq / Hkv;
+  p->Nb[0] = p->Nb[1] = 1;
+  p->splits[0] = p->splits[1] = 1;
+  p->merged = 1;
+  p->G = 1;
+  if (B == 0 || Sq == 0) return QF2_OK;
+  // two query tiles per CTA where that still fills the SMs
+  const bool two = D != 256 && Sq > kBlk && B * Hq * ((Sq + 2 * kBlk - 1) / (2 * kBlk)) >= kSms;
+  int64_t hw = Hq;
+  if (two) {
+    p->nt = 2;
+    p->T = kBlk;
+    p->qtiles[0] = (int)((Sq + 2 * kBlk - 1) / (2 * kBlk));
+  } else {
+    p->nt = 1;
+    // pack a group's query heads where that makes fewer tiles
+    const int64_t tp = group <= kBlk ? std::min<int64_t>(Sq, kBlk / group) : 0;
+    if (group > 1 && tp > 0 && Hkv * ((Sq + tp - 1) / tp) < Hq * ((Sq + kBlk - 1) / kBlk)) {
+      p->G = (int)group;
+      p->T = (int)tp;
+      hw = Hkv;
+    } else {
+      p->T = (int)std::min<int64_t>(Sq, kBlk);
+    }
+    p->qtiles[0] = (int)((Sq + p->T - 1) / p->T);
+    // rows of several batch elements share a prefix item where two or more fit a tile
+    if (P > 0 && p->T == Sq) {
+      const int64_t nb = std::min<int64_t>(B, kBlk / ((int64_t)p->G * p->T));
+      if (nb > 1) {
+        p->merged = 0;
+        p->Nb[1] = (int)nb;
+        p->qtiles[1] = (int)((B + nb - 1) / nb);
+      }
+    }
+  }
+  const int64_t n0 = B * hw * p->qtiles[0], n1 = hw * p->qtiles[1];
+  const int64_t t0 = (p->merged ? ntp : 0) + nto, t1 = p->merged ? 0 : ntp;
+  if (p->nt == 1) {
+    // Split the key tiles so that the waves of CTAs are short: a wave costs its longest CTA
+    // (about 1.4 us a tile of head dim 128 and 4 us to start and end); a split also writes
+    // and reads fp32 partial rows and launches the merge (about 4 us).
+    const double tile_us = 0.5 + 0.9 * (double)D / 128.0;
+    const double row_us = (double)(B * Sq * Hq) * (double)D * 8.0 / 5.0e6;
+    double best = 1e30;
+    for (int64_t n = 1; n <= kSms; ++n) {
+      const int64_t len = std::max<int64_t>(1, (std::max(t0, t1) + n - 1) / n);
+      const int64_t s0 = std::max<int64_t>(1, (t0 + len - 1) / len), s1 = std::max<int64_t>(1, (t1 + len - 1) / len);
+      if (s0 + s1 > kMaxSplits) break;
+      const int64_t ctas = n0 * s0 + n1 * s1;
+      const int64_t parts = s0 + (n1 > 0 ? s1 : 0);
+      double c = (double)((ctas + kSms - 1) / kSms) * ((double)len * tile_us + 4.0);
+      if (parts > 1) c += 4.0 + row_us * (double)parts;
+      if (c < best) {
+        best = c;
+        p->splits[0] = (int)s0;
+        p->splits[1] = (int)s1;
+      }
+      if (len == 1) break;
+    }
+  }
+  p->items[0] = n0 * p->splits[0];
+  p->items[1] = n1 * p->splits[1];
+  if (p->items[0] + p->items[1] > 0x7fffffffll) return QF2_ERR_SHAPE;
+  const int64_t parts = p->splits[0] + (n1 > 0 ? p->splits[1] : 0), R = B * Sq * Hq;
+  auto up = [](int64_t x) { return (x + 255) & ~255ll; };
+  int64_t off = 0;
+  p->ids_off = off;
+  if (ids) off += up(B * nto * kBlk * 4);
+  p->rng_off = off;
+  if (ids) off += up(B * nto * 8);
+  p->ml_off = off;
+  if (parts > 1) off += up(parts * R * 8);
+  p->o_off = off;
+  if (parts > 1) off += up(parts * R * D * 4);
+  if (parts > 1 && R > 0x7fffffffll) return QF2_ERR_SHAPE;  // the merge's grid
+  p->bytes = off;
+  return QF2_OK;
+}
+
+static bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// strides {batch, head, seq}; a dimension of one element has no stride to speak of
+static int check_strides(const int64_t* st, int64_t B, int64_t H, int64_t S) {
+  const int64_t n[3] = {B, H, S};
+  for (int i = 0; i < 3; ++i)
+    if (n[i] > 1 && (st[i] % 8 || st[i] <= 0 || st[i] >= (1ll << 38))) return QF2_ERR_ALIGN;
+  return QF2_OK;
+}
+
+// rows of D channels; dims (D, d1, d2, d3) with element strides
+static bool make_map(CUtensorMap* m, const void* base, int64_t D, const int64_t n[3], const int64_t st[3],
+                     const uint32_t box[3], bool f16) {
+  const uint64_t dims[4] = {(uint64_t)D, (uint64_t)n[0], (uint64_t)n[1], (uint64_t)n[2]};
+  uint64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = n[i] > 1 ? (uint64_t)st[i] * 2 : (uint64_t)D * 2;
+  const uint32_t bx[4] = {64, box[0], box[1], box[2]};
+  return qf2_make_tmap_4d(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, base, dims,
+                          strides, bx);
+}
+
+template <bool F16>
+static void launch_merge(const Args& a, int64_t D, int parts, int64_t R, cudaStream_t s) {
+  const unsigned grid = (unsigned)R;
+  uint8_t* out = reinterpret_cast<uint8_t*>(a.out);
+  if (D == 64) mattn_merge_kernel<64, F16><<<grid, 128, 0, s>>>(a.part_o, a.part_ml, parts, R, out, a.os, a.Sq, a.Hq);
+  else if (D == 96) mattn_merge_kernel<96, F16><<<grid, 128, 0, s>>>(a.part_o, a.part_ml, parts, R, out, a.os, a.Sq, a.Hq);
+  else if (D == 128) mattn_merge_kernel<128, F16><<<grid, 128, 0, s>>>(a.part_o, a.part_ml, parts, R, out, a.os, a.Sq, a.Hq);
+  else mattn_merge_kernel<256, F16><<<grid, 128, 0, s>>>(a.part_o, a.part_ml, parts, R, out, a.os, a.Sq, a.Hq);
+}
+
+}  // namespace mattn
+}  // namespace qf2
+
+using namespace qf2::mattn;
+
+extern "C" int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv,
+                                                   int64_t P, int64_t D, int with_ids) {
+  Plan p;
+  const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids != 0);
+  return st != QF2_OK ? (int64_t)st : p.bytes;
+}
+
+extern "C" int qf2_masked_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                               const void* v, const int64_t* v_strides, void* out, const int64_t* out_strides,
+                               int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D,
+                               const void* prefix_k, const int64_t* prefix_k_strides, const void* prefix_v,
+                               const int64_t* prefix_v_strides, int64_t P, const qf2_attn_mask* mask, float sm_scale,
+                               int dtype, void* workspace, int64_t workspace_bytes, qf2_stream_t stream) {
+  if (dtype != QF2_BF16 && dtype != QF2_F16) return QF2_ERR_DTYPE;
+  if (!mask) return QF2_ERR_ARG;
+  const qf2_attn_mask& M = *mask;
+  const bool ids = M.k_ids != nullptr;
+  Plan p;
+  int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids);
+  if (st != QF2_OK) return st;
+  if (B == 0 || Sq == 0) return QF2_OK;
+  if (!q || !q_strides || !out || !out_strides) return QF2_ERR_ARG;
+  if (Skv > 0 && (!k || !k_strides || !v || !v_strides)) return QF2_ERR_ARG;
+  if (P > 0 && (!prefix_k || !prefix_k_strides || !prefix_v || !prefix_v_strides)) return QF2_ERR_ARG;
+  if ((M.q_ids != nullptr) != ids || (ids && P > 0)) return QF2_ERR_ARG;
+  if (M.q_offset_mode < QF2_OFFSET_CONST || M.q_offset_mode > QF2_OFFSET_END ||
+      (M.q_offset_mode == QF2_OFFSET_ARRAY && !M.q_offsets))
+    return QF2_ERR_ARG;
+  if (M.slopes && M.bias_table) return QF2_ERR_ARG;
+  if (M.bias_table && (M.bias_reach < 0 || M.bias_reach > kMaxReach)) return QF2_ERR_SHAPE;
+  if (!(M.softcap >= 0.f) || !(sm_scale > 0.f) || isinf(M.softcap) || isinf(sm_scale)) return QF2_ERR_ARG;
+  if (!al16(q) || !al16(out) || (Skv > 0 && (!al16(k) || !al16(v))) || (P > 0 && (!al16(prefix_k) || !al16(prefix_v))))
+    return QF2_ERR_ALIGN;
+  st = check_strides(q_strides, B, Hq, Sq);
+  if (st == QF2_OK) st = check_strides(out_strides, B, Hq, Sq);
+  if (st == QF2_OK && Skv > 0) st = check_strides(k_strides, B, Hkv, Skv);
+  if (st == QF2_OK && Skv > 0) st = check_strides(v_strides, B, Hkv, Skv);
+  if (st == QF2_OK && P > 0) st = check_strides(prefix_k_strides, 1, Hkv, P);
+  if (st == QF2_OK && P > 0) st = check_strides(prefix_v_strides, 1, Hkv, P);
+  if (st != QF2_OK) return st;
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || !al16(workspace))) return QF2_ERR_WORKSPACE;
+
+  const bool f16 = dtype == QF2_F16;
+  Maps m;
+  {
+    const int64_t n[3] = {Hq, Sq, B}, s[3] = {q_strides[1], q_strides[2], q_strides[0]};
+    const uint32_t box[3] = {(uint32_t)p.G, (uint32_t)p.T, 1}, box1[3] = {(uint32_t)p.G, (uint32_t)p.T, (uint32_t)p.Nb[1]};
+    if (!make_map(&m.q, q, D, n, s, box, f16)) return QF2_ERR_ALIGN;
+    m.q1 = m.q;
+    if (p.Nb[1] > 1 && !make_map(&m.q1, q, D, n, s, box1, f16)) return QF2_ERR_ALIGN;
+  }
+  m.k = m.v = m.pk = m.pv = m.q;  // never loaded through where there are no such keys
+  const uint32_t kbox[3] = {(uint32_t)kBlk, 1, 1};
+  if (Skv > 0) {
+    const int64_t n[3] = {Skv, Hkv, B};
+    const int64_t sk[3] = {k_strides[2], k_strides[1], k_strides[0]}, sv[3] = {v_strides[2], v_strides[1], v_strides[0]};
+    if (!make_map(&m.k, k, D, n, sk, kbox, f16) || !make_map(&m.v, v, D, n, sv, kbox, f16)) return QF2_ERR_ALIGN;
+  }
+  if (P > 0) {
+    const int64_t n[3] = {P, Hkv, 1};
+    const int64_t sk[3] = {prefix_k_strides[2], prefix_k_strides[1], 0}, sv[3] = {prefix_v_strides[2], prefix_v_strides[1], 0};
+    if (!make_map(&m.pk, prefix_k, D, n, sk, kbox, f16) || !make_map(&m.pv, prefix_v, D, n, sv, kbox, f16))
+      return QF2_ERR_ALIGN;
+  }
+
+  void* status = nullptr;
+  QF2_CUDA_CHECK(cudaGetSymbolAddress(&status, g_status));
+  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+  const bool split = p.splits[0] > 1 || p.items[1] > 0;
+  Args a{};
+  a.out = out;
+  a.os = S3{out_strides[0], out_strides[1], out_strides[2]};
+  a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Sq = (int)Sq; a.Skv = (int)Skv; a.P = (int)P;
+  a.ntp = p.ntp; a.nto = p.nto; a.group = (int)(Hq / Hkv);
+  a.G = p.G; a.T = p.T;
+  for (int i = 0; i < 2; ++i) { a.Nb[i] = p.Nb[i]; a.qtiles[i] = p.qtiles[i]; a.splits[i] = p.splits[i]; }
+  a.items1 = (int)p.items[1];
+  a.merged = p.merged;
+  a.part_o = split ? reinterpret_cast<float*>(ws + p.o_off) : nullptr;
+  a.part_ml = split ? reinterpret_cast<float2*>(ws + p.ml_off) : nullptr;
+  a.kv_lens = M.kv_lens;
+  a.prefix_lens = M.prefix_lens;
+  a.q_off = M.q_offsets;
+  a.q_off_mode = M.q_offset_mode;
+  const int64_t far = 1ll << 29;
+  a.q_off_const = (int)std::min(std::max(M.q_offset, -far), far);
+  a.left = M.left < 0 ? -1 : (int)std::min(M.left, far);
+  a.right = M.right < 0 ? -1 : (int)std::min(M.right, far);
+  a.q_ids = M.q_ids;
+  a.k_ids = ids ? reinterpret_cast<int32_t*>(ws + p.ids_off) : nullptr;
+  a.k_rng = ids ? reinterpret_cast<int2*>(ws + p.rng_off) : nullptr;
+  const double l2e = 1.4426950408889634;
+  a.scale = (float)((double)sm_scale * l2e);
+  if (M.softcap > 0.f) {
+    a.cap_in = (float)(2.0 * (double)sm_scale / (double)M.softcap * l2e);
+    a.cap_out = (float)((double)M.softcap * l2e);
+  }
+  a.slopes = M.slopes;
+  a.table = M.bias_table;
+  a.reach = (int)M.bias_reach;
+  a.status = reinterpret_cast<int*>(status);
+  const bool score = M.softcap > 0.f || M.slopes || M.bias_table;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (ids && p.nto > 0) {
+    mattn_ids_kernel<<<dim3((unsigned)p.nto, (unsigned)B), 128, 0, s>>>(
+        M.k_ids, (int)Skv, p.nto, reinterpret_cast<int32_t*>(ws + p.ids_off), reinterpret_cast<int2*>(ws + p.rng_off));
+    QF2_LAUNCH_CHECK();
+  }
+  const unsigned grid = (unsigned)(p.items[0] + p.items[1]);
+  cudaError_t e;
+  if (D == 64) e = launch_d64(m, a, grid, p.nt, f16, score, s);
+  else if (D == 96) e = launch_d96(m, a, grid, p.nt, f16, score, s);
+  else if (D == 128) e = launch_d128(m, a, grid, p.nt, f16, score, s);
+  else e = launch_d256(m, a, grid, p.nt, f16, score, s);
+  QF2_CUDA_CHECK(e);
+  if (split) {
+    const int parts = p.splits[0] + (p.items[1] > 0 ? p.splits[1] : 0);
+    if (f16) launch_merge<true>(a, D, parts, B * Sq * Hq, s);
+    else launch_merge<false>(a, D, parts, B * Sq * Hq, s);
+    QF2_LAUNCH_CHECK();
+  }
+  return QF2_OK;
+}
+
+extern "C" int qf2_masked_attn_status(qf2_stream_t stream) {
+  void* p = nullptr;
+  QF2_CUDA_CHECK(cudaGetSymbolAddress(&p, g_status));
+  return qf2_workspace_status(p, stream);
+}

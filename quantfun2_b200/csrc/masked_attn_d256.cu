@@ -1,0 +1,14 @@
+// Masked attention at head dim 256: one query tile per CTA (its fp32 output fills half of
+// tensor memory).
+#include "masked_attn.cuh"
+
+namespace qf2 {
+namespace mattn {
+
+cudaError_t launch_d256(const Maps& m, const Args& a, unsigned grid, int nt, bool f16, bool score, cudaStream_t s) {
+  (void)nt;
+  return launch_nt<256, 1>(m, a, grid, f16, score, s);
+}
+
+}  // namespace mattn
+}  // namespace qf2

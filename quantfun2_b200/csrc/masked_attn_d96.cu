@@ -1,0 +1,12 @@
+// Masked attention at head dim 96.
+#include "masked_attn.cuh"
+
+namespace qf2 {
+namespace mattn {
+
+cudaError_t launch_d96(const Maps& m, const Args& a, unsigned grid, int nt, bool f16, bool score, cudaStream_t s) {
+  return nt == 2 ? launch_nt<96, 2>(m, a, grid, f16, score, s) : launch_nt<96, 1>(m, a, grid, f16, score, s);
+}
+
+}  // namespace mattn
+}  // namespace qf2

@@ -12,6 +12,12 @@ B200.
   rmsnorm_apply(x, weight, eps)        -> Tensor              __init__.py:73-80
   inplace_softmax(x, dim=-1)           -> x                   __init__.py:83-87
   topk_attn(xq, xk, xv, mask, ...)     -> (out, POS_DICT)     __init__.py:146-195 (block form)
+
+and beside rope_apply, for text encoders (no counterpart in the reference's kernel seam):
+
+  rotary_apply(xq, xk, positions, inv_freq, ...)   -> (xq_out, xk_out)   from positions
+  rotary_apply_(xq, xk, positions, inv_freq, ...)  -> (xq, xk) in place
+  rotary_inv_freq(rotary_dim, base, scaling, ...)  -> fp64 frequencies
 """
 from __future__ import annotations
 
@@ -20,13 +26,16 @@ import math
 import torch
 
 from . import _lib
-from ._lib import QF2Error, check, dtype_code, i64, require_device, stream_ptr
+from ._lib import QF2Error, check, dtype_code, i64, on_device, require_device, stream_ptr
 
 __all__ = [
     "copy_chunks",
     "implemented_as",
     "rope_apply",
     "rope_apply_",
+    "rotary_apply",
+    "rotary_apply_",
+    "rotary_inv_freq",
     "rmsnorm_apply",
     "inplace_softmax",
     "topk_attn",
@@ -112,6 +121,103 @@ def rope_apply_(xq: torch.Tensor, xk: torch.Tensor, freqs_cis: torch.Tensor, fp1
     """Triton-body semantics (src/kernels/triton/rope.py:83-134): rotates in place and
     returns the same tensors; cos/sin rounded to fp16 as rope_triton does."""
     _rope(xq, xk, freqs_cis, xq, xk, fp16_trig=fp16_trig)
+    return xq, xk
+
+
+def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                    original_length: int = 4096, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                    device=None) -> torch.Tensor:
+    """fp64 frequencies [rotary_dim / 2] of rotary_apply, base^(-2p / rotary_dim), for contexts
+    `factor` times longer than `original_length` by one of
+      "none"      as they are
+      "linear"    all divided by factor (positions interpolated)
+      "ntk"       base * factor^(r / (r - 2)): the slowest pair divided by factor, the
+                  fastest kept
+      "by_parts"  a pair that turns more than beta_fast times over original_length is kept,
+                  one that turns less than beta_slow times is divided by factor, a linear
+                  ramp over the turns in between (0.1 ln(factor) + 1 is the customary
+                  `magnitude` of rotary_apply beside it)"""
+    r = int(rotary_dim)
+    if r < 2 or r % 2:
+        raise QF2Error(f"rotary_dim must be even and positive, got {rotary_dim}")
+    if not (base > 0 and factor > 0):
+        raise QF2Error("base and factor must be positive")
+    if scaling not in ("none", "linear", "ntk", "by_parts"):
+        raise QF2Error(f"unknown rotary scaling {scaling!r}")
+    if scaling == "ntk" and r > 2:
+        base = base * factor ** (r / (r - 2))
+    f = float(base) ** (-torch.arange(0, r, 2, dtype=torch.float64) / r)
+    if scaling == "linear" or (scaling == "ntk" and r == 2):
+        f = f / factor
+    elif scaling == "by_parts":
+        if not beta_fast > beta_slow:
+            raise QF2Error("beta_fast must be greater than beta_slow")
+        turns = original_length * f / (2 * math.pi)
+        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0.0, 1.0)
+        f = f * keep + f / factor * (1 - keep)
+    return f.to(device) if device is not None else f
+
+
+def _rotary(xq, xk, positions, inv_freq, out_q, out_k, layout, magnitude, inverse):
+    require_device(xq)
+    if layout not in ("half", "interleaved"):
+        raise QF2Error(f"unknown rotary layout {layout!r}")
+    if xq.dim() != 4 or xq.stride(-1) != 1 or out_q.stride(-1) != 1:
+        raise QF2Error("rotary_apply expects [B, S, H, D] tensors with a contiguous last dim")
+    B, S, Hq, D = xq.shape
+    dt = dtype_code(xq.dtype)
+    dev = xq.device
+    if xk is not None and (xk.dim() != 4 or xk.shape[0] != B or xk.shape[1] != S or xk.shape[3] != D
+                           or xk.dtype != xq.dtype or xk.device != dev or xk.stride(-1) != 1 or out_k.stride(-1) != 1):
+        raise QF2Error("xk must match xq in batch, seq, head_dim, dtype and device, with a contiguous last dim")
+    if torch.is_grad_enabled() and (xq.requires_grad or (xk is not None and xk.requires_grad)):
+        raise QF2Error("rotary_apply is an inference op: its inputs must not require a gradient")
+    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != dev or \
+            not inv_freq.is_contiguous():
+        raise QF2Error("inv_freq must be a contiguous fp64 vector on the tensors' device")
+    if positions.device != dev or positions.dtype not in (torch.int32, torch.int64):
+        raise QF2Error("positions must be int32 or int64 on the tensors' device")
+    if positions.shape == (S,):
+        ps = (0, positions.stride(0))
+    elif positions.shape == (B, S) or positions.shape == (1, S):
+        ps = (positions.stride(0) if positions.shape[0] > 1 else 0, positions.stride(1))
+    else:
+        raise QF2Error(f"positions must be [{S}] or [{B}, {S}], got {tuple(positions.shape)}")
+    st = lambda t: i64(t.stride(0), t.stride(1), t.stride(2))  # noqa: E731
+    has_k = xk is not None
+    with on_device(dev):
+        check(_lib.load().qf2_rotary_apply(
+            xq.data_ptr(), out_q.data_ptr(), Hq, st(xq), st(out_q),
+            xk.data_ptr() if has_k else None, out_k.data_ptr() if has_k else None, xk.shape[2] if has_k else 0,
+            st(xk) if has_k else None, st(out_k) if has_k else None, positions.data_ptr(), i64(*ps),
+            int(positions.dtype == torch.int64), inv_freq.data_ptr(), 2 * inv_freq.shape[0],
+            _lib.QF2_ROTARY_HALF if layout == "half" else _lib.QF2_ROTARY_INTERLEAVED, float(magnitude),
+            int(bool(inverse)), B, S, D, dt, stream_ptr(dev)), "qf2_rotary_apply")
+
+
+def rotary_apply(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                 layout: str = "half", magnitude: float = 1.0, inverse: bool = False):
+    """Rotary positions of xq [B, S, H, D] and xk [B, S, Hkv, D] (or None) at `positions`
+    (int32 / int64 [S], [1, S] or [B, S]): pair p turns by positions * inv_freq[p] (fp64
+    [r / 2], from rotary_inv_freq) and is scaled by `magnitude`.  layout "half" pairs channel
+    p with p + r / 2, "interleaved" 2p with 2p + 1; channels from r on are copied.
+    inverse=True turns back (the transposed rotation: a cached key moves to another position
+    by one inverse and one plain call).  Returns new tensors.  fp32, fp16 or bf16; angles are
+    formed in 64 bits, so far positions keep fp32 accuracy."""
+    out_q = torch.empty_like(xq)
+    out_k = torch.empty_like(xk) if xk is not None else None
+    _rotary(xq, xk, positions, inv_freq, out_q, out_k, layout, magnitude, inverse)
+    return out_q, out_k
+
+
+def rotary_apply_(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
+                  layout: str = "half", magnitude: float = 1.0, inverse: bool = False):
+    """rotary_apply in place; returns the same tensors.  Tensors whose elements share memory
+    (expanded views) are refused."""
+    for t in (xq, xk):
+        if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise QF2Error("rotary_apply_ needs tensors whose elements do not share memory")
+    _rotary(xq, xk, positions, inv_freq, xq, xk, layout, magnitude, inverse)
     return xq, xk
 
 

@@ -1,0 +1,439 @@
+"""GPU: masked, capped and biased attention and its shared-prefix form against the 64-bit
+formula (oracle.text), with the elementwise bound derived there."""
+import math
+
+import pytest
+import torch
+
+from oracle import text as ot
+
+pytestmark = pytest.mark.gpu
+
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def _inputs(dev, B, Sq, Skv, Hq, Hkv, D, dtype, seed=0, P=0, amp=1.5):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, device=dev, generator=g)  # noqa: E731
+    q = (r(B, Sq, Hq, D) * amp).to(dtype)
+    k = (r(B, Skv, Hkv, D) + 0.5 * r(1, 1, Hkv, D)).to(dtype)
+    v = r(B, Skv, Hkv, D).to(dtype)
+    if P:
+        return q, k, v, r(P, Hkv, D).to(dtype), r(P, Hkv, D).to(dtype)
+    return q, k, v
+
+
+def _compare(out, q, k, v, offsets=None, kv_lens=None, rows=None, **kw):
+    """out against the oracle on all rows, or on the listed ones."""
+    from quantfun2_b200 import attention as A
+
+    A.masked_attn_status()
+    Sq, Skv = q.shape[1], k.shape[1]
+    if rows is not None:
+        base = [Skv - Sq if offsets is None else int(offsets[b]) for b in range(q.shape[0])]
+        refs = []
+        for i in rows:
+            sub = dict(kw)
+            if kw.get("q_ids") is not None:
+                sub["q_ids"] = kw["q_ids"][:, i:i + 1]
+            refs.append(ot.attention(q[:, i:i + 1], k, v, offsets=[o + i for o in base], kv_lens=kv_lens, **sub))
+        ref, mag, keys = (torch.cat([r[n] for r in refs], 1) for n in range(3))
+        out = out[:, rows]
+    else:
+        ref, mag, keys = ot.attention(q, k, v, offsets=offsets, kv_lens=kv_lens, **kw)
+    v_max = v[torch.isfinite(v)].abs().max().double().item() if v.numel() else 0.0
+    if kw.get("prefix_v") is not None:
+        v_max = max(v_max, kw["prefix_v"].abs().max().double().item())
+    tol = ot.attention_bound(ref, mag, keys, q.dtype, v_max)
+    err = (out.double() - ref).abs()
+    assert torch.isfinite(out).all()
+    assert (err <= tol).all(), f"{(err / tol).max().item():.3f} of the bound, {err.max().item():.4g} off"
+    assert not out[(keys == 0)].any()
+
+
+def _window(causal, left=-1):
+    return (left, 0 if causal else -1)
+
+
+# lengths around the tile edges, head dims, groups, both directions, both types
+@pytest.mark.parametrize("B,Sq,Hq,Hkv,D,dtype,causal", [
+    (1, 1, 1, 1, 64, BF16, True), (2, 1, 3, 1, 128, FP16, False), (1, 2, 4, 2, 96, BF16, True),
+    (2, 77, 4, 4, 64, FP16, True), (1, 127, 2, 2, 128, BF16, True), (1, 128, 3, 1, 256, BF16, True),
+    (1, 129, 2, 1, 64, BF16, False), (2, 200, 4, 1, 256, FP16, True), (1, 257, 6, 2, 96, FP16, True),
+    (1, 300, 2, 2, 128, FP16, False), (1, 385, 5, 5, 128, BF16, True), (1, 33, 40, 1, 128, BF16, True),
+    (1, 3, 130, 1, 64, BF16, True),
+])
+def test_dense_and_causal(cuda, B, Sq, Hq, Hkv, D, dtype, causal):
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, B, Sq, Sq, Hq, Hkv, D, dtype, seed=Sq)
+    out = A.masked_attn(q, k, v, window=_window(causal), tensor_layout="NHD")
+    _compare(out, q, k, v, window=_window(causal))
+    hnd = A.masked_attn(q.transpose(1, 2).contiguous(), k.transpose(1, 2).contiguous(), v.transpose(1, 2).contiguous(),
+                        window=_window(causal))
+    assert torch.equal(hnd.transpose(1, 2), out)
+
+
+# grids that fill the SMs: two query tiles per CTA (heads * batch large), spot rows
+@pytest.mark.parametrize("B,S,Hq,Hkv,D,dtype,window", [
+    (4, 300, 40, 8, 64, BF16, (-1, 0)), (3, 513, 24, 8, 96, FP16, (-1, -1)), (8, 640, 24, 24, 128, BF16, (100, 0)),
+    (4, 1000, 24, 8, 128, BF16, (-1, 0)), (2, 1281, 24, 8, 128, FP16, (130, 40)), (13, 257, 12, 12, 64, FP16, (0, 0)),
+])
+def test_two_tile_grids(cuda, B, S, Hq, Hkv, D, dtype, window):
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, B, S, S, Hq, Hkv, D, dtype, seed=S)
+    out = A.masked_attn(q, k, v, window=window, tensor_layout="NHD")
+    rows = sorted({0, 1, 31, 127, 128, 129, 255, 256, S // 2, S - 2, S - 1})
+    _compare(out, q, k, v, rows=rows, window=window)
+
+
+@pytest.mark.parametrize("Hq,two", [(2, False), (80, True)])
+@pytest.mark.parametrize("D,dtype", [(64, FP16), (128, BF16)])
+def test_scores_capped_and_biased(cuda, Hq, two, D, dtype):
+    from quantfun2_b200 import attention as A
+
+    B, S = 2, 290
+    q, k, v = _inputs(cuda, B, S, S, Hq, Hq // 2, D, dtype, seed=5, amp=4.0)
+    slopes = torch.rand(Hq, device=cuda) * 0.2
+    rows = [0, 3, 127, 128, 200, 289]
+    for R in (0, 1, 40, 700, 1024):
+        table = torch.randn(Hq, 2 * R + 1, device=cuda)
+        out = A.masked_attn(q, k, v, bias_table=table, tensor_layout="NHD")
+        _compare(out, q, k, v, rows=rows, bias_table=table)
+    for cap in (2.0, 50.0):
+        out = A.masked_attn(q, k, v, window=(-1, 0), softcap=cap, tensor_layout="NHD")
+        _compare(out, q, k, v, rows=rows, window=(-1, 0), softcap=cap)
+        out = A.masked_attn(q, k, v, window=(50, 20), softcap=cap, slopes=slopes, sm_scale=0.3, tensor_layout="NHD")
+        _compare(out, q, k, v, rows=rows, window=(50, 20), softcap=cap, slopes=slopes, sm_scale=0.3)
+    out = A.masked_attn(q, k, v, slopes=slopes, tensor_layout="NHD")
+    _compare(out, q, k, v, rows=rows, slopes=slopes)
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(2, 1), (80, 40)])
+def test_bias_of_the_lowest_value_and_minus_infinity(cuda, Hq, Hkv):
+    """A table of the type's lowest value everywhere weighs all keys alike; minus infinity
+    hides keys; a row that has only such keys is zero."""
+    from quantfun2_b200 import attention as A
+
+    B, S, D = 2, 200, 64
+    q, k, v = _inputs(cuda, B, S, S, Hq, Hkv, D, BF16, seed=8)
+    low = torch.full((Hq, 3), torch.finfo(torch.float32).min, device=cuda)
+    out = A.masked_attn(q, k, v, bias_table=low, tensor_layout="NHD")
+    even = v.double().mean(1, keepdim=True).repeat_interleave(Hq // Hkv, 2).expand(B, S, Hq, D)
+    mag = v.double().abs().mean(1, keepdim=True).repeat_interleave(Hq // Hkv, 2).expand(B, S, Hq, D)
+    keys = torch.full((B, S), S, device=cuda)
+    assert ((out.double() - even).abs() <= ot.attention_bound(even, mag, keys, BF16, 0.0)).all()
+    past = torch.zeros(Hq, 3, device=cuda)
+    past[:, 1:] = -math.inf                       # only keys strictly before the query
+    out = A.masked_attn(q, k, v, bias_table=past, tensor_layout="NHD")
+    _compare(out, q, k, v, rows=[1, 2, 100, 199], offsets=[-1] * B, window=(-1, 0))  # the same mask by a band
+    assert not out[:, 0].any()
+
+
+def test_prefix_window_and_lengths(cuda):
+    from quantfun2_b200 import attention as A
+
+    B, S, Hq, Hkv, D = 5, 270, 4, 2, 96
+    q, k, v = _inputs(cuda, B, S, S, Hq, Hkv, D, BF16, seed=9)
+    pre = torch.tensor([0, 1, 128, 200, 999], device=cuda)
+    lens = torch.tensor([270, 0, 1, 129, 500], device=cuda, dtype=torch.int32)
+    out = A.masked_attn(q, k, v, window=(-1, 0), prefix_lens=pre, tensor_layout="NHD")
+    _compare(out, q, k, v, window=(-1, 0), prefix_lens=pre.tolist())
+    out = A.masked_attn(q, k, v, window=(30, 0), prefix_lens=pre, kv_lens=lens, q_offset=0, tensor_layout="NHD")
+    _compare(out, q, k, v, window=(30, 0), prefix_lens=pre.tolist(), kv_lens=lens.tolist(), offsets=[0] * B)
+    # without a band the lengths alone matter and no offset is needed
+    out = A.masked_attn(q, k, v, kv_lens=lens, tensor_layout="NHD")
+    _compare(out, q, k, v, kv_lens=lens.tolist())
+
+
+def test_offsets(cuda):
+    from quantfun2_b200 import attention as A
+
+    B, Sq, Skv, Hq, D = 4, 40, 300, 2, 64
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hq, D, BF16, seed=10)
+    off = torch.tensor([-50, 0, 100, 4000], device=cuda)
+    out = A.masked_attn(q, k, v, window=(60, 0), q_offset=off, tensor_layout="NHD")
+    _compare(out, q, k, v, window=(60, 0), offsets=off.tolist())
+    assert not out[0].any()                                  # positions before the first key
+    far = torch.tensor([2 ** 31 - 1, -2 ** 31, 2 ** 30, -2 ** 30], device=cuda, dtype=torch.int32)
+    out = A.masked_attn(q, k, v, window=(10, 0), q_offset=far, tensor_layout="NHD")
+    assert not out.any()
+    out = A.masked_attn(q, k, v, window=(-1, 0), q_offset=2 ** 40, tensor_layout="NHD")
+    _compare(out, q, k, v)                                    # every key lies before such queries
+    lens = torch.tensor([300, 41, 40, 3], device=cuda)
+    out = A.masked_attn(q, k, v, window=(-1, 0), kv_lens=lens, q_offset="end", tensor_layout="NHD")
+    _compare(out, q, k, v, window=(-1, 0), kv_lens=lens.tolist(), offsets=[n - Sq for n in lens.tolist()])
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(3, 1), (48, 16)])
+def test_documents_and_padding(cuda, Hq, Hkv):
+    from quantfun2_b200 import attention as A
+
+    B, S, D = 4, 520, 64
+    q, k, v = _inputs(cuda, B, S, S, Hq, Hkv, D, BF16, seed=11)
+    ids = torch.zeros(B, S, dtype=torch.int64, device=cuda)
+    for cut in (1, 40, 128, 256, 300, 511):
+        ids[0, cut:] += 1                                    # packed texts
+    ids[1, 200:] = -1                                        # padded tail
+    ids[2] = torch.randint(-1, 3, (S,), device=cuda)         # any order
+    ids[3] = -1                                              # nothing but padding
+    rows = [0, 1, 39, 40, 127, 128, 199, 200, 300, 519]
+    for window in ((-1, -1), (-1, 0), (64, 10)):
+        out = A.masked_attn(q, k, v, window=window, segment_ids=ids, tensor_layout="NHD")
+        _compare(out, q, k, v, rows=rows, window=window, q_ids=ids, k_ids=ids)
+        assert not out[3].any() and not out[1, 200:].any()
+    # queries and keys of unlike lengths
+    out = A.masked_attn(q[:, :100], k, v, segment_ids=(ids[:, 150:250], ids), tensor_layout="NHD")
+    _compare(out, q[:, :100], k, v, rows=[0, 49, 50, 99], q_ids=ids[:, 150:250], k_ids=ids)
+
+
+# single tokens (and few) on caches: one to many splits, packed groups, ragged lengths
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hkv,D,dtype", [
+    (1, 1, 1, 4, 4, 64, BF16), (1, 1, 5000, 8, 1, 128, BF16), (3, 1, 1025, 24, 8, 96, FP16), (2, 5, 3000, 8, 4, 256, BF16),
+    (16, 1, 700, 4, 2, 128, FP16), (1, 1, 40000, 2, 2, 64, BF16), (200, 1, 130, 2, 1, 64, BF16), (2, 17, 2000, 12, 1, 128, BF16),
+])
+def test_few_tokens_on_caches(cuda, B, Sq, Skv, Hq, Hkv, D, dtype):
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, seed=Skv)
+    g = torch.Generator().manual_seed(Skv)
+    lens = torch.randint(max(1, Skv // 3), Skv + 1, (B,), generator=g)
+    lens[0] = Skv
+    if B > 2:
+        lens[1], lens[2] = 0, 1
+    lens = lens.to(cuda)
+    slopes = torch.rand(Hq, device=cuda) * 0.01
+    table = torch.randn(Hq, 65, device=cuda)
+    for kw in (dict(), dict(softcap=20.0, slopes=slopes), dict(bias_table=table)):
+        out = A.masked_attn(q, k, v, window=(-1, 0), kv_lens=lens, q_offset="end", tensor_layout="NHD", **kw)
+        _compare(out, q, k, v, window=(-1, 0), kv_lens=lens.tolist(), offsets=[n - Sq for n in lens.tolist()], **kw)
+    out = A.masked_attn(q, k, v, window=(77, 0), kv_lens=lens, q_offset="end", tensor_layout="NHD")
+    _compare(out, q, k, v, window=(77, 0), kv_lens=lens.tolist(), offsets=[n - Sq for n in lens.tolist()])
+
+
+@pytest.mark.parametrize("B,S,P,Hq,Hkv,D,dtype", [
+    (3, 1, 1000, 4, 2, 128, BF16), (64, 1, 3001, 6, 2, 96, FP16), (5, 40, 77, 4, 4, 64, BF16), (2, 300, 130, 2, 1, 256, BF16),
+    (8, 300, 260, 24, 8, 128, BF16), (130, 1, 129, 2, 2, 64, BF16), (1, 1, 1, 1, 1, 64, FP16), (9, 3, 500, 4, 1, 128, FP16),
+])
+def test_shared_prefix(cuda, B, S, P, Hq, Hkv, D, dtype):
+    from quantfun2_b200 import attention as A
+
+    q, k, v, pk, pv = _inputs(cuda, B, S, S + 9, Hq, Hkv, D, dtype, seed=P, P=P)
+    lens = torch.randint(0, S + 10, (B,), device=cuda, generator=torch.Generator(device=cuda).manual_seed(P))
+    lens[-1] = S + 9
+    rows = sorted({0, S // 2, S - 1})
+    slopes = torch.rand(Hq, device=cuda) * 0.02
+    for kw in (dict(), dict(softcap=30.0), dict(slopes=slopes), dict(bias_table=torch.randn(Hq, 41, device=cuda))):
+        out = A.shared_prefix_attn(q, pk, pv, k, v, window=(-1, 0), kv_lens=lens, q_offset=9, tensor_layout="NHD", **kw)
+        _compare(out, q, k, v, rows=rows, window=(-1, 0), kv_lens=lens.tolist(), offsets=[9] * B, prefix_k=pk, prefix_v=pv,
+                 **kw)
+    out = A.shared_prefix_attn(q, pk, pv, k, v, window=(60, 0), tensor_layout="NHD")
+    _compare(out, q, k, v, rows=rows, window=(60, 0), offsets=[9] * B, prefix_k=pk, prefix_v=pv)
+    # the same keys in one cache per element
+    cat_k = torch.cat([pk.expand(B, P, Hkv, D), k], 1)
+    cat_v = torch.cat([pv.expand(B, P, Hkv, D), v], 1)
+    hnd = A.shared_prefix_attn(q.transpose(1, 2), pk.transpose(0, 1), pv.transpose(0, 1), k.transpose(1, 2),
+                               v.transpose(1, 2), window=(-1, 0))
+    _compare(hnd.transpose(1, 2), q, cat_k, cat_v, rows=rows, window=(-1, 0))
+
+
+def test_no_keys_and_no_queries(cuda):
+    from quantfun2_b200 import attention as A
+
+    for Sq in (1, 300):
+        q, k, v = _inputs(cuda, 2, Sq, 0, 80, 80, 64, BF16)
+        out = torch.full_like(q, 7.0)
+        assert A.masked_attn(q, k, v, window=(-1, 0), tensor_layout="NHD", out=out) is out and not out.any()
+    q, k, v, pk, pv = _inputs(cuda, 2, 5, 0, 2, 2, 64, BF16, P=30)
+    out = A.shared_prefix_attn(q, pk, pv, k, v, tensor_layout="NHD")
+    _compare(out, q, k, v, rows=[0, 4], offsets=[0, 0], prefix_k=pk, prefix_v=pv)
+    out = A.shared_prefix_attn(q, pk[:0], pv[:0], k, v, tensor_layout="NHD")
+    assert not out.any()
+    assert A.masked_attn(q[:, :0], k, v, tensor_layout="NHD").shape == (2, 0, 2, 64)
+    assert A.masked_attn(q[:0], k[:0], v[:0], tensor_layout="NHD").shape == (0, 5, 2, 64)
+
+
+@pytest.mark.parametrize("Sq,Hq", [(1, 4), (200, 4), (300, 80)])
+def test_hidden_garbage_changes_nothing(cuda, Sq, Hq):
+    """Infinities and NaN in keys that no row sees: behind the lengths, in padding, before the
+    window; the bits of the result are those with zeros there."""
+    from quantfun2_b200 import attention as A
+
+    B, Skv, D = 2, 700, 128
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hq // 2, D, BF16, seed=13)
+    lens = torch.tensor([650, 333], device=cuda)
+    ids = torch.zeros(B, Skv, dtype=torch.int32, device=cuda)
+    ids[0, :70], ids[1, 500:] = -1, -1
+    qid = torch.zeros(B, Sq, dtype=torch.int32, device=cuda)
+    left = 100
+    first = [n - Sq - left for n in lens.tolist()]
+    calls = [
+        (dict(kv_lens=lens), lambda b, j: j >= lens[b]),
+        (dict(segment_ids=(qid, ids)), lambda b, j: ids[b] < 0),
+        (dict(kv_lens=lens, q_offset="end", window=(left, 0)), lambda b, j: (j >= lens[b]) | (j < first[b])),
+    ]
+    j = torch.arange(Skv, device=cuda)
+    for kw, hidden in calls:
+        bad = torch.stack([hidden(b, j) for b in range(B)])
+        assert bad.any()
+        outs = []
+        for fill_k, fill_v in ((0.0, 0.0), (math.nan, math.nan), (math.inf, -math.inf)):
+            kk = torch.where(bad[:, :, None, None], fill_k, k.float()).to(BF16)
+            vv = torch.where(bad[:, :, None, None], fill_v, v.float()).to(BF16)
+            outs.append(A.masked_attn(q, kk, vv, tensor_layout="NHD", **kw))
+        assert torch.isfinite(outs[0]).all() and outs[0].any()
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+def test_seen_nan_reaches_its_rows(cuda):
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, 1, 1, 3000, 2, 2, 64, BF16, seed=14)
+    k[0, 2100, 1, 3] = math.nan
+    out = A.masked_attn(q, k, v, tensor_layout="NHD")
+    assert out[0, 0, 1].isnan().all() and torch.isfinite(out[0, 0, 0]).all()
+
+
+def test_strided_inputs_and_outputs(cuda):
+    from quantfun2_b200 import attention as A
+
+    B, S, H, D = 2, 150, 3, 64
+    joint = torch.randn(B, S, 3 * H, D + 8, device=cuda).to(BF16)
+    q, k, v = (joint[:, :, n * H:(n + 1) * H, :D] for n in range(3))
+    buf = torch.full((B, S + 5, 2 * H, D), 3.0, device=cuda, dtype=BF16)
+    out = buf[:, 2:S + 2, H:]
+    assert A.masked_attn(q, k, v, window=(-1, 0), tensor_layout="NHD", out=out) is out
+    _compare(out, q, k, v, rows=[0, 64, 149], window=(-1, 0))
+    rest = buf.clone()
+    rest[:, 2:S + 2, H:] = 3.0
+    assert (rest == 3.0).all()                             # nothing beside the view was written
+    odd = torch.randn(B, S, 3 * H, D + 1, device=cuda).to(BF16)[..., 1:]     # rows off the 16-byte alignment
+    out = A.masked_attn(odd[:, :, :H], odd[:, :, H:2 * H], odd[:, :, 2 * H:], tensor_layout="NHD")
+    _compare(out, odd[:, :, :H], odd[:, :, H:2 * H], odd[:, :, 2 * H:], rows=[0, 149])
+    one = k[:1].expand(B, S, H, D)                         # one batch element's keys for all
+    out = A.masked_attn(q, one, v[:1].expand(B, S, H, D), tensor_layout="NHD")
+    _compare(out, q, one, v[:1].expand(B, S, H, D), rows=[0, 149])
+
+
+def test_two_streams_and_a_graph(cuda):
+    """Calls at once on two streams, and a captured call replayed on other lengths and values:
+    the bits of the calls alone."""
+    from quantfun2_b200 import attention as A
+
+    sets = [_inputs(cuda, 2, 1, 9000, 8, 2, 128, BF16, seed=20 + n) for n in range(2)]
+    lens = [torch.tensor([9000, 4000], device=cuda, dtype=torch.int32), torch.tensor([77, 8999], device=cuda, dtype=torch.int32)]
+    call = lambda n: A.masked_attn(*sets[n], window=(-1, 0), kv_lens=lens[n], q_offset="end", tensor_layout="NHD")  # noqa: E731
+    alone = [call(n) for n in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(5):
+        for n, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[n].append(call(n))
+    torch.cuda.synchronize()
+    for n in range(2):
+        assert all(torch.equal(o, alone[n]) for o in got[n])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = call(0)
+    for t, u in zip(sets[0], sets[1]):
+        t.copy_(u)
+    lens[0].copy_(lens[1])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(o, alone[1])
+    A.masked_attn_status()
+
+
+def test_prompt_then_tokens_then_shared_prefix(cuda):
+    """A run as an encoder-decoder of texts would make it: rotate, store, attend for a prompt;
+    then token by token on the cache; then the prompt as the shared prefix of three answers."""
+    from quantfun2_b200 import attention as A
+    from quantfun2_b200 import kernels as K
+
+    Hq, Hkv, D, S, more = 6, 2, 128, 150, 4
+    g = torch.Generator(device=cuda).manual_seed(30)
+    f = K.rotary_inv_freq(64, device=cuda)
+    tok = lambda n, B=1: [torch.randn(B, n, h, D, device=cuda, generator=g).to(BF16) for h in (Hq, Hkv, Hkv)]  # noqa: E731
+    cache_k = torch.full((1, 256, Hkv, D), math.nan, device=cuda, dtype=BF16)   # the unused end holds garbage
+    cache_v = torch.full_like(cache_k, math.nan)
+    kw = dict(window=(-1, 0), softcap=30.0, tensor_layout="NHD")
+    q, k, v = tok(S)
+    q, k = K.rotary_apply(q, k, torch.arange(S, device=cuda), f)
+    cache_k[:, :S], cache_v[:, :S] = k, v
+    out = A.masked_attn(q, k, v, **kw)
+    _compare(out, q, k, v, rows=[0, 128, S - 1], window=(-1, 0), softcap=30.0)
+    lens = torch.tensor([S], device=cuda, dtype=torch.int32)
+    for n in range(more):
+        q, k, v = tok(1)
+        K.rotary_apply_(q, k, torch.full((1, 1), S + n, device=cuda), f)
+        cache_k[:, S + n], cache_v[:, S + n] = k[:, 0], v[:, 0]
+        lens += 1
+        out = A.masked_attn(q, cache_k, cache_v, kv_lens=lens, q_offset="end", **kw)
+        _compare(out, q, cache_k[:, :S + n + 1], cache_v[:, :S + n + 1], window=(-1, 0), softcap=30.0)
+    B, P = 3, S + more
+    q, k, v = tok(7, B)
+    pos = P + torch.arange(7, device=cuda)
+    q, k = K.rotary_apply(q, k, pos, f)
+    own = torch.tensor([7, 5, 6], device=cuda)
+    out = A.shared_prefix_attn(q, cache_k[0, :P], cache_v[0, :P], k, v, kv_lens=own, q_offset=0, **kw)
+    _compare(out, q, k, v, window=(-1, 0), softcap=30.0, kv_lens=own.tolist(), offsets=[0] * B, prefix_k=cache_k[0, :P],
+             prefix_v=cache_v[0, :P])
+
+
+def test_do_attn_masked_backend(cuda):
+    from quantfun2_b200 import attention as A
+
+    B, S, Hq, Hkv, D = 3, 300, 6, 2, 96
+    q, k, v = _inputs(cuda, B, S, S, Hq, Hkv, D, BF16, seed=31)
+    mask = torch.ones(B, S, dtype=torch.bool, device=cuda)
+    mask[1, 200:] = False
+    mask[2] = torch.rand(S, device=cuda) < 0.5
+    A.ATTN = "masked"
+    try:
+        out = A.do_attn(None, q, k, v, mask)
+        dense = A.do_attn(None, q, k, v, None)
+    finally:
+        A.ATTN = "b200"
+    ids = mask.int() - 1
+    _compare(out, q, k, v, rows=[0, 100, 199, 200, 299], q_ids=ids, k_ids=ids)
+    assert not out[~mask].any()
+    _compare(dense, q, k, v, rows=[0, 299])
+
+
+def test_refusals(cuda):
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, 2, 4, 8, 4, 2, 64, BF16)
+    nhd = dict(tensor_layout="NHD")
+    i32 = lambda *x: torch.tensor(x, device=cuda, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(A.QF2Error):
+        A.masked_attn(q.float(), k.float(), v.float(), **nhd)
+    bad = [
+        ((q, k.half(), v), {}), ((q, k, v[:, :7]), {}), ((q, k[:1], v[:1]), {}), ((q[0], k, v), {}),
+        ((q[..., :56], k[..., :56], v[..., :56]), {}), ((q[:, :, :3], k, v), {}), ((q.cpu(), k, v), {}),
+        ((q, k, v), dict(tensor_layout="other")), ((q, k, v), dict(kv_lens=i32(1))), ((q, k, v), dict(kv_lens=i32(1, 1).cpu())),
+        ((q, k, v), dict(kv_lens=i32(1, 1).float())), ((q, k, v), dict(kv_lens=i32(1, 1), window=(-1, 0))),
+        ((q, k, v), dict(q_offset="start")), ((q, k, v), dict(q_offset=i32(1))), ((q, k, v), dict(segment_ids=torch.zeros(2, 4, device=cuda, dtype=torch.int32))),
+        ((q, k, v), dict(softcap=-1.0)), ((q, k, v), dict(softcap=math.inf)), ((q, k, v), dict(sm_scale=0.0)),
+        ((q, k, v), dict(slopes=torch.ones(2, device=cuda))), ((q, k, v), dict(slopes=torch.ones(4, device=cuda).half())),
+        ((q, k, v), dict(bias_table=torch.ones(4, 4, device=cuda))), ((q, k, v), dict(bias_table=torch.ones(4, 2051, device=cuda))),
+        ((q, k, v), dict(slopes=torch.ones(4, device=cuda), bias_table=torch.ones(4, 3, device=cuda))),
+        ((q, k, v), dict(out=torch.empty(2, 4, 4, 64, device=cuda))), ((q, k, v), dict(out=torch.empty(2, 5, 4, 64, device=cuda, dtype=BF16))),
+        ((q, k, v), dict(out=torch.empty(2, 4, 4, 68, device=cuda, dtype=BF16)[..., :64])),
+        ((q.requires_grad_(), k, v), {}),
+    ]
+    for args, kw in bad:
+        with pytest.raises(A.QF2Error):
+            A.masked_attn(*args, **{**nhd, **kw})
+    q = q.detach()
+    pk = k[0]
+    for args in ((q, None, None, k, v), (q, pk, None, k, v), (q, pk[None], pk[None], k, v), (q, pk[:, :1], pk[:, :1], k, v),
+                 (q, pk[..., :32], pk[..., :32], k, v), (q, pk.half(), pk.half(), k, v)):
+        with pytest.raises(A.QF2Error):
+            A.shared_prefix_attn(*args, **nhd)
+    with torch.no_grad():                                    # a parameter's values are fine where no gradient is wanted
+        A.masked_attn(q.clone().requires_grad_(), k, v, **nhd)
+    A.masked_attn_status()

@@ -1,0 +1,105 @@
+"""CPU: frequencies, argument checks and work plans of the text-side operators."""
+import ctypes
+import math
+
+import pytest
+import torch
+
+from quantfun2_b200 import _lib
+from quantfun2_b200._lib import QF2Error
+
+
+def test_rotary_frequencies():
+    from quantfun2_b200.kernels import rotary_inv_freq
+
+    r = 64
+    f = rotary_inv_freq(r, base=500.0)
+    ref = torch.tensor([500.0 ** (-2 * p / r) for p in range(r // 2)], dtype=torch.float64)
+    assert f.dtype == torch.float64 and torch.allclose(f, ref, rtol=1e-14, atol=0)
+    assert torch.allclose(rotary_inv_freq(r, scaling="linear", factor=4.0), rotary_inv_freq(r) / 4, rtol=1e-14, atol=0)
+    ntk = rotary_inv_freq(r, scaling="ntk", factor=4.0)
+    assert ntk[0] == 1.0 and math.isclose(ntk[-1].item(), rotary_inv_freq(r)[-1].item() / 4, rel_tol=1e-12)
+    plain, parts = rotary_inv_freq(r), rotary_inv_freq(r, scaling="by_parts", factor=4.0, original_length=4096)
+    for p in range(r // 2):
+        turns = 4096 * plain[p].item() / (2 * math.pi)
+        keep = min(1.0, max(0.0, (turns - 1.0) / 31.0))
+        assert math.isclose(parts[p].item(), plain[p].item() * (keep + (1 - keep) / 4), rel_tol=1e-12)
+    for bad in (dict(rotary_dim=7), dict(rotary_dim=0), dict(rotary_dim=8, scaling="other"), dict(rotary_dim=8, base=0.0),
+                dict(rotary_dim=8, scaling="linear", factor=-1.0),
+                dict(rotary_dim=8, scaling="by_parts", beta_fast=1.0, beta_slow=1.0)):
+        with pytest.raises(QF2Error):
+            rotary_inv_freq(**bad)
+
+
+def test_ops_refuse_host_tensors():
+    from quantfun2_b200 import attention, kernels
+
+    x = torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(QF2Error):
+        kernels.rotary_apply(x, None, torch.arange(2), kernels.rotary_inv_freq(64))
+    with pytest.raises(QF2Error):
+        attention.masked_attn(x, x, x)
+    with pytest.raises(QF2Error):
+        attention.shared_prefix_attn(x, None, None, x, x)
+
+
+def _call(**kw):
+    """qf2_masked_attn with aligned dummy pointers: every refusal below comes before a launch."""
+    lib = _lib.load()
+    a = dict(B=1, Hq=2, Hkv=2, Sq=4, Skv=4, D=64, P=0, dtype=_lib.QF2_BF16, scale=0.1, q=1024, k=1024, v=1024, out=1024,
+             stride=64, ws=None, nbytes=0, pk=None)
+    mask = _lib.AttnMask(left=-1, right=-1)
+    for key, val in kw.items():
+        if key in a:
+            a[key] = val
+        else:
+            setattr(mask, key, val)
+    s = _lib.i64(a["stride"], a["stride"], a["stride"])
+    p = lambda x: None if x is None else ctypes.c_void_p(x)  # noqa: E731
+    return lib.qf2_masked_attn(p(a["q"]), s, p(a["k"]), s, p(a["v"]), s, p(a["out"]), s, a["B"], a["Hq"], a["Hkv"],
+                               a["Sq"], a["Skv"], a["D"], p(a["pk"]), s, p(a["pk"]), s, a["P"], mask, a["scale"],
+                               a["dtype"], p(a["ws"]), a["nbytes"], None)
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(dtype=_lib.QF2_F32), -2), (dict(D=80), -1), (dict(Hq=3), -1), (dict(Hkv=0), -1), (dict(Sq=-1), -1),
+    (dict(B=70000), -1), (dict(Skv=(1 << 20) + 1), -1), (dict(Skv=1 << 20, P=1), -1), (dict(q=None), -8), (dict(k=None), -8),
+    (dict(out=None), -8), (dict(P=4), -8), (dict(q_ids=1024), -8), (dict(k_ids=1024), -8), (dict(q_offset_mode=3), -8),
+    (dict(q_offset_mode=1), -8), (dict(slopes=1024, bias_table=1024), -8), (dict(bias_table=1024, bias_reach=1025), -1),
+    (dict(softcap=-1.0), -8), (dict(softcap=math.nan), -8), (dict(scale=0.0), -8), (dict(scale=math.inf), -8),
+    (dict(q=1032), -5), (dict(v=1032), -5), (dict(stride=60), -5), (dict(stride=0), -5),
+    (dict(q_ids=1024, k_ids=1024), -6), (dict(q_ids=1024, k_ids=1024, pk=1024, P=4), -8),
+])
+def test_attention_refusals_without_device(kw, status):
+    assert _call(**kw) == status
+
+
+def test_empty_batches_return_at_once():
+    assert _call(B=0, q=None) == 0 and _call(Sq=0) == 0
+
+
+def test_workspace_plans():
+    ws = _lib.load().qf2_masked_attn_workspace_bytes
+    # long queries: no split; ids: a padded copy and one range per key tile
+    assert ws(1, 24, 8, 16384, 16384, 0, 128, 0) == 0
+    tiles = 16384 // 128
+    assert ws(1, 24, 8, 16384, 16384, 0, 128, 1) == tiles * 128 * 4 + tiles * 8
+    # single tokens on a long cache are split: fp32 rows and (max, sum) pairs of each split
+    one = ws(1, 8, 8, 1, 65536, 0, 128, 0)
+    assert one > 0 and (one - 0) % 256 == 0
+    assert ws(1, 8, 8, 1, 100, 0, 128, 0) == 0                     # one key tile: nothing to split
+    assert ws(64, 24, 8, 1, 512, 16384, 128, 0) > 0                 # prefix items have partial rows
+    assert ws(1, 24, 7, 1, 1, 0, 128, 0) == -1
+
+
+def test_rotary_refusals_without_device():
+    lib = _lib.load()
+    s3, s2, p = _lib.i64(64, 64, 64), _lib.i64(0, 1), ctypes.c_void_p(1024)
+
+    def call(xq=p, Hq=1, xk=None, Hk=0, pos=p, f=p, r=64, layout=0, B=1, S=1, D=64, dtype=2):
+        return lib.qf2_rotary_apply(xq, xq, Hq, s3, s3, xk, xk, Hk, s3, s3, pos, s2, 1, f, r, layout, 1.0, 0, B, S, D,
+                                    dtype, None)
+
+    assert call(dtype=3) == -2 and call(layout=2) == -8 and call(r=63) == -1 and call(r=66) == -1 and call(r=0) == -1
+    assert call(D=2048) == -1 and call(B=-1) == -1 and call(Hk=1) == -8 and call(xq=None) == -8 and call(pos=None) == -8
+    assert call(f=None) == -8 and call(B=0) == 0 and call(Hq=0) == 0 and call(S=0, pos=None) == 0
