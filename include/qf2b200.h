@@ -118,11 +118,22 @@ int qf2_rope_scatter(const void* x, const int64_t* x_strides, const float* f, in
  * that are not 16-byte aligned take single-element accesses. */
 #define QF2_ROTARY_HALF 0
 #define QF2_ROTARY_INTERLEAVED 1
-int qf2_rotary_apply(const void* xq, void* xq_out, int64_t Hq, const int64_t* xq_strides,
-                     const int64_t* xq_out_strides, const void* xk, void* xk_out, int64_t Hk,
-                     const int64_t* xk_strides, const int64_t* xk_out_strides, const void* positions,
-                     const int64_t* pos_strides, int pos_is_i64, const double* inv_freq, int64_t rotary_dim, int layout,
-                     float gain, int inverse, int64_t B, int64_t S, int64_t D, int dtype, qf2_stream_t stream);
+typedef struct qf2_rotary_args { /* every field 8 bytes */
+  const void* xq;
+  void* xq_out;
+  const void* xk;
+  void* xk_out;
+  const void* positions;
+  const double* inv_freq;
+  int64_t xq_strides[3], xq_out_strides[3], xk_strides[3], xk_out_strides[3];
+  int64_t pos_strides[2];
+  int64_t pos_is_i64;
+  int64_t B, S, Hq, Hk, D, rotary_dim;
+  int64_t layout, inverse, dtype;
+  double gain;
+  qf2_stream_t stream;
+} qf2_rotary_args;
+int qf2_rotary_apply(const qf2_rotary_args* args);
 
 /* ------------------------------------------------------------- RMSNorm --
  * Replaces rmsnorm_apply (src/kernels/__init__.py:73-80) and the Triton
@@ -261,9 +272,10 @@ int qf2_blocksparse_attn(const void* q, const int64_t* q_strides, const void* k,
  *   j < kv_lens[b] (clamped to [0, Skv]; NULL: Skv)  and
  *   j < prefix_lens[b]  or  (left < 0 or j >= t_i - left) and (right < 0 or j <= t_i + right)
  *   and, with ids, q_ids[b][i] == k_ids[b][j] >= 0 (ids of documents; negative = padding).
- * Causal attention is right = 0.  A key hidden from every row is not read into the result,
- * whatever its bits; a NaN or infinite value that some rows see may reach the others of
- * its 128-row tile (0 * NaN), as it does in a plain product.
+ * Causal attention is right = 0.  Keys behind kv_lens, of a negative id, or outside every
+ * query's band and prefix do not enter the result, whatever their bits; a NaN or infinite
+ * value that some rows see may reach the others of
+ * its tile (0 * NaN), as it does in a plain product.
  * prefix_k / prefix_v [P, Hkv, D] (strides {-, head, seq}): keys and values that all batch
  * elements share at positions 0 .. P - 1, read once for the rows of many batch elements;
  * the own key j, the queries and kv_lens then count from position P.  Not with ids.
@@ -276,28 +288,36 @@ int qf2_blocksparse_attn(const void* q, const int64_t* q_strides, const void* k,
 #define QF2_OFFSET_CONST 0
 #define QF2_OFFSET_ARRAY 1
 #define QF2_OFFSET_END 2
-typedef struct qf2_attn_mask {
-  int64_t left, right;        /* band around the query's position, < 0: open           */
-  const int32_t* kv_lens;     /* [B] or NULL                                           */
-  const int32_t* prefix_lens; /* [B] or NULL                                           */
-  const int32_t* q_offsets;   /* [B], for QF2_OFFSET_ARRAY                             */
-  int64_t q_offset;           /* for QF2_OFFSET_CONST                                  */
+typedef struct qf2_masked_attn_args { /* every field 8 bytes */
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const void* prefix_k;
+  const void* prefix_v;
+  int64_t q_strides[3], k_strides[3], v_strides[3], out_strides[3]; /* {batch, head, seq} */
+  int64_t prefix_k_strides[2], prefix_v_strides[2];                 /* {head, seq}        */
+  int64_t B, Hq, Hkv, Sq, Skv, P, D, dtype;
+  int64_t left, right;        /* band around the query's position, < 0: open             */
+  const int32_t* kv_lens;     /* [B] or NULL                                             */
+  const int32_t* prefix_lens; /* [B] or NULL                                             */
+  const int32_t* q_offsets;   /* [B], for QF2_OFFSET_ARRAY                               */
+  int64_t q_offset;           /* for QF2_OFFSET_CONST                                    */
   int64_t q_offset_mode;
-  const int32_t* q_ids;       /* [B, Sq] or NULL                                       */
-  const int32_t* k_ids;       /* [B, Skv] or NULL, with q_ids                          */
-  const float* slopes;        /* [Hq] or NULL                                          */
-  const float* bias_table;    /* [Hq, 2 * bias_reach + 1] or NULL, not with slopes     */
+  const int32_t* q_ids;       /* [B, Sq] or NULL                                         */
+  const int32_t* k_ids;       /* [B, Skv] or NULL, with q_ids                            */
+  const float* slopes;        /* [Hq] or NULL                                            */
+  const float* bias_table;    /* [Hq, 2 * bias_reach + 1] or NULL, not with slopes       */
   int64_t bias_reach;
-  float softcap;              /* 0: none                                               */
-} qf2_attn_mask;
+  double softcap;             /* 0: none                                                 */
+  double sm_scale;
+  void* workspace;            /* qf2_masked_attn_workspace_bytes                         */
+  int64_t workspace_bytes;
+  qf2_stream_t stream;
+} qf2_masked_attn_args;
 int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P,
                                         int64_t D, int with_ids);
-int qf2_masked_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, const void* v,
-                    const int64_t* v_strides, void* out, const int64_t* out_strides, int64_t B, int64_t Hq,
-                    int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D, const void* prefix_k,
-                    const int64_t* prefix_k_strides, const void* prefix_v, const int64_t* prefix_v_strides, int64_t P,
-                    const qf2_attn_mask* mask, float sm_scale, int dtype, void* workspace, int64_t workspace_bytes,
-                    qf2_stream_t stream);
+int qf2_masked_attn(const qf2_masked_attn_args* args);
 int qf2_masked_attn_status(qf2_stream_t stream);
 
 /* ------------------------------------------------------ quantized linears --

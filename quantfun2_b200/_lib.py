@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_int64, c_void_p, POINTER
 from pathlib import Path
 
@@ -28,13 +29,38 @@ _P32 = POINTER(ctypes.c_int32)
 
 
 
-class AttnMask(ctypes.Structure):
-    """qf2_attn_mask of include/qf2b200.h."""
+class _Args:
+    """An argument struct of include/qf2b200.h whose fields are all 8 bytes, filled by one
+    struct.pack: a ctypes call of two dozen arguments costs the host more than a small kernel
+    takes.  `fields`: (name, count, format q or d) in order."""
 
-    _fields_ = [("left", c_int64), ("right", c_int64), ("kv_lens", c_void_p), ("prefix_lens", c_void_p),
-                ("q_offsets", c_void_p), ("q_offset", c_int64), ("q_offset_mode", c_int64), ("q_ids", c_void_p),
-                ("k_ids", c_void_p), ("slopes", c_void_p), ("bias_table", c_void_p), ("bias_reach", c_int64),
-                ("softcap", c_float)]
+    def __init__(self, fields):
+        self.fields = fields
+        self._struct = struct.Struct("=" + "".join(f"{n}{f}" for _, n, f in fields))
+        self.pack = self._struct.pack
+
+    def pack_named(self, **values) -> bytes:
+        flat = []
+        for name, n, _ in self.fields:
+            v = values.get(name) or 0
+            flat += list(v) if isinstance(v, (tuple, list)) else [v] * n
+        return self.pack(*flat)
+
+
+ROTARY_ARGS = _Args([
+    ("xq", 1, "q"), ("xq_out", 1, "q"), ("xk", 1, "q"), ("xk_out", 1, "q"), ("positions", 1, "q"), ("inv_freq", 1, "q"),
+    ("xq_strides", 3, "q"), ("xq_out_strides", 3, "q"), ("xk_strides", 3, "q"), ("xk_out_strides", 3, "q"),
+    ("pos_strides", 2, "q"), ("pos_is_i64", 1, "q"), ("B", 1, "q"), ("S", 1, "q"), ("Hq", 1, "q"), ("Hk", 1, "q"),
+    ("D", 1, "q"), ("rotary_dim", 1, "q"), ("layout", 1, "q"), ("inverse", 1, "q"), ("dtype", 1, "q"), ("gain", 1, "d"),
+    ("stream", 1, "q")])
+MASKED_ATTN_ARGS = _Args([
+    ("q", 1, "q"), ("k", 1, "q"), ("v", 1, "q"), ("out", 1, "q"), ("prefix_k", 1, "q"), ("prefix_v", 1, "q"),
+    ("q_strides", 3, "q"), ("k_strides", 3, "q"), ("v_strides", 3, "q"), ("out_strides", 3, "q"),
+    ("prefix_k_strides", 2, "q"), ("prefix_v_strides", 2, "q"), ("B", 1, "q"), ("Hq", 1, "q"), ("Hkv", 1, "q"),
+    ("Sq", 1, "q"), ("Skv", 1, "q"), ("P", 1, "q"), ("D", 1, "q"), ("dtype", 1, "q"), ("left", 1, "q"), ("right", 1, "q"),
+    ("kv_lens", 1, "q"), ("prefix_lens", 1, "q"), ("q_offsets", 1, "q"), ("q_offset", 1, "q"), ("q_offset_mode", 1, "q"),
+    ("q_ids", 1, "q"), ("k_ids", 1, "q"), ("slopes", 1, "q"), ("bias_table", 1, "q"), ("bias_reach", 1, "q"),
+    ("softcap", 1, "d"), ("sm_scale", 1, "d"), ("workspace", 1, "q"), ("workspace_bytes", 1, "q"), ("stream", 1, "q")])
 
 
 # name -> (restype, argtypes); mirrors include/qf2b200.h
@@ -100,19 +126,10 @@ SIGNATURES = {
         [c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_int64, c_int64, c_int64, c_int64,
          c_int64, c_void_p, c_int64, c_float, c_int, c_void_p, c_int64, c_void_p],
     ),
-    "qf2_rotary_apply": (
-        c_int,
-        [c_void_p, c_void_p, c_int64, _P64, _P64, c_void_p, c_void_p, c_int64, _P64, _P64, c_void_p, _P64, c_int,
-         c_void_p, c_int64, c_int, c_float, c_int, c_int64, c_int64, c_int64, c_int, c_void_p],
-    ),
+    "qf2_rotary_apply": (c_int, [ctypes.c_char_p]),
     "qf2_masked_attn_workspace_bytes": (
         c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
-    "qf2_masked_attn": (
-        c_int,
-        [c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_void_p, _P64, c_int64, c_int64, c_int64, c_int64, c_int64,
-         c_int64, c_void_p, _P64, c_void_p, _P64, c_int64, POINTER(AttnMask), c_float, c_int, c_void_p, c_int64,
-         c_void_p],
-    ),
+    "qf2_masked_attn": (c_int, [ctypes.c_char_p]),
     "qf2_masked_attn_status": (c_int, [c_void_p]),
     "qf2_quantize_rows": (
         c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p]),
@@ -231,6 +248,13 @@ def on_device(device):
     if device.index is None or device.index == torch.cuda.current_device():
         return _NO_GUARD
     return torch.cuda.device(device)
+
+
+def raw_stream(index: int) -> int:
+    """Handle of the current stream of device `index`."""
+    import torch
+
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def stream_ptr(device=None) -> c_void_p:

@@ -15,12 +15,13 @@ PyTorch's caching allocator for each call; the library itself allocates nothing.
 """
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
 
 from . import _lib
-from ._lib import AttnMask, QF2Error, check, i64, on_device, ptr32, require_device, stream_ptr
+from ._lib import QF2Error, check, i64, on_device, ptr32, raw_stream, require_device, stream_ptr
 
 __all__ = ["sageattn", "sageattn_varlen", "sage_quantize", "sage_workspace_layout", "block_topk_select",
            "blocksparse_attn", "flash_attn", "masked_attn", "shared_prefix_attn", "masked_attn_status", "do_attn",
@@ -240,18 +241,20 @@ def blocksparse_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, idx: tor
 
 
 # ------------------------------------------- masked, capped, biased attention --
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    # rows a tensor map can read: contiguous channels, 16-byte aligned, no dimension on itself
-    if t.stride(-1) != 1 or t.data_ptr() % 16 or \
-            any(n > 1 and (s % 8 or s <= 0) for s, n in zip(t.stride()[:-1], t.shape)):
+def _rows16(t: torch.Tensor):
+    """t with rows a tensor map can read (contiguous channels, 16-byte aligned, no dimension
+    lying on itself), and its strides."""
+    st = t.stride()
+    if st[-1] != 1 or t.data_ptr() % 16 or any((x % 8 or x <= 0) and n > 1 for x, n in zip(st[:-1], t.shape)):
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-    return t
+        st = t.stride()
+    return t, st
 
 
 def _int32(t: torch.Tensor, shape, what: str, device) -> torch.Tensor:
-    if t.device != device or tuple(t.shape) != tuple(shape) or t.dtype not in (torch.int32, torch.int64):
+    if t.device != device or t.shape != shape or t.dtype not in (torch.int32, torch.int64):
         raise QF2Error(f"{what} must be int32 (or int64) of shape {tuple(shape)} on {device}")
     if t.dtype != torch.int32:
         t = t.to(torch.int32)
@@ -264,100 +267,123 @@ def _float32(t: torch.Tensor, what: str, device) -> torch.Tensor:
     return t if t.is_contiguous() else t.contiguous()
 
 
+@functools.lru_cache(maxsize=4096)
+def _masked_workspace(B, Hq, Hkv, Sq, Skv, P, D, with_ids) -> int:
+    nbytes = int(_lib.load().qf2_masked_attn_workspace_bytes(B, Hq, Hkv, Sq, Skv, P, D, with_ids))
+    if nbytes < 0:
+        check(nbytes, "qf2_masked_attn_workspace_bytes")
+    return nbytes
+
+
 def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_lens, q_offset, softcap, slopes,
             bias_table, sm_scale, tensor_layout, out):
     require_device(q)
-    dev = q.device
-    for t, what in ((k, "k"), (v, "v"), (prefix_k, "prefix_k"), (prefix_v, "prefix_v")):
-        if t is not None and (t.dtype != q.dtype or t.device != dev):
-            raise QF2Error(f"{what} must have q's dtype and device")
-    if q.dim() != 4 or k.dim() != 4:
-        raise QF2Error("q, k and v must have four dimensions")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k, v, prefix_k, prefix_v, slopes, bias_table)):
-        raise QF2Error("masked attention is an inference op: its inputs must not require a gradient")
+    dev, dtype = q.device, q.dtype
     dt = _dt(q)
-    B, Hq, Sq, D, _ = _hnd(q, tensor_layout)
-    Bk, Hkv, Skv, Dk, _ = _hnd(k, tensor_layout)
-    if v.shape != k.shape or Bk != B or Dk != D or Hkv == 0 or Hq % Hkv:
-        raise QF2Error("k and v must be alike, with q's batch and head dim and a number of heads that divides q's")
-    P = 0
+    if k.dtype != dtype or v.dtype != dtype or k.device != dev or v.device != dev:
+        raise QF2Error("k and v must have q's dtype and device")
+    if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape:
+        raise QF2Error("q, k and v must have four dimensions, k and v alike")
+    if tensor_layout == "NHD":
+        B, Sq, Hq, D = q.shape
+        Bk, Skv, Hkv, Dk = k.shape
+        h, n = 2, 1
+    elif tensor_layout == "HND":
+        B, Hq, Sq, D = q.shape
+        Bk, Hkv, Skv, Dk = k.shape
+        h, n = 1, 2
+    else:
+        raise QF2Error(f"unknown tensor_layout {tensor_layout}")
+    if Bk != B or Dk != D or Hkv == 0 or Hq % Hkv:
+        raise QF2Error("k and v must have q's batch and head dim and a number of heads that divides q's")
+    P = pkp = pvp = pk_h = pk_n = pv_h = pv_n = 0
     if prefix_k is not None:
-        if prefix_v is None or prefix_k.dim() != 3 or prefix_v.shape != prefix_k.shape or prefix_k.shape[2] != D:
-            raise QF2Error("prefix_k and prefix_v must be alike, three-dimensional, with q's head dim")
-        ph, P = (prefix_k.shape[0], prefix_k.shape[1]) if tensor_layout == "HND" else \
-            (prefix_k.shape[1], prefix_k.shape[0])
-        if ph != Hkv:
-            raise QF2Error("the prefix must have the own keys' heads")
+        for t in (prefix_k, prefix_v):
+            if t.dtype != dtype or t.device != dev or t.dim() != 3 or t.shape != prefix_k.shape or t.shape[2] != D \
+                    or t.shape[h - 1] != Hkv:
+                raise QF2Error("prefix_k and prefix_v must be alike, three-dimensional, with the own keys' dtype, "
+                               "device, heads and head dim")
+        P = prefix_k.shape[n - 1]
+    if torch.is_grad_enabled():
+        for t in (q, k, v, prefix_k, prefix_v, slopes, bias_table):
+            if t is not None and t.requires_grad:
+                raise QF2Error("masked attention is an inference op: its inputs must not require a gradient")
     if out is None:
         out = torch.empty_like(q)
-        if out.stride(-1) != 1 or any(s % 8 for s in out.stride()[:-1]):
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or out.stride(-1) != 1 or \
-            any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
-        raise QF2Error("out must match q's shape, dtype and device, with a contiguous last dim")
-    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+        os = out.stride()
+        if os[3] != 1 or os[0] % 8 or os[1] % 8 or os[2] % 8:
+            out = torch.empty(q.shape, dtype=dtype, device=dev)
+            os = out.stride()
+    else:
+        os = out.stride()
+        if out.shape != q.shape or out.dtype != dtype or out.device != dev or os[3] != 1 or \
+                any(x == 0 and m > 1 for x, m in zip(os, out.shape)):
+            raise QF2Error("out must match q's shape, dtype and device, with a contiguous last dim")
+    q, qs = _rows16(q)
+    k, ks = _rows16(k)
+    v, vs = _rows16(v)
     if P:
-        prefix_k, prefix_v = _rows16(prefix_k), _rows16(prefix_v)
+        prefix_k, st = _rows16(prefix_k)
+        pkp, pk_h, pk_n = prefix_k.data_ptr(), st[h - 1], st[n - 1]
+        prefix_v, st = _rows16(prefix_v)
+        pvp, pv_h, pv_n = prefix_v.data_ptr(), st[h - 1], st[n - 1]
 
-    m = AttnMask()
-    left, right = (-1, -1) if window is None else (int(window[0]), int(window[1]))
-    m.left, m.right = max(left, -1), max(right, -1)
-    keep = []  # converted arrays stay referenced until the launch is queued
-
-    def dev_ptr(t):
-        keep.append(t)
-        return t.data_ptr()
-
+    left = right = -1
+    if window is not None:
+        left, right = max(int(window[0]), -1), max(int(window[1]), -1)
+    lens_p = pre_p = off_p = off = mode = qi_p = ki_p = slope_p = table_p = reach = 0
     if kv_lens is not None:
-        m.kv_lens = dev_ptr(_int32(kv_lens, (B,), "kv_lens", dev))
+        kv_lens = _int32(kv_lens, (B,), "kv_lens", dev)
+        lens_p = kv_lens.data_ptr()
     if prefix_lens is not None:
-        m.prefix_lens = dev_ptr(_int32(prefix_lens, (B,), "prefix_lens", dev))
+        prefix_lens = _int32(prefix_lens, (B,), "prefix_lens", dev)
+        pre_p = prefix_lens.data_ptr()
     if segment_ids is not None:
         qi, ki = segment_ids if isinstance(segment_ids, (tuple, list)) else (segment_ids, segment_ids)
-        m.q_ids = dev_ptr(_int32(qi, (B, Sq), "segment_ids of the queries", dev))
-        m.k_ids = dev_ptr(_int32(ki, (B, Skv), "segment_ids of the keys", dev))
+        qi = _int32(qi, (B, Sq), "segment_ids of the queries", dev)
+        ki = _int32(ki, (B, Skv), "segment_ids of the keys", dev)
+        qi_p, ki_p = qi.data_ptr(), ki.data_ptr()
+        if ki_p == 0:
+            ki_p = qi_p = 16  # no keys: never read, but ids are in use
     if q_offset is None:
         if kv_lens is not None and (left >= 0 or right >= 0 or slopes is not None or bias_table is not None):
             raise QF2Error("with kv_lens, give q_offset: 0 for right-padded prompts, 'end' for the last tokens of a "
                            "cache, or the first query's position")
-        m.q_offset = Skv - Sq
+        off = Skv - Sq
     elif isinstance(q_offset, str):
         if q_offset != "end":
             raise QF2Error(f"unknown q_offset {q_offset!r}")
-        m.q_offset_mode = _lib.QF2_OFFSET_END
+        mode = _lib.QF2_OFFSET_END
     elif isinstance(q_offset, torch.Tensor):
-        m.q_offsets = dev_ptr(_int32(q_offset, (B,), "q_offset", dev))
-        m.q_offset_mode = _lib.QF2_OFFSET_ARRAY
+        q_offset = _int32(q_offset, (B,), "q_offset", dev)
+        off_p, mode = q_offset.data_ptr(), _lib.QF2_OFFSET_ARRAY
     else:
-        m.q_offset = int(q_offset)
+        off = int(q_offset)
     if slopes is not None:
         if bias_table is not None:
             raise QF2Error("give slopes or bias_table, not both")
-        if tuple(slopes.shape) != (Hq,):
+        if slopes.shape != (Hq,):
             raise QF2Error(f"slopes must be [{Hq}]")
-        m.slopes = dev_ptr(_float32(slopes, "slopes", dev))
+        slopes = _float32(slopes, "slopes", dev)
+        slope_p = slopes.data_ptr()
     if bias_table is not None:
         if bias_table.dim() != 2 or bias_table.shape[0] != Hq or bias_table.shape[1] % 2 == 0:
             raise QF2Error(f"bias_table must be [{Hq}, 2 R + 1]")
-        m.bias_table = dev_ptr(_float32(bias_table, "bias_table", dev))
-        m.bias_reach = bias_table.shape[1] // 2
-    m.softcap = float(softcap or 0.0)
+        bias_table = _float32(bias_table, "bias_table", dev)
+        table_p, reach = bias_table.data_ptr(), bias_table.shape[1] // 2
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    lib = _lib.load()
-    nbytes = int(lib.qf2_masked_attn_workspace_bytes(B, Hq, Hkv, Sq, Skv, P, D, int(segment_ids is not None)))
-    if nbytes < 0:
-        check(nbytes, "qf2_masked_attn_workspace_bytes")
+    nbytes = _masked_workspace(B, Hq, Hkv, Sq, Skv, P, D, int(segment_ids is not None))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    st = lambda t: i64(*_hnd(t, tensor_layout)[4])  # noqa: E731
-    pst = lambda t: i64(0, t.stride(0), t.stride(1)) if tensor_layout == "HND" else i64(0, t.stride(1), t.stride(0))  # noqa: E731
+    args = _lib.MASKED_ATTN_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), pkp, pvp, qs[0], qs[h], qs[n], ks[0], ks[h], ks[n],
+        vs[0], vs[h], vs[n], os[0], os[h], os[n], pk_h, pk_n, pv_h, pv_n, B, Hq, Hkv, Sq, Skv, P, D, dt, left, right,
+        lens_p, pre_p, off_p, off, mode, qi_p, ki_p, slope_p, table_p, reach, softcap or 0.0, sm_scale,
+        ws.data_ptr() if nbytes else 0, nbytes, raw_stream(dev.index))
     with on_device(dev):
-        check(lib.qf2_masked_attn(
-            q.data_ptr(), st(q), k.data_ptr(), st(k), v.data_ptr(), st(v), out.data_ptr(), st(out), B, Hq, Hkv, Sq,
-            Skv, D, prefix_k.data_ptr() if P else None, pst(prefix_k) if P else None,
-            prefix_v.data_ptr() if P else None, pst(prefix_v) if P else None, P, m, float(sm_scale), dt,
-            ws.data_ptr() if nbytes else None, nbytes, stream_ptr(dev)), "qf2_masked_attn")
+        status = _lib.load().qf2_masked_attn(args)
+    if status:
+        check(status, "qf2_masked_attn")
     return out
 
 

@@ -4,6 +4,7 @@
 #include "masked_attn.cuh"
 
 #include <algorithm>
+#include <cfloat>
 
 namespace qf2 {
 namespace mattn {
@@ -13,48 +14,111 @@ namespace mattn {
 __device__ int g_status;
 
 // ------------------------------------------------------------- key ids --
-// Padded copy of a batch element's key ids (tiles of 128, pad -2) and the least and
-// greatest id of each tile: a tile is skipped where its range meets none of the rows' ids.
-// grid (nto, B), 128 threads.
+// Padded copy of a batch element's key ids (tiles of 128, pad -2), the least and greatest id of
+// each tile, and whether the tile's ids, and the next tile's first, do not fall (as unsigned
+// numbers: the negative ids of padding come last).  grid (nto, B), 128 threads.
 __global__ void __launch_bounds__(128) mattn_ids_kernel(const int32_t* __restrict__ ids, int Skv, int nto,
-                                                        int32_t* __restrict__ out, int2* __restrict__ rng) {
+                                                        int32_t* __restrict__ out, int2* __restrict__ rng,
+                                                        int* __restrict__ rising) {
   const int t = blockIdx.x, b = blockIdx.y, i = threadIdx.x;
   const int j = t * kBlk + i;
   const int v = j < Skv ? ids[(int64_t)b * Skv + j] : -2;
+  const int next = j + 1 < Skv ? ids[(int64_t)b * Skv + j + 1] : -1;
+  const int fine = __syncthreads_and(j + 1 >= Skv || (uint32_t)v <= (uint32_t)next);
   out[((int64_t)b * nto + t) * kBlk + i] = v;
   __shared__ int2 part[4];
   const int mn = __reduce_min_sync(0xffffffffu, v), mx = __reduce_max_sync(0xffffffffu, v);
   if ((i & 31) == 0) part[i >> 5] = make_int2(mn, mx);
   __syncthreads();
-  if (i == 0)
+  if (i == 0) {
     rng[(int64_t)b * nto + t] = make_int2(min(min(part[0].x, part[1].x), min(part[2].x, part[3].x)),
                                           max(max(part[0].y, part[1].y), max(part[2].y, part[3].y)));
+    rising[(int64_t)b * nto + t] = fine;
+  }
+}
+
+// Where a batch element's key ids are in order, the keys of each query's id are one run, found by
+// two binary searches: the attention kernel then masks by ranges (documents, padded ends) and
+// looks at no id.  grid (ceil(Sq / 128), B), 128 threads.
+__global__ void __launch_bounds__(128) mattn_runs_kernel(const int32_t* __restrict__ q_ids,
+                                                         const int32_t* __restrict__ k_ids,
+                                                         const int* __restrict__ rising, int Sq, int Skv, int nto,
+                                                         int2* __restrict__ q_rng, int* __restrict__ sorted) {
+  const int b = blockIdx.y, i = blockIdx.x * 128 + threadIdx.x;
+  int fine = 1;
+  for (int t = threadIdx.x; t < nto; t += 128) fine &= rising[(int64_t)b * nto + t];
+  fine = __syncthreads_and(fine);
+  if (blockIdx.x == 0 && threadIdx.x == 0) sorted[b] = fine;
+  if (!fine || i >= Sq) return;
+  const int id = q_ids[(int64_t)b * Sq + i];
+  const int32_t* k = k_ids + (int64_t)b * nto * kBlk;
+  int2 r = make_int2(0, 0);
+  if (id >= 0) {
+    // first key with an id of at least `id`, first with a greater one
+    int lo = 0, hi = Skv;
+    while (lo < hi) {
+      const int m = (lo + hi) >> 1;
+      if ((uint32_t)k[m] < (uint32_t)id) lo = m + 1; else hi = m;
+    }
+    r.x = lo;
+    hi = Skv;
+    while (lo < hi) {
+      const int m = (lo + hi) >> 1;
+      if ((uint32_t)k[m] <= (uint32_t)id) lo = m + 1; else hi = m;
+    }
+    r.y = lo;
+  }
+  q_rng[(int64_t)b * Sq + i] = r;
 }
 
 // ----------------------------------------------------------- merge splits --
 // out = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s over the splits of one row (a split
 // that saw nothing has m = -inf and is not read).  One CTA per (batch, token, head) row:
 // D / 4 threads cover the row in 16-byte pieces, 128 / (D / 4) such groups take every
-// second, fifth, ... split, and the groups are added in a fixed order.
+// second, fifth, ... split, and the groups are added in a fixed order.  A row's splits are up
+// to two runs of partial rows: the own items' and the prefix items'.
 template <int D, bool F16>
-__global__ void __launch_bounds__(128) mattn_merge_kernel(const float* __restrict__ part_o,
-                                                          const float2* __restrict__ part_ml, int ns, int64_t R,
-                                                          uint8_t* __restrict__ out, S3 os, int Sq, int Hq) {
+__global__ void __launch_bounds__(128) mattn_merge_kernel(const __grid_constant__ Args A) {
   constexpr int C = D / 4, NG = 128 / C;
-  __shared__ float wgt[kMaxSplits];
+  __shared__ float wgt[2 * kMaxSplits];
   __shared__ float4 acc[NG][C];
   __shared__ float redm[4], redl[4];
-  const int64_t r = blockIdx.x;
   const int tid = threadIdx.x;
+  const int h = blockIdx.x % A.Hq;
+  const int bt = blockIdx.x / A.Hq;
+  const int tok = bt % A.Sq, b = bt / A.Sq;
+  const int Hw = A.Hw, hw = h / A.G, g = h % A.G, T = A.T;
+  // own run: n0 partial rows, step0 apart, from row0
+  const int64_t step0 = (int64_t)A.G * T * A.Nb[0], step1 = (int64_t)A.G * T * A.Nb[1];
+  int64_t row0, row1 = 0;
+  int n0, n1 = 0;
+  if (A.even > 0) {
+    const int2 e = A.part_tab[b * Hw + hw];
+    row0 = e.x * step0;
+    n0 = e.y;
+  } else {
+    const int nq = A.qtiles[0];
+    n0 = A.splits[0];
+    row0 = ((((int64_t)b * Hw + hw) * nq + (nq - 1 - tok / T)) * n0) * step0;
+  }
+  row0 += (tok % T) * A.G + g;
+  if (A.items1 > 0) {
+    const int nq = A.qtiles[1], tt = (A.Sq + T - 1) / T, qt = (b / A.Nb[1]) * tt + tok / T;
+    n1 = A.splits[1];
+    row1 = A.part_off1 + (((int64_t)hw * nq + (nq - 1 - qt)) * n1) * step1 + ((b % A.Nb[1]) * T + tok % T) * A.G + g;
+  }
+  const int ns = n0 + n1;
+  if (ns == 1) return;  // the attention kernel wrote the row
+  auto part = [&](int s) -> int64_t { return s < n0 ? row0 + s * step0 : row1 + (s - n0) * step1; };
   float m = -INFINITY;
-  for (int s = tid; s < ns; s += 128) m = fmaxf(m, part_ml[s * R + r].x);
+  for (int s = tid; s < ns; s += 128) m = fmaxf(m, A.part_ml[part(s)].x);
   for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
   if ((tid & 31) == 0) redm[tid >> 5] = m;
   __syncthreads();
   const float M = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
   float l = 0.f;
   for (int s = tid; s < ns; s += 128) {
-    const float2 ml = part_ml[s * R + r];
+    const float2 ml = A.part_ml[part(s)];
     // a NaN sum (its maximum may be -inf: NaN scores leave it) goes on to the output
     const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
     wgt[s] = w;
@@ -64,18 +128,18 @@ __global__ void __launch_bounds__(128) mattn_merge_kernel(const float* __restric
   if ((tid & 31) == 0) redl[tid >> 5] = l;
   __syncthreads();
   l = (redl[0] + redl[1]) + (redl[2] + redl[3]);
-  const int g = tid / C, c = tid % C;
+  const int grp = tid / C, c = tid % C;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (g < NG) {
+  if (grp < NG) {
 #pragma unroll 4
-    for (int s = g; s < ns; s += NG) {
+    for (int s = grp; s < ns; s += NG) {
       const float w = wgt[s];
       if (w != 0.f) {
-        const float4 o = *reinterpret_cast<const float4*>(part_o + ((int64_t)s * R + r) * D + 4 * c);
+        const float4 o = *reinterpret_cast<const float4*>(A.part_o + part(s) * D + 4 * c);
         a.x = fmaf(w, o.x, a.x); a.y = fmaf(w, o.y, a.y); a.z = fmaf(w, o.z, a.z); a.w = fmaf(w, o.w, a.w);
       }
     }
-    acc[g][c] = a;
+    acc[grp][c] = a;
   }
   __syncthreads();
   if (tid < C) {
@@ -85,21 +149,21 @@ __global__ void __launch_bounds__(128) mattn_merge_kernel(const float* __restric
     }
     const bool zero = l == 0.f;
     const float inv = zero ? 0.f : 1.0f / l;
-    const int h = (int)(r % Hq);
-    const int64_t bt = r / Hq;
-    const int64_t tok = bt % Sq, b = bt / Sq;
     uint2 w;
     w.x = zero ? 0u : pack16<F16>(a.x * inv, a.y * inv);
     w.y = zero ? 0u : pack16<F16>(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2*>(out + 2 * (b * os.b + (int64_t)h * os.h + tok * os.s + 4 * tid)) = w;
+    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(A.out) +
+                              2 * (b * A.os.b + (int64_t)h * A.os.h + tok * A.os.s + 4 * tid)) = w;
   }
 }
 
 // ------------------------------------------------------------------- plan --
 struct Plan {
-  int nt, G, T, Nb[2], qtiles[2], splits[2], ntp, nto, merged;
+  int form, G, T, Nb[2], qtiles[2], splits[2], ntp, nto, merged, even;
   int64_t items[2];  // CTAs of own and prefix items, splits counted
-  int64_t ids_off, rng_off, ml_off, o_off, bytes;
+  bool parts;        // partial rows and a merge
+  int64_t rows0;     // partial rows of the own items
+  int64_t ids_off, rng_off, rising_off, qrng_off, sorted_off, tab_off, ml_off, o_off, bytes;
 };
 
 static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P, int64_t D,
@@ -122,11 +186,10 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   const bool two = D != 256 && Sq > kBlk && B * Hq * ((Sq + 2 * kBlk - 1) / (2 * kBlk)) >= kSms;
   int64_t hw = Hq;
   if (two) {
-    p->nt = 2;
+    p->form = kPair;
     p->T = kBlk;
     p->qtiles[0] = (int)((Sq + 2 * kBlk - 1) / (2 * kBlk));
   } else {
-    p->nt = 1;
     // pack a group's query heads where that makes fewer tiles
     const int64_t tp = group <= kBlk ? std::min<int64_t>(Sq, kBlk / group) : 0;
     if (group > 1 && tp > 0 && Hkv * ((Sq + tp - 1) / tp) < Hq * ((Sq + kBlk - 1) / kBlk)) {
@@ -149,44 +212,61 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   }
   const int64_t n0 = B * hw * p->qtiles[0], n1 = hw * p->qtiles[1];
   const int64_t t0 = (p->merged ? ntp : 0) + nto, t1 = p->merged ? 0 : ntp;
-  if (p->nt == 1) {
-    // Split the key tiles so that the waves of CTAs are short: a wave costs its longest CTA
-    // (about 1.4 us a tile of head dim 128 and 4 us to start and end); a split also writes
-    // and reads fp32 partial rows and launches the merge (about 4 us).
-    const double tile_us = 0.5 + 0.9 * (double)D / 128.0;
-    const double row_us = (double)(B * Sq * Hq) * (double)D * 8.0 / 5.0e6;
-    double best = 1e30;
-    for (int64_t n = 1; n <= kSms; ++n) {
-      const int64_t len = std::max<int64_t>(1, (std::max(t0, t1) + n - 1) / n);
-      const int64_t s0 = std::max<int64_t>(1, (t0 + len - 1) / len), s1 = std::max<int64_t>(1, (t1 + len - 1) / len);
-      if (s0 + s1 > kMaxSplits) break;
-      const int64_t ctas = n0 * s0 + n1 * s1;
-      const int64_t parts = s0 + (n1 > 0 ? s1 : 0);
-      double c = (double)((ctas + kSms - 1) / kSms) * ((double)len * tile_us + 4.0);
-      if (parts > 1) c += 4.0 + row_us * (double)parts;
-      if (c < best) {
-        best = c;
-        p->splits[0] = (int)s0;
-        p->splits[1] = (int)s1;
+  if (!two) {
+    // many keys for few items: one CTA per SM streams them; else two, of half the size
+    const bool deep = D == 256 || (n1 == 0 && p->qtiles[0] == 1 && n0 * t0 >= 6 * kSms && t0 >= 16);
+    p->form = deep ? kDeep : kSmall;
+    const int64_t cap = deep ? kSms : 2 * kSms;  // CTAs at work at once
+    // prefix items: as many splits as fill the SMs, of four tiles or more
+    if (n1 > 0) p->splits[1] = (int)std::max<int64_t>(1, std::min((t1 + 3) / 4, std::min<int64_t>(cap / n1, kMaxSplits)));
+    if (p->qtiles[0] == 1 && B <= kMaxEven && t0 > 2 && n0 < 2 * cap) {
+      // one query tile per batch element: split by the keys each has (lengths are known on the
+      // device), over a grid of whole waves
+      p->even = (int)(cap * (n0 / cap + 1));
+    } else {
+      // Split the key tiles so that the waves of CTAs are short: a wave costs its longest CTA
+      // (about 2.2 us a tile of head dim 128 with two on an SM, and 5 us to start and end); a
+      // split also writes and reads fp32 partial rows and launches the merge (about 4 us).
+      const double tile_us = D == 256 ? 2.5 : 1.3 + 0.9 * (double)D / 128.0;
+      const double row_us = (double)(B * Sq * Hq) * (double)D * 8.0 / 5.0e6;
+      double best = 1e30;
+      for (int64_t n = 1; n <= kSms; ++n) {
+        const int64_t len = std::max<int64_t>(1, (t0 + n - 1) / n);
+        const int64_t s0 = std::max<int64_t>(1, (t0 + len - 1) / len);
+        if (s0 > kMaxSplits) break;
+        const int64_t ctas = n0 * s0;
+        double c = (double)((ctas + cap - 1) / cap) * ((double)len * tile_us + 5.0);
+        if (s0 > 1) c += 4.0 + row_us * (double)s0;
+        if (c < best) {
+          best = c;
+          p->splits[0] = (int)s0;
+        }
+        if (len == 1) break;
       }
-      if (len == 1) break;
     }
   }
-  p->items[0] = n0 * p->splits[0];
+  p->items[0] = p->even > 0 ? p->even : n0 * p->splits[0];
   p->items[1] = n1 * p->splits[1];
   if (p->items[0] + p->items[1] > 0x7fffffffll) return QF2_ERR_SHAPE;
-  const int64_t parts = p->splits[0] + (n1 > 0 ? p->splits[1] : 0), R = B * Sq * Hq;
-  auto up = [](int64_t x) { return (x + 255) & ~255ll; };
+  p->parts = p->even > 0 || p->splits[0] > 1 || n1 > 0;
+  if (p->parts && B * Sq * Hq > 0x7fffffffll) return QF2_ERR_SHAPE;  // the merge's grid
+  const int64_t per = (int64_t)p->G * p->T;
+  p->rows0 = p->items[0] * per;
+  const int64_t rows = p->rows0 + p->items[1] * per * p->Nb[1];
   int64_t off = 0;
-  p->ids_off = off;
-  if (ids) off += up(B * nto * kBlk * 4);
-  p->rng_off = off;
-  if (ids) off += up(B * nto * 8);
-  p->ml_off = off;
-  if (parts > 1) off += up(parts * R * 8);
-  p->o_off = off;
-  if (parts > 1) off += up(parts * R * D * 4);
-  if (parts > 1 && R > 0x7fffffffll) return QF2_ERR_SHAPE;  // the merge's grid
+  auto take = [&](bool want, int64_t n) {
+    const int64_t at = off;
+    if (want) off += (n + 255) & ~255ll;
+    return at;
+  };
+  p->ids_off = take(ids, B * nto * kBlk * 4);
+  p->rng_off = take(ids, B * nto * 8);
+  p->rising_off = take(ids, B * nto * 4);
+  p->qrng_off = take(ids, B * Sq * 8);
+  p->sorted_off = take(ids, B * 4);
+  p->tab_off = take(p->even > 0, B * hw * 8);
+  p->ml_off = take(p->parts, rows * 8);
+  p->o_off = take(p->parts, rows * D * 4);
   p->bytes = off;
   return QF2_OK;
 }
@@ -213,13 +293,12 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t D, const int64_t 
 }
 
 template <bool F16>
-static void launch_merge(const Args& a, int64_t D, int parts, int64_t R, cudaStream_t s) {
-  const unsigned grid = (unsigned)R;
-  uint8_t* out = reinterpret_cast<uint8_t*>(a.out);
-  if (D == 64) mattn_merge_kernel<64, F16><<<grid, 128, 0, s>>>(a.part_o, a.part_ml, parts, R, out, a.os, a.Sq, a.Hq);
-  else if (D == 96) mattn_merge_kernel<96, F16><<<grid, 128, 0, s>>>(a.part_o, a.part_ml, parts, R, out, a.os, a.Sq, a.Hq);
-  else if (D == 128) mattn_merge_kernel<128, F16><<<grid, 128, 0, s>>>(a.part_o, a.part_ml, parts, R, out, a.os, a.Sq, a.Hq);
-  else mattn_merge_kernel<256, F16><<<grid, 128, 0, s>>>(a.part_o, a.part_ml, parts, R, out, a.os, a.Sq, a.Hq);
+static void launch_merge(const Args& a, int64_t D, int64_t rows, cudaStream_t s) {
+  const unsigned grid = (unsigned)rows;
+  if (D == 64) mattn_merge_kernel<64, F16><<<grid, 128, 0, s>>>(a);
+  else if (D == 96) mattn_merge_kernel<96, F16><<<grid, 128, 0, s>>>(a);
+  else if (D == 128) mattn_merge_kernel<128, F16><<<grid, 128, 0, s>>>(a);
+  else mattn_merge_kernel<256, F16><<<grid, 128, 0, s>>>(a);
 }
 
 }  // namespace mattn
@@ -234,118 +313,151 @@ extern "C" int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_
   return st != QF2_OK ? (int64_t)st : p.bytes;
 }
 
-extern "C" int qf2_masked_attn(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
-                               const void* v, const int64_t* v_strides, void* out, const int64_t* out_strides,
-                               int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t D,
-                               const void* prefix_k, const int64_t* prefix_k_strides, const void* prefix_v,
-                               const int64_t* prefix_v_strides, int64_t P, const qf2_attn_mask* mask, float sm_scale,
-                               int dtype, void* workspace, int64_t workspace_bytes, qf2_stream_t stream) {
+extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
+  if (!args) return QF2_ERR_ARG;
+  const qf2_masked_attn_args& M = *args;
+  const int64_t B = M.B, Hq = M.Hq, Hkv = M.Hkv, Sq = M.Sq, Skv = M.Skv, P = M.P, D = M.D, dtype = M.dtype;
   if (dtype != QF2_BF16 && dtype != QF2_F16) return QF2_ERR_DTYPE;
-  if (!mask) return QF2_ERR_ARG;
-  const qf2_attn_mask& M = *mask;
   const bool ids = M.k_ids != nullptr;
   Plan p;
   int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids);
   if (st != QF2_OK) return st;
   if (B == 0 || Sq == 0) return QF2_OK;
-  if (!q || !q_strides || !out || !out_strides) return QF2_ERR_ARG;
-  if (Skv > 0 && (!k || !k_strides || !v || !v_strides)) return QF2_ERR_ARG;
-  if (P > 0 && (!prefix_k || !prefix_k_strides || !prefix_v || !prefix_v_strides)) return QF2_ERR_ARG;
+  if (!M.q || !M.out) return QF2_ERR_ARG;
+  if (Skv > 0 && (!M.k || !M.v)) return QF2_ERR_ARG;
+  if (P > 0 && (!M.prefix_k || !M.prefix_v)) return QF2_ERR_ARG;
   if ((M.q_ids != nullptr) != ids || (ids && P > 0)) return QF2_ERR_ARG;
   if (M.q_offset_mode < QF2_OFFSET_CONST || M.q_offset_mode > QF2_OFFSET_END ||
       (M.q_offset_mode == QF2_OFFSET_ARRAY && !M.q_offsets))
     return QF2_ERR_ARG;
   if (M.slopes && M.bias_table) return QF2_ERR_ARG;
   if (M.bias_table && (M.bias_reach < 0 || M.bias_reach > kMaxReach)) return QF2_ERR_SHAPE;
-  if (!(M.softcap >= 0.f) || !(sm_scale > 0.f) || isinf(M.softcap) || isinf(sm_scale)) return QF2_ERR_ARG;
-  if (!al16(q) || !al16(out) || (Skv > 0 && (!al16(k) || !al16(v))) || (P > 0 && (!al16(prefix_k) || !al16(prefix_v))))
+  if (!(M.softcap >= 0.0) || !(M.sm_scale > 0.0) || M.softcap > FLT_MAX || M.sm_scale > FLT_MAX) return QF2_ERR_ARG;
+  if (!al16(M.q) || !al16(M.out) || (Skv > 0 && (!al16(M.k) || !al16(M.v))) ||
+      (P > 0 && (!al16(M.prefix_k) || !al16(M.prefix_v))))
     return QF2_ERR_ALIGN;
-  st = check_strides(q_strides, B, Hq, Sq);
-  if (st == QF2_OK) st = check_strides(out_strides, B, Hq, Sq);
-  if (st == QF2_OK && Skv > 0) st = check_strides(k_strides, B, Hkv, Skv);
-  if (st == QF2_OK && Skv > 0) st = check_strides(v_strides, B, Hkv, Skv);
-  if (st == QF2_OK && P > 0) st = check_strides(prefix_k_strides, 1, Hkv, P);
-  if (st == QF2_OK && P > 0) st = check_strides(prefix_v_strides, 1, Hkv, P);
+  st = check_strides(M.q_strides, B, Hq, Sq);
+  if (st == QF2_OK) st = check_strides(M.out_strides, B, Hq, Sq);
+  if (st == QF2_OK && Skv > 0) st = check_strides(M.k_strides, B, Hkv, Skv);
+  if (st == QF2_OK && Skv > 0) st = check_strides(M.v_strides, B, Hkv, Skv);
+  const int64_t spk[3] = {0, M.prefix_k_strides[0], M.prefix_k_strides[1]};
+  const int64_t spv[3] = {0, M.prefix_v_strides[0], M.prefix_v_strides[1]};
+  if (st == QF2_OK && P > 0) st = check_strides(spk, 1, Hkv, P);
+  if (st == QF2_OK && P > 0) st = check_strides(spv, 1, Hkv, P);
   if (st != QF2_OK) return st;
-  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes || !al16(workspace))) return QF2_ERR_WORKSPACE;
+  if (p.bytes > 0 && (!M.workspace || M.workspace_bytes < p.bytes || !al16(M.workspace))) return QF2_ERR_WORKSPACE;
 
   const bool f16 = dtype == QF2_F16;
   Maps m;
   {
-    const int64_t n[3] = {Hq, Sq, B}, s[3] = {q_strides[1], q_strides[2], q_strides[0]};
+    const int64_t n[3] = {Hq, Sq, B}, s[3] = {M.q_strides[1], M.q_strides[2], M.q_strides[0]};
     const uint32_t box[3] = {(uint32_t)p.G, (uint32_t)p.T, 1}, box1[3] = {(uint32_t)p.G, (uint32_t)p.T, (uint32_t)p.Nb[1]};
-    if (!make_map(&m.q, q, D, n, s, box, f16)) return QF2_ERR_ALIGN;
+    if (!make_map(&m.q, M.q, D, n, s, box, f16)) return QF2_ERR_ALIGN;
+    const int64_t so[3] = {M.out_strides[1], M.out_strides[2], M.out_strides[0]};
+    if (!make_map(&m.o, M.out, D, n, so, box, f16)) return QF2_ERR_ALIGN;
     m.q1 = m.q;
-    if (p.Nb[1] > 1 && !make_map(&m.q1, q, D, n, s, box1, f16)) return QF2_ERR_ALIGN;
+    if (p.Nb[1] > 1 && !make_map(&m.q1, M.q, D, n, s, box1, f16)) return QF2_ERR_ALIGN;
   }
   m.k = m.v = m.pk = m.pv = m.q;  // never loaded through where there are no such keys
   const uint32_t kbox[3] = {(uint32_t)kBlk, 1, 1};
   if (Skv > 0) {
     const int64_t n[3] = {Skv, Hkv, B};
-    const int64_t sk[3] = {k_strides[2], k_strides[1], k_strides[0]}, sv[3] = {v_strides[2], v_strides[1], v_strides[0]};
-    if (!make_map(&m.k, k, D, n, sk, kbox, f16) || !make_map(&m.v, v, D, n, sv, kbox, f16)) return QF2_ERR_ALIGN;
+    const int64_t sk[3] = {M.k_strides[2], M.k_strides[1], M.k_strides[0]};
+    const int64_t sv[3] = {M.v_strides[2], M.v_strides[1], M.v_strides[0]};
+    if (!make_map(&m.k, M.k, D, n, sk, kbox, f16) || !make_map(&m.v, M.v, D, n, sv, kbox, f16)) return QF2_ERR_ALIGN;
   }
   if (P > 0) {
     const int64_t n[3] = {P, Hkv, 1};
-    const int64_t sk[3] = {prefix_k_strides[2], prefix_k_strides[1], 0}, sv[3] = {prefix_v_strides[2], prefix_v_strides[1], 0};
-    if (!make_map(&m.pk, prefix_k, D, n, sk, kbox, f16) || !make_map(&m.pv, prefix_v, D, n, sv, kbox, f16))
+    const int64_t sk[3] = {spk[2], spk[1], 0}, sv[3] = {spv[2], spv[1], 0};
+    if (!make_map(&m.pk, M.prefix_k, D, n, sk, kbox, f16) || !make_map(&m.pv, M.prefix_v, D, n, sv, kbox, f16))
       return QF2_ERR_ALIGN;
   }
 
   void* status = nullptr;
   QF2_CUDA_CHECK(cudaGetSymbolAddress(&status, g_status));
-  uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  const bool split = p.splits[0] > 1 || p.items[1] > 0;
+  uint8_t* ws = reinterpret_cast<uint8_t*>(M.workspace);
   Args a{};
-  a.out = out;
-  a.os = S3{out_strides[0], out_strides[1], out_strides[2]};
+  a.out = M.out;
+  a.os = S3{M.out_strides[0], M.out_strides[1], M.out_strides[2]};
   a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Sq = (int)Sq; a.Skv = (int)Skv; a.P = (int)P;
   a.ntp = p.ntp; a.nto = p.nto; a.group = (int)(Hq / Hkv);
   a.G = p.G; a.T = p.T;
   for (int i = 0; i < 2; ++i) { a.Nb[i] = p.Nb[i]; a.qtiles[i] = p.qtiles[i]; a.splits[i] = p.splits[i]; }
+  a.Hw = (int)(Hq / p.G);
+  auto div = [](int64_t d) {
+    Div v{(uint32_t)d, 0, 0};
+    while ((1ll << v.s) < d) ++v.s;
+    v.m = (uint32_t)(((1ull << 32) * ((1ull << v.s) - (uint64_t)d)) / (uint64_t)d + 1);
+    return v;
+  };
+  a.by_G = div(a.G);
+  a.by_T = div(a.T);
+  a.by_group = div(a.group);
+  a.by_Hw = div(a.Hw);
+  a.by_tt = div(a.qtiles[0]);
+  for (int i = 0; i < 2; ++i) {
+    a.by_qtiles[i] = div(a.qtiles[i] > 0 ? a.qtiles[i] : 1);
+    a.by_splits[i] = div(a.splits[i]);
+  }
   a.items1 = (int)p.items[1];
   a.merged = p.merged;
-  a.part_o = split ? reinterpret_cast<float*>(ws + p.o_off) : nullptr;
-  a.part_ml = split ? reinterpret_cast<float2*>(ws + p.ml_off) : nullptr;
+  a.even = p.even;
+  if (p.parts) {
+    a.part_o = reinterpret_cast<float*>(ws + p.o_off);
+    a.part_ml = reinterpret_cast<float2*>(ws + p.ml_off);
+    a.part_tab = reinterpret_cast<int2*>(ws + p.tab_off);
+    a.part_off1 = p.rows0;
+  }
   a.kv_lens = M.kv_lens;
   a.prefix_lens = M.prefix_lens;
   a.q_off = M.q_offsets;
-  a.q_off_mode = M.q_offset_mode;
+  a.q_off_mode = (int)M.q_offset_mode;
   const int64_t far = 1ll << 29;
   a.q_off_const = (int)std::min(std::max(M.q_offset, -far), far);
   a.left = M.left < 0 ? -1 : (int)std::min(M.left, far);
   a.right = M.right < 0 ? -1 : (int)std::min(M.right, far);
   a.q_ids = M.q_ids;
-  a.k_ids = ids ? reinterpret_cast<int32_t*>(ws + p.ids_off) : nullptr;
-  a.k_rng = ids ? reinterpret_cast<int2*>(ws + p.rng_off) : nullptr;
+  if (ids) {
+    a.k_ids = reinterpret_cast<int32_t*>(ws + p.ids_off);
+    a.k_rng = reinterpret_cast<int2*>(ws + p.rng_off);
+    a.q_rng = reinterpret_cast<int2*>(ws + p.qrng_off);
+    a.sorted = reinterpret_cast<int*>(ws + p.sorted_off);
+  }
   const double l2e = 1.4426950408889634;
-  a.scale = (float)((double)sm_scale * l2e);
-  if (M.softcap > 0.f) {
-    a.cap_in = (float)(2.0 * (double)sm_scale / (double)M.softcap * l2e);
-    a.cap_out = (float)((double)M.softcap * l2e);
+  a.scale = (float)(M.sm_scale * l2e);
+  if (M.softcap > 0.0) {
+    a.cap_in = (float)(2.0 * M.sm_scale / M.softcap * l2e);
+    a.cap_out = (float)(M.softcap * l2e);
   }
   a.slopes = M.slopes;
   a.table = M.bias_table;
   a.reach = (int)M.bias_reach;
   a.status = reinterpret_cast<int*>(status);
-  const bool score = M.softcap > 0.f || M.slopes || M.bias_table;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (ids && p.nto > 0) {
-    mattn_ids_kernel<<<dim3((unsigned)p.nto, (unsigned)B), 128, 0, s>>>(
-        M.k_ids, (int)Skv, p.nto, reinterpret_cast<int32_t*>(ws + p.ids_off), reinterpret_cast<int2*>(ws + p.rng_off));
+  const bool score = M.softcap > 0.0 || M.slopes || M.bias_table;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(M.stream);
+  if (ids) {
+    int32_t* k_ids = reinterpret_cast<int32_t*>(ws + p.ids_off);
+    int* rising = reinterpret_cast<int*>(ws + p.rising_off);
+    if (p.nto > 0) {
+      mattn_ids_kernel<<<dim3((unsigned)p.nto, (unsigned)B), 128, 0, s>>>(
+          M.k_ids, (int)Skv, p.nto, k_ids, reinterpret_cast<int2*>(ws + p.rng_off), rising);
+      QF2_LAUNCH_CHECK();
+    }
+    mattn_runs_kernel<<<dim3((unsigned)((Sq + 127) / 128), (unsigned)B), 128, 0, s>>>(
+        M.q_ids, k_ids, rising, (int)Sq, (int)Skv, p.nto, reinterpret_cast<int2*>(ws + p.qrng_off),
+        reinterpret_cast<int*>(ws + p.sorted_off));
     QF2_LAUNCH_CHECK();
   }
   const unsigned grid = (unsigned)(p.items[0] + p.items[1]);
   cudaError_t e;
-  if (D == 64) e = launch_d64(m, a, grid, p.nt, f16, score, s);
-  else if (D == 96) e = launch_d96(m, a, grid, p.nt, f16, score, s);
-  else if (D == 128) e = launch_d128(m, a, grid, p.nt, f16, score, s);
-  else e = launch_d256(m, a, grid, p.nt, f16, score, s);
+  if (D == 64) e = launch_d64(m, a, grid, p.form, f16, score, s);
+  else if (D == 96) e = launch_d96(m, a, grid, p.form, f16, score, s);
+  else if (D == 128) e = launch_d128(m, a, grid, p.form, f16, score, s);
+  else e = launch_d256(m, a, grid, p.form, f16, score, s);
   QF2_CUDA_CHECK(e);
-  if (split) {
-    const int parts = p.splits[0] + (p.items[1] > 0 ? p.splits[1] : 0);
-    if (f16) launch_merge<true>(a, D, parts, B * Sq * Hq, s);
-    else launch_merge<false>(a, D, parts, B * Sq * Hq, s);
+  if (p.parts) {
+    if (f16) launch_merge<true>(a, D, B * Sq * Hq, s);
+    else launch_merge<false>(a, D, B * Sq * Hq, s);
     QF2_LAUNCH_CHECK();
   }
   return QF2_OK;

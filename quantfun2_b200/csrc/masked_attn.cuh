@@ -14,14 +14,24 @@
 //   warp 0      producer: Q once, then K and V tiles by TMA into a ring of slots
 //   warp 1      issues the products: S_t = Q_t K^T, then O_t += P_t V
 //   the rest    softmax, one thread per row, four warps per query tile
-// NT = 2 (long queries): the two tiles' scores are single buffers of their own, so one tile's
-// softmax runs while the tensor cores work for the other, and K and V feed 256 rows.
-// NT = 1 (few query rows, or head dim 256, whose output takes half of tensor memory): the
-// scores are double-buffered, so the next Q K^T runs under the softmax.
+// Three forms:
+//   kPair   long queries, NT = 2: one tile's softmax runs while the tensor cores work for the
+//           other, and K and V feed 256 rows; all of tensor memory, one CTA per SM
+//   kSmall  few query rows on few keys: half of everything, two CTAs per SM, one of which
+//           starts, ends or waits for memory while the other works
+//   kDeep   few query rows on many keys, and head dim 256 (whose output takes half of tensor
+//           memory): one CTA per SM with a deep ring; the scores are double-buffered, so the
+//           next Q K^T runs under the softmax
 // A tile's rows are (batch element, token, query head of a group): one row per token, or all
 // query heads of a kv head packed side by side, so that single tokens read K and V once.
+//
+// Bound for long queries by one chain per tile: scores read, maximum, 128 exponentials a row
+// (the exponent unit takes 16 per SM and cycle, as long as both products), probabilities
+// stored, the last of P V and the next Q K^T.
 #pragma once
 #include "qf2_common.cuh"
+
+#include <type_traits>
 
 namespace qf2 {
 namespace mattn {
@@ -32,18 +42,32 @@ constexpr int kMaxTiles = 8192;       // key tiles of a call (2^20 keys)
 constexpr int kMaxReach = 1024;       // distance table: 2 * reach + 1 entries
 constexpr int kTabPad = 256;          // clamped entries on each side of the table in shared memory
 constexpr float kTau = 8.0f;          // log2 units the running maximum may lag behind
+constexpr int kPart = 96;             // keys whose P V starts before the rest's exponentials are done
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kMaxSplits = 320;     // partial rows of one output row
+constexpr int kMaxSplits = 320;       // partial rows of one output row
+constexpr int kMaxEven = 1024;        // batch elements whose lengths a CTA weighs against each other
 constexpr int kSms = 148;             // B200; sizes the grids and splits (a count, not a limit)
 
 struct S3 { int64_t b, h, s; };
 
+template <int N>
+using Int = std::integral_constant<int, N>;
+
 // NT = 2: three warpgroups, so that registers can move from the first (producer, products,
 // two idle warps) to the softmax ones: launched with 168 a thread (384 x 168 = 64512), then
-// 128 x 56 + 256 x 224 = 64512.  NT = 1: two warps and four, 255 registers each.
+// 128 x 88 + 256 x 208 = 64512.  (88: with 56 the product warp kept its descriptors in local
+// memory.)  Two threads per row, exchanging maxima through shared memory, and a first part of
+// the exponentials taken before the maximum is known were both slower (8192 x 8192, 24 heads of
+// 128: 734 us; 772; 773), as were 1/8 to 3/8 of the exponentials on the FMA pipe.
 constexpr int threads(int nt) { return nt == 2 ? 384 : 192; }
-constexpr int kRegsFew = 56, kRegsSoftmax = 224;
+enum Form { kSmall = 0, kDeep = 1, kPair = 2 };
+constexpr int kRegsFew = 88, kRegsSoftmax = 208;
 
+// Division by a number known on the host: x / d = (umulhi(x, m) + x) >> s for x < 2^31.
+struct Div {
+  uint32_t d, m, s;
+};
+QF2_DEV int div_of(const Div& v, int x) { return (int)((__umulhi((uint32_t)x, v.m) + (uint32_t)x) >> v.s); }
 
 struct Args {
   void* out;
@@ -51,12 +75,18 @@ struct Args {
   int B, Hq, Hkv, Sq, Skv, P;       // own keys, shared prefix keys
   int ntp, nto;                       // key tiles of the prefix and of the own keys
   int group;                          // query heads per kv head
-  // rows of a tile: g heads x T tokens x Nb batch elements ([0] own items, [1] prefix items)
+  // rows of a tile: G heads x T tokens x Nb batch elements ([0] own items, [1] prefix items)
   int G, T, Nb[2], qtiles[2], splits[2];
+  int Hw;                             // head slots: query heads, or kv heads with their group packed
+  Div by_G, by_T, by_group, by_Hw, by_qtiles[2], by_splits[2], by_tt;  // tt: query tiles of a batch element
   int items1;                         // CTAs of prefix items (they come first)
   int merged;                         // own items walk the prefix tiles too
-  float* part_o;                      // split partials: fp32 rows and (max, sum), or null
+  int even;                           // > 0: CTAs of the own items, split by what each has to read
+  // split partials: fp32 rows, their (max, sum), and the slots of an item where even > 0
+  float* part_o;                      // null: no splits
   float2* part_ml;
+  int2* part_tab;
+  int64_t part_off1;                  // first row of the prefix items' slots
   // mask
   const int32_t* kv_lens;
   const int32_t* prefix_lens;
@@ -67,33 +97,38 @@ struct Args {
   const int32_t* q_ids;
   const int32_t* k_ids;               // padded copy [B][nto * 128] (pad -2)
   const int2* k_rng;                  // [B][nto] least and greatest id of a key tile
+  const int2* q_rng;                  // [B][Sq] keys of the row's id, where they are in order
+  const int* sorted;                  // [B] key ids in order: q_rng holds
   // scores
-  float scale;                        // plain: sm_scale * log2 e; else see score_args
-  float cap_in, cap_out;              // cap > 0: 2 scale log2e / cap, cap log2e; else 0
+  float scale;                        // sm_scale * log2 e
+  float cap_in, cap_out;              // cap > 0: 2 scale log2 e / cap, cap log2 e; else 0
   const float* slopes;
   const float* table;                 // [Hq][2 * reach + 1]
   int reach;
   int* status;
 };
 
-template <int D, int NT>
+template <int D, int FORM>
 struct Smem {
+  static constexpr bool two = FORM == kSmall;           // two CTAs per SM
+  static constexpr int nt = FORM == kPair ? 2 : 1;
   static constexpr int nb = (D + 63) / 64;            // 64-channel columns
   static constexpr int op = nb * kTile;                // bytes of a 128-row operand
-  // ring slots (K and V tiles alternate); every variant stays above half of the SM's shared
-  // memory, so one CTA is resident and its 512 TMEM columns are free when it starts
-  static constexpr int slots = D == 256 ? 2 : (D == 64 ? 8 : (NT == 2 ? 4 : 5));
-  static constexpr int q = 0;
-  static constexpr int ring = NT * op;
+  // ring slots: K and V tiles alternate
+  static constexpr int slots = D == 256 ? 2 : (D == 64 ? (two ? 4 : 8) : (two ? 2 : (FORM == kPair ? 4 : 5)));
+  static constexpr int q = 0;                           // Q; the output goes out through it
+  static constexpr int ring = nt * op;
   static constexpr int tab = ring + slots * op;        // distance table with its pads
   static constexpr int tab_floats = 2 * kMaxReach + 1 + 2 * kTabPad;
   static constexpr int bits = tab + ((tab_floats * 4 + 15) & ~15);
   static constexpr int bars = bits + kMaxTiles / 8;
-  static constexpr int nbars = 1 + 2 * slots + 2 + 2 + 2 + 1;
+  static constexpr int nbars = 1 + 2 * slots + 2 + 4 + 2 + 1;
   static constexpr int misc = bars + nbars * 8;
-  static constexpr int total = misc + 64;
-  static_assert(total <= 227 * 1024, "shared memory");
-  static_assert(total > 114 * 1024, "one CTA per SM");
+  static constexpr int total = misc + 16 + 8 * 8 * 4;
+  // TMEM: 512 columns where one CTA has the SM (no second fits beside it), else 256 each
+  static constexpr int cols = two ? 256 : 512;
+  static_assert(total <= (two ? 113 : 227) * 1024, "shared memory");
+  static_assert(two || total > 114 * 1024, "one CTA per SM");
 };
 
 template <bool F16>
@@ -123,17 +158,18 @@ QF2_DEV float bias_log2(float b) {
 // bits [0, n) of a 32-bit word
 QF2_DEV uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
-// walks the set bits of the active-tile words (every role walks the same sequence)
-struct TileIter {
-  const uint32_t* w;
+// The key tiles of a CTA in order: two runs [a0, a1), [b0, b1) of tile numbers, or (ids out of
+// order) the set bits of words in shared memory; every role walks the same sequence.
+struct Tiles {
+  int a0, na, b0, j;
+  const uint32_t* w;  // null: runs
   int word;
   uint32_t rest;
-  QF2_DEV void init(const uint32_t* bits, int first_word, uint32_t first_rest) {
-    w = bits;
-    word = first_word;
-    rest = first_rest;
-  }
   QF2_DEV int next() {
+    if (w == nullptr) {
+      const int i = j++;
+      return i < na ? a0 + i : b0 + i - na;
+    }
     while (rest == 0) rest = w[++word];
     const int t = word * 32 + __ffs(rest) - 1;
     rest &= rest - 1;
@@ -141,20 +177,116 @@ struct TileIter {
   }
 };
 
+// What the rows of batch element b see by their lengths and offsets.
+struct Span { int off, len, pre; };  // own offset of query 0, end of the keys, prefix (positions)
+QF2_DEV Span span_of(const Args& A, int b) {
+  Span s;
+  int len = A.Skv;
+  if (A.kv_lens) len = min(max(A.kv_lens[b], 0), A.Skv);
+  int off = A.q_off_const;
+  if (A.q_off_mode == 1) off = A.q_off[b];
+  off = min(max(off, -(1 << 29)), 1 << 29);
+  if (A.q_off_mode == 2) off = len - A.Sq;
+  s.len = len + A.P;
+  s.off = A.P + off;
+  s.pre = A.prefix_lens ? min(max(A.prefix_lens[b], 0), s.len) : 0;
+  return s;
+}
+
 // SCORE: scores are capped and / or biased (log2 units before the mask); else the scale is
 // folded into the exponent
-template <int D, int NT, bool F16, bool SCORE>
-__global__ void __launch_bounds__(threads(NT), 1)
+template <int D, int FORM, bool F16, bool SCORE>
+__global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall ? 2 : 1)
     masked_attn_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmq1,
+                       const __grid_constant__ CUtensorMap tmo,
                        const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                        const __grid_constant__ CUtensorMap tmpk, const __grid_constant__ CUtensorMap tmpv,
                        const __grid_constant__ Args A) {
-  using L = Smem<D, NT>;
+  using L = Smem<D, FORM>;
+  constexpr int NT = L::nt;
+  constexpr bool DB = FORM == kDeep;   // scores double-buffered
   constexpr int kThreads = threads(NT);
   constexpr int W0 = NT == 2 ? 4 : 2;  // first softmax warp
   constexpr int NS = L::slots;
-  constexpr uint32_t kTmemO = 256;  // S at 0 and 128 (P over its first 64 columns), O from 256
+  // S of tile t (or buffer) at t * 128, P over its first 64 columns; O behind them
+  constexpr uint32_t kTmemO = L::two ? 128 : 256;
   extern __shared__ __align__(1024) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // ------------------------------------------------------------- work item --
+  if (threadIdx.x == 0) {
+    prefetch_tmap(&tmq);
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
+  }
+  int x = blockIdx.x;
+  const int kind = x < A.items1 ? 1 : 0;
+  if (!kind) x -= A.items1;
+  const int T = A.T, Nb = A.Nb[kind], G = A.G, Hw = A.Hw;
+  int nsplit = A.splits[kind], split, qt = 0, hw, b0;
+  const int slot = x;
+  if (!kind && A.even > 0) {
+    // One query tile per batch element, lengths known on the device only: the tiles(b) key tiles
+    // of an item are split over ceil(tiles(b) / len) CTAs, len such that all fit the grid.
+    auto tiles_of = [&](int b) -> int {
+      const Span s = span_of(A, b);
+      const int base = A.merged ? 0 : A.P;
+      const int l = max(A.left < 0 ? 0 : s.off - A.left, base);
+      const int h = A.right < 0 ? s.len : min(s.off + A.Sq + A.right, s.len);
+      int n = h > l ? (h - base + kBlk - 1) / kBlk - (l - base) / kBlk : 0;
+      const int p = min(s.pre, l);
+      if (p > base) n += (p - base + kBlk - 1) / kBlk;
+      return max(n, 1);
+    };
+    const int mine = lane < A.B ? tiles_of(lane) : 0;
+    float all = (float)mine;
+    for (int b = lane + 32; b < A.B; b += 32) all += (float)tiles_of(b);
+    for (int d = 16; d; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+    // rounded up beyond the sum's own rounding, so that the CTAs never outnumber the grid
+    const int len = max((int)(__fdividef(all * (float)Hw, (float)(A.even - Hw * A.B)) * 1.0001f) + 1, 2);
+    int before = 0, b = -1, c_b = 1, first = 0;
+    for (int bb = 0; bb < A.B && b < 0; bb += 32) {
+      const int tl = bb == 0 ? mine : (bb + lane < A.B ? tiles_of(bb + lane) : 0);
+      const int c = min((int)((uint32_t)(tl + len - 1) / (uint32_t)len), kMaxSplits);
+      int sum = c;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += o;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, (before + sum) * Hw > x);
+      if (hit) {
+        const int l = __ffs(hit) - 1;
+        b = bb + l;
+        c_b = __shfl_sync(0xffffffffu, c, l);
+        first = (before + __shfl_sync(0xffffffffu, sum, l) - c_b) * Hw;
+      } else {
+        before += __shfl_sync(0xffffffffu, sum, 31);
+      }
+    }
+    if (b < 0) return;  // the grid has room for the most that rounding up can take
+    b0 = b;
+    nsplit = c_b;
+    hw = (int)((uint32_t)(x - first) / (uint32_t)nsplit);
+    split = x - first - hw * nsplit;
+    if (threadIdx.x == 0 && split == 0) A.part_tab[b * Hw + hw] = make_int2(x, nsplit);
+  } else {
+    const int y = div_of(A.by_splits[kind], x);
+    split = x - y * nsplit;
+    const int nq = A.qtiles[kind], z = div_of(A.by_qtiles[kind], y);
+    qt = nq - 1 - (y - z * nq);  // the last rows first: a causal mask gives them the most keys
+    b0 = div_of(A.by_Hw, z);
+    hw = z - b0 * Hw;
+  }
+  const int hk = G > 1 ? hw : div_of(A.by_group, hw);
+  int tok0 = qt * NT * T;
+  if (kind) {  // prefix items: tiles over (batch elements, tokens)
+    const int e = div_of(A.by_tt, qt);
+    b0 = e * Nb;
+    tok0 = (qt - e * A.qtiles[0]) * T;
+  }
+  const int t_lo = kind ? 0 : (A.merged ? 0 : A.ntp);
+  const int t_hi = kind ? A.ntp : A.ntp + A.nto;
+
   if (smem_u32(smem) & 1023) {  // the 128-byte swizzle needs 1024-byte aligned tiles
     if (threadIdx.x == 0) atomicExch(A.status, kDevBadLaunch);
     return;
@@ -167,119 +299,88 @@ __global__ void __launch_bounds__(threads(NT), 1)
   uint64_t* bar_q = bars;
   uint64_t* bar_full = bars + 1;            // [NS]
   uint64_t* bar_empty = bar_full + NS;      // [NS]
-  uint64_t* bar_s = bar_empty + NS;         // [2] scores of query tile t (NT = 2) / buffer j & 1
-  uint64_t* bar_p = bar_s + 2;              // [2] probabilities written
-  uint64_t* bar_o = bar_p + 2;              // [2] NT = 2: O_t complete; NT = 1: PV of tile j, [j & 1]
+  uint64_t* bar_s = bar_empty + NS;         // [2] scores of query tile t (DB: buffer j & 1)
+  uint64_t* bar_p = bar_s + 2;              // [2][2] probabilities written: first kPart keys, all
+  uint64_t* bar_o = bar_p + 4;              // [2] O_t complete; DB: PV of key tile j, [j & 1]
   uint64_t* bar_drain = bar_o + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::misc + 4);
-  // rows of the CTA: least first key, greatest end, greatest prefix, least and greatest id
-  int* red = reinterpret_cast<int*>(smem + L::misc + 8);
+  int* red = reinterpret_cast<int*>(smem + L::misc + 16);  // [softmax warp][8]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  // ------------------------------------------------------------- work item --
-  int x = blockIdx.x;
-  const int kind = x < A.items1 ? 1 : 0;
-  if (!kind) x -= A.items1;
-  const int nsplit = A.splits[kind];
-  const int split = x % nsplit;
-  x /= nsplit;
-  const int nq = A.qtiles[kind];
-  const int qt = nq - 1 - x % nq;  // the last rows first: a causal mask gives them the most keys
-  x /= nq;
-  const int Hw = A.Hq / A.G;       // head slots: query heads, or kv heads with their group packed
-  const int hw = x % Hw, b_item = x / Hw;
-  const int hk = A.G > 1 ? hw : hw / A.group;
-  const int T = A.T, Nb = A.Nb[kind], G = A.G;
-  int b0 = b_item, tok0 = qt * NT * T;
-  if (kind) {  // prefix items: tiles over (batch elements, tokens)
-    const int tt = (A.Sq + T - 1) / T;
-    b0 = (qt / tt) * Nb;
-    tok0 = (qt % tt) * T;
-  }
-  const int t_lo = kind ? 0 : (A.merged ? 0 : A.ntp);
-  const int t_hi = kind ? A.ntp : A.ntp + A.nto;
-
-  if (threadIdx.x == 0) {
-    mbar_init(bar_q, 1);
-    for (int s = 0; s < NS; ++s) {
-      mbar_init(bar_full + s, 1);
-      mbar_init(bar_empty + s, 1);
+  if (warp == 0) {
+    if (lane == 0) {
+      mbar_init(bar_q, 1);
+      for (int s = 0; s < NS; ++s) {
+        mbar_init(bar_full + s, 1);
+        mbar_init(bar_empty + s, 1);
+      }
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(bar_s + s, 1);
+        mbar_init(bar_p + 2 * s, 4);
+        mbar_init(bar_p + 2 * s + 1, 4);
+        mbar_init(bar_o + s, 1);
+      }
+      mbar_init(bar_drain, 1);
+      *abort_flag = 0;
+      fence_mbar_init();
+      // Q is on its way while the masks are worked out
+      mbar_arrive_expect_tx(bar_q, (uint32_t)(NT * L::nb) * 128u * (uint32_t)(G * T * Nb));
+      for (int t = 0; t < NT; ++t)
+        for (int c = 0; c < L::nb; ++c)
+          tma_load_4d(sQ + t * L::op + c * kTile, kind ? &tmq1 : &tmq, c * 64, G > 1 ? hw * G : hw, tok0 + t * T, b0,
+                      bar_q);
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(bar_s + s, 1);
-      mbar_init(bar_p + s, 4);
-      mbar_init(bar_o + s, 1);
-    }
-    mbar_init(bar_drain, 1);
-    *abort_flag = 0;
-    red[0] = 0x7fffffff; red[1] = 0; red[2] = 0; red[3] = 0x7fffffff; red[4] = -1;
-    fence_mbar_init();
-  }
-  if (warp == 1) {
-    tmem_alloc(tmem_slot, 512);
+    __syncwarp();
+  } else if (warp == 1) {
+    tmem_alloc(tmem_slot, L::cols);
     tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-
-  if (warp == 0 && lane == 0) {  // Q is on its way while the masks are worked out
-    prefetch_tmap(&tmk);
-    prefetch_tmap(&tmv);
-    mbar_arrive_expect_tx(bar_q, (uint32_t)(NT * L::nb) * 128u * (uint32_t)(G * T * Nb));
-    for (int t = 0; t < NT; ++t)
-      for (int c = 0; c < L::nb; ++c)
-        tma_load_4d(sQ + t * L::op + c * kTile, kind ? &tmq1 : &tmq, c * 64, G > 1 ? hw * G : hw, tok0 + t * T, b0,
-                    bar_q);
   }
 
   // ------------------------------------------------------------- row masks --
-  // this thread's row (softmax warps): position, head, and the keys it sees:
-  // [lo, hi) or [0, pre), with the id `id`
+  // this thread's row (softmax warps): position, head, and the keys it sees: [lo, hi) or
+  // [plo, pre), and where ids are out of order only those of its id
   const int tile = NT == 2 ? (warp - W0) >> 2 : 0;
   const int quarter = warp & 3;
   const int row = quarter * 32 + lane;
-  int rb = 0, rtok = 0, rh = 0, qpos = 0, lo = 0, hi = 0, pre = 0, id = 0;
+  int rb = 0, rtok = 0, rh = 0, qpos = 0, lo = 0, hi = 0, plo = 0, pre = 0, id = 0;
   bool exists = false;
+  const bool by_id = A.q_ids != nullptr && A.sorted[b0] == 0;
   if (warp >= W0) {
-    const int g = row % G, xr = row / G;
-    rtok = tok0 + tile * T + xr % T;
-    rb = b0 + xr / T;
+    const int xr = div_of(A.by_G, row), g = row - xr * G;
+    const int xb = div_of(A.by_T, xr);
+    rtok = tok0 + tile * T + xr - xb * T;
+    rb = b0 + xb;
     rh = G > 1 ? hw * G + g : hw;
-    exists = xr / T < Nb && rb < A.B && rtok < A.Sq;
+    exists = xb < Nb && rb < A.B && rtok < A.Sq;
     const int bc = min(rb, A.B - 1);
-    int len = A.Skv;
-    if (A.kv_lens) len = min(max(A.kv_lens[bc], 0), A.Skv);
-    int off = A.q_off_const;
-    if (A.q_off_mode == 1) off = A.q_off[bc];
-    off = min(max(off, -(1 << 29)), 1 << 29);
-    if (A.q_off_mode == 2) off = len - A.Sq;
-    len += A.P;
-    qpos = A.P + off + rtok;
+    const Span s = span_of(A, bc);
+    qpos = s.off + rtok;
     lo = A.left < 0 ? 0 : max(qpos - A.left, 0);
-    hi = A.right < 0 ? len : min(max(qpos + A.right + 1, 0), len);
-    if (A.prefix_lens) pre = min(max(A.prefix_lens[bc], 0), len);
-    bool sees = exists && (lo < hi || pre > 0);
-    if (A.q_ids) {
-      id = exists ? A.q_ids[(int64_t)bc * A.Sq + rtok] : -1;
-      sees = sees && id >= 0;
+    hi = A.right < 0 ? s.len : min(max(qpos + A.right + 1, 0), s.len);
+    pre = s.pre;
+    bool sees = exists;
+    if (A.q_ids && exists) {
+      const int64_t i = (int64_t)bc * A.Sq + rtok;
+      if (by_id) {
+        id = A.q_ids[i];
+        sees = id >= 0;
+      } else {
+        const int2 r = A.q_rng[i];
+        lo = max(lo, r.x);
+        hi = min(hi, r.y);
+        plo = r.x;
+        pre = min(pre, r.y);
+      }
     }
-    if (!sees) { lo = 0; hi = 0; pre = 0; }
-    const int wlo = __reduce_min_sync(0xffffffffu, sees && lo < hi ? lo : 0x7fffffff);
-    const int whi = __reduce_max_sync(0xffffffffu, hi);
-    const int wpre = __reduce_max_sync(0xffffffffu, pre);
-    const int wi0 = __reduce_min_sync(0xffffffffu, sees ? id : 0x7fffffff);
-    const int wi1 = __reduce_max_sync(0xffffffffu, sees ? id : -1);
-    if (lane == 0) {
-      atomicMin(red + 0, wlo);
-      atomicMax(red + 1, whi);
-      atomicMax(red + 2, wpre);
-      atomicMin(red + 3, wi0);
-      atomicMax(red + 4, wi1);
-    }
+    if (!sees || lo >= hi) lo = hi = 0;
+    if (!sees || plo >= pre) plo = pre = 0;
+    const bool blind = !(lo < hi || plo < pre);
+    const int big = 0x7fffffff;
+    const int v[6] = {__reduce_min_sync(0xffffffffu, lo < hi ? lo : big), __reduce_max_sync(0xffffffffu, hi),
+                      __reduce_min_sync(0xffffffffu, plo < pre ? plo : big), __reduce_max_sync(0xffffffffu, pre),
+                      __reduce_min_sync(0xffffffffu, blind ? big : id), __reduce_max_sync(0xffffffffu, blind ? -1 : id)};
+    if (lane == 0)
+      for (int i = 0; i < 6; ++i) red[(warp - W0) * 8 + i] = v[i];
   }
   // the head's distance table with clamped pads (log2 units), where the rows of a warp are
   // consecutive positions of one head
@@ -290,134 +391,190 @@ __global__ void __launch_bounds__(threads(NT), 1)
     for (int i = threadIdx.x; i < n + 2 * kTabPad; i += kThreads)
       tab[i] = bias_log2(__ldg(src + min(max(i - kTabPad, 0), n - 1)));
   }
+  tc_fence_before();
   __syncthreads();
-  const int ulo = red[0], uhi = red[1], upre = red[2], uid0 = red[3], uid1 = red[4];
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  // what any row of the CTA sees: [ulo, uhi), [uplo, upre), ids uid0 .. uid1
+  int ulo = 0x7fffffff, uhi = 0, uplo = 0x7fffffff, upre = 0, uid0 = 0x7fffffff, uid1 = -1;
+#pragma unroll
+  for (int w = 0; w < 4 * NT; ++w) {
+    ulo = min(ulo, red[w * 8]);
+    uhi = max(uhi, red[w * 8 + 1]);
+    uplo = min(uplo, red[w * 8 + 2]);
+    upre = max(upre, red[w * 8 + 3]);
+    uid0 = min(uid0, red[w * 8 + 4]);
+    uid1 = max(uid1, red[w * 8 + 5]);
+  }
 
   // ---------------------------------------------------------- active tiles --
-  // position of a key tile's first key and the end of its store
+  // position of a key tile's first key, the end of its store, and the tile of a position
   auto tile_pos = [&](int t) -> int { return t < A.ntp ? t * kBlk : A.P + (t - A.ntp) * kBlk; };
   auto tile_end = [&](int t) -> int { return t < A.ntp ? A.P : 0x7fffffff; };
-  const int2* krng = A.k_rng ? A.k_rng + (int64_t)b0 * A.nto : nullptr;
-  const int w_lo = t_lo >> 5, w_hi = (t_hi + 31) >> 5;
-  for (int w = w_lo + warp; w < w_hi; w += kThreads / 32) {
-    const int t = w * 32 + lane;
-    bool act = t >= t_lo && t < t_hi;
-    if (act) {
-      const int p0 = tile_pos(t), p1 = min(p0 + kBlk, tile_end(t));
-      act = (p0 < uhi && p1 > ulo) || p0 < upre;
-      if (act && krng) {
-        const int2 r = krng[t - A.ntp];
-        act = r.y >= uid0 && r.x <= uid1;
-      }
-    }
-    const uint32_t word = __ballot_sync(0xffffffffu, act);
-    if (lane == 0) bits[w] = word;
-  }
-  __syncthreads();
+  auto tile_at = [&](int p) -> int { return p < A.P ? p / kBlk : A.ntp + (p - A.P) / kBlk; };
+  const int2* krng = by_id ? A.k_rng + (int64_t)b0 * A.nto : nullptr;
   int n = 0;  // tiles of this CTA
-  TileIter it;
+  Tiles it;
   {
-    int total = 0;
-    for (int w = w_lo + lane; w < w_hi; w += 32) total += __popc(bits[w]);
-    total = __reduce_add_sync(0xffffffffu, total);
-    const int f = (int)((int64_t)total * split / nsplit), e = (int)((int64_t)total * (split + 1) / nsplit);
-    n = e - f;
-    int skip = f, w = w_lo;
-    uint32_t rest = w < w_hi ? bits[w] : 0;
-    if (n > 0) {
+    int total, w_lo = t_lo >> 5;
+    // the two runs in order, without what they share
+    int a0 = t_lo, a1 = t_lo, c0 = t_lo, c1 = t_lo;
+    if (uplo < upre) a0 = max(tile_at(uplo), t_lo), a1 = min(tile_at(upre - 1) + 1, t_hi);
+    if (ulo < uhi) c0 = max(tile_at(ulo), t_lo), c1 = min(tile_at(uhi - 1) + 1, t_hi);
+    if (a0 >= a1 || (c0 < c1 && c0 < a0)) {
+      const int s0 = a0, s1 = a1;
+      a0 = c0, a1 = c1, c0 = s0, c1 = s1;
+    }
+    c0 = max(c0, a1);
+    const int na = max(a1 - a0, 0), nc = max(c1 - c0, 0);
+    if (krng) {
+      const int w_hi = (t_hi + 31) >> 5;
+      for (int w = w_lo + warp; w < w_hi; w += kThreads / 32) {
+        const int t = w * 32 + lane;
+        bool act = (t >= a0 && t < a1) || (t >= c0 && t < c1);
+        if (act) {
+          const int2 r = krng[t - A.ntp];
+          act = r.y >= uid0 && r.x <= uid1;
+        }
+        const uint32_t word = __ballot_sync(0xffffffffu, act);
+        if (lane == 0) bits[w] = word;
+      }
+      __syncthreads();
+      total = 0;
+      for (int w = w_lo + lane; w < w_hi; w += 32) total += __popc(bits[w]);
+      total = __reduce_add_sync(0xffffffffu, total);
+    } else {
+      total = na + nc;
+    }
+    // (at most 2^13 tiles and kMaxSplits splits)
+    int f = 0;
+    n = total;
+    if (nsplit > 1) {
+      f = (int)((uint32_t)(total * split) / (uint32_t)nsplit);
+      n = (int)((uint32_t)(total * (split + 1)) / (uint32_t)nsplit) - f;
+    }
+    it.a0 = a0;
+    it.na = na;
+    it.b0 = c0;
+    it.j = f;
+    it.w = nullptr;
+    it.word = w_lo;
+    it.rest = 0;
+    if (krng && n > 0) {
+      int skip = f, w = w_lo;
+      uint32_t rest = bits[w];
       while (skip >= __popc(rest)) {
         skip -= __popc(rest);
         rest = bits[++w];
       }
       for (; skip > 0; --skip) rest &= rest - 1;
+      it.w = bits;
+      it.word = w;
+      it.rest = rest;
     }
-    it.init(bits, w, rest);
   }
 
   auto fail = [&](int code) {
     atomicExch(A.status, code);
     *abort_flag = 1;
   };
+  // warp-wide bounded wait; the abort flag is looked at only while the barrier is not there
   auto wwait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    const bool w = mbar_wait(bar, parity) && (*abort_flag == 0);
-    return __all_sync(0xffffffffu, w);
+    const uint32_t a = smem_u32(bar);
+    if (__all_sync(0xffffffffu, mbar_try_wait(a, parity))) return true;
+    const long long t0 = clock64();
+    while (true) {
+      if (__all_sync(0xffffffffu, mbar_try_wait(a, parity))) return true;
+      if (__any_sync(0xffffffffu, *abort_flag != 0 || clock64() - t0 > kWaitClocks)) return false;
+    }
   };
 
   if (warp < W0) {
-  if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
-  if (warp == 0) {
-    // ------------------------------------------------------------ producer --
-    int issued = 0;
-    bool ok = true;
-    for (int j = 0; ok && j < n; ++j) {
-      const int t = it.next();
-      const bool px = t < A.ntp;
-      const int y = (px ? t : t - A.ntp) * kBlk;
+    if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
+    if (warp == 0) {
+      // ---------------------------------------------------------- producer --
+      int issued = 0;
+      bool ok = true;
+      for (int j = 0; ok && j < n; ++j) {
+        const int t = it.next();
+        const bool px = t < A.ntp;
+        const int y = (px ? t : t - A.ntp) * kBlk;
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv) {
-        const int i = 2 * j + kv, s = i % NS;
-        if (!wwait(bar_empty + s, ((i / NS) & 1) ^ 1)) {
-          if (lane == 0) fail(kDevTimeoutProducer);
-          ok = false;
-          break;
+        for (int kv = 0; kv < 2; ++kv) {
+          const int i = 2 * j + kv, s = i % NS;
+          if (!wwait(bar_empty + s, ((i / NS) & 1) ^ 1)) {
+            if (lane == 0) fail(kDevTimeoutProducer);
+            ok = false;
+            break;
+          }
+          if (lane == 0) {
+            const CUtensorMap* m = kv ? (px ? &tmpv : &tmv) : (px ? &tmpk : &tmk);
+            uint8_t* dst = sR + s * L::op;
+            mbar_arrive_expect_tx(bar_full + s, L::op);
+            for (int c = 0; c < L::nb; ++c) tma_load_4d(dst + c * kTile, m, c * 64, y, hk, px ? 0 : b0, bar_full + s);
+          }
+          __syncwarp();
+          issued = i + 1;
         }
-        if (lane == 0) {
-          const CUtensorMap* m = kv ? (px ? &tmpv : &tmv) : (px ? &tmpk : &tmk);
-          uint8_t* dst = sR + s * L::op;
-          mbar_arrive_expect_tx(bar_full + s, L::op);
-          for (int c = 0; c < L::nb; ++c) tma_load_4d(dst + c * kTile, m, c * 64, y, hk, px ? 0 : b0, bar_full + s);
-        }
-        __syncwarp();
-        issued = i + 1;
       }
-    }
-    // copies in flight land before the CTA ends (Q also where no key tile was active)
-    if (lane == 0) {
-      mbar_wait(bar_q, 0);
-      if (*abort_flag)
-        for (int i = issued > NS ? issued - NS : 0; i < issued; ++i) mbar_wait(bar_full + (i % NS), (i / NS) & 1);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // ----------------------------------------------------------- products --
-    if (n > 0) {
+      // copies in flight land before the CTA ends (Q also where no key tile was active)
+      if (lane == 0) {
+        mbar_wait(bar_q, 0);
+        if (*abort_flag)
+          for (int i = issued > NS ? issued - NS : 0; i < issued; ++i) mbar_wait(bar_full + (i % NS), (i / NS) & 1);
+      }
+      __syncwarp();
+    } else if (warp == 1 && n > 0) {
+      // ---------------------------------------------------------- products --
       constexpr uint32_t ab = F16 ? 0u : 1u;
       constexpr uint32_t idesc_qk = make_idesc(1, ab, ab, 0, 0, kBlk, kBlk);  // K-major x K-major
       constexpr uint32_t idesc_pv = make_idesc(1, ab, ab, 0, 1, kBlk, D);     // P x MN-major V
-      const uint32_t aQ = smem_u32(sQ), aR = smem_u32(sR);
+      const uint32_t aR = smem_u32(sR);
       auto slot_full = [&](int i) -> bool { return wwait(bar_full + i % NS, (i / NS) & 1); };
+      // descriptors differ from these in the start address alone (16-byte units in the low bits);
+      // one elected lane issues, with the warp converged around it (a branch on lane 0 and
+      // descriptors built anew took 100 cycles a product of 64: 946 against 737 us, 8192 x 8192,
+      // 24 heads of 128)
+      const uint64_t dq0 = sdesc_sw128_kmajor(smem_u32(sQ)), dk0 = sdesc_sw128_kmajor(aR);
+      const uint64_t dv0 = sdesc_sw128_mnmajor(aR, kTile, 1024);
+      // scores of key tile j for query tile t; the key slot is free after the last tile's
       auto issue_qk = [&](int t, int buf, int j) {
-        if (lane == 0) {
-          const uint32_t q = aQ + t * L::op, k = aR + (2 * j % NS) * L::op;
+        const int slot = 2 * j % NS;
+        const uint64_t q = dq0 + (uint64_t)(t * (L::op >> 4)), k = dk0 + (uint64_t)(slot * (L::op >> 4));
+        const uint32_t d = tmem + buf * kBlk;
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * kTile + (kk & 3) * 32;
-            mma_f16(tmem + buf * kBlk, sdesc_sw128_kmajor(q + off), sdesc_sw128_kmajor(k + off), idesc_qk,
-                    kk > 0 ? 1u : 0u);
+            const uint32_t off = ((kk >> 2) * kTile + (kk & 3) * 32) >> 4;
+            mma_f16(d, q + off, k + off, idesc_qk, kk > 0 ? 1u : 0u);
           }
           tc_commit(bar_s + buf);
+          if (t == NT - 1) tc_commit(bar_empty + slot);
         }
         __syncwarp();
       };
-      auto issue_pv = [&](int t, int buf, int j) {
-        if (lane == 0) {
-          const uint32_t v = aR + ((2 * j + 1) % NS) * L::op;
+      // 16 keys per step: 8 TMEM columns of P, 16 rows of V
+      auto issue_pv = [&](int t, int buf, int j, auto k0, auto k1) {
+        const uint64_t v = dv0 + (uint64_t)(((2 * j + 1) % NS) * (L::op >> 4));
+        const uint32_t d = tmem + kTmemO + t * 128, pa = tmem + buf * kBlk;
+        const uint32_t first = j > 0 ? 1u : 0u;
+        if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)  // 16 keys per step: 8 TMEM columns of P, 16 rows of V
-            mma_f16_tmem_a(tmem + kTmemO + t * 128, tmem + buf * kBlk + kk * 8,
-                           sdesc_sw128_mnmajor(v + kk * 16 * 128, kTile, 1024), idesc_pv, (j > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = k0; kk < k1; ++kk)
+            mma_f16_tmem_a(d, pa + kk * 8, v + (uint64_t)(kk * 128), idesc_pv, kk > 0 ? 1u : first);
+          if (k1 == kBlk / 16) {
+            if (t == NT - 1) tc_commit(bar_empty + (2 * j + 1) % NS);
+            if (DB) tc_commit(bar_o + (j & 1));
+            else if (j + 1 == n) tc_commit(bar_o + t);
+          }
         }
-        __syncwarp();
-      };
-      auto release = [&](int i) {
-        if (lane == 0) tc_commit(bar_empty + i % NS);
         __syncwarp();
       };
       // keys that no row of the CTA sees weigh nothing, yet 0 * NaN would reach every row:
       // their V rows are cleared (a cache's unused end, padding, another text)
       auto clear_dead = [&](int t, int j) {
         const int p0 = tile_pos(t), p1 = min(p0 + kBlk, tile_end(t));
-        bool all = (p1 <= uhi && p0 >= ulo) || p1 <= upre;
+        bool all = (p1 <= uhi && p0 >= ulo) || (p1 <= upre && p0 >= uplo);
         const int32_t* ids = nullptr;
         if (krng) {
           const int2 r = krng[t - A.ntp];
@@ -428,7 +585,7 @@ __global__ void __launch_bounds__(threads(NT), 1)
         uint8_t* v = sR + ((2 * j + 1) % NS) * L::op;
         for (int r = lane; r < kBlk; r += 32) {
           const int p = p0 + r;
-          bool dead = !((p < uhi && p >= ulo) || p < upre) || p >= p1;
+          bool dead = !((p < uhi && p >= ulo) || (p < upre && p >= uplo)) || p >= p1;
           if (ids) dead = dead || ids[r] < uid0 || ids[r] > uid1;
           if (dead)
             for (int c = 0; c < L::nb; ++c)
@@ -438,73 +595,78 @@ __global__ void __launch_bounds__(threads(NT), 1)
         fence_async_smem();
         __syncwarp();
       };
+      // P of key tile j for query tile t in two parts, each multiplied when it is there
+      auto pv_when_ready = [&](int t, int buf, int j) -> bool {
+        const uint32_t ph = DB ? ((j >> 1) & 1) : (j & 1);
+        if (!wwait(bar_p + 2 * buf, ph)) return false;
+        tc_fence_after();
+        issue_pv(t, buf, j, Int<0>{}, Int<kPart / 16>{});
+        if (!wwait(bar_p + 2 * buf + 1, ph)) return false;
+        tc_fence_after();
+        issue_pv(t, buf, j, Int<kPart / 16>{}, Int<kBlk / 16>{});
+        return true;
+      };
       bool ok = wwait(bar_q, 0) && slot_full(0);
       if (ok) {
         tc_fence_after();
         for (int t = 0; t < NT; ++t) issue_qk(t, t, 0);
-        release(0);
       }
-      for (int j = 0; ok && j < n; ++j) {
-        const int kt = it.next();
-        const bool more = j + 1 < n;
-        if (NT == 1 && more) {
-          // the other buffer's P was read by the PV of tile j - 1, issued before this product
-          if (!slot_full(2 * j + 2)) { ok = false; break; }
-          tc_fence_after();
-          issue_qk(0, (j + 1) & 1, j + 1);
-          release(2 * j + 2);
+      if constexpr (DB) {
+        for (int j = 0; ok && j < n; ++j) {
+          if (j + 1 < n) {
+            // the other buffer's P was read by the PV of tile j - 1, issued before this product
+            if (!slot_full(2 * j + 2)) { ok = false; break; }
+            tc_fence_after();
+            issue_qk(0, (j + 1) & 1, j + 1);
+          }
+          if (!slot_full(2 * j + 1)) { ok = false; break; }
+          clear_dead(it.next(), j);
+          if (!pv_when_ready(0, j & 1, j)) { ok = false; break; }
         }
-        if (!slot_full(2 * j + 1)) { ok = false; break; }
-        clear_dead(kt, j);
-        if (NT == 2 && more && !slot_full(2 * j + 2)) { ok = false; break; }
+      } else {
+        // One warp for both tiles keeps their softmaxes out of phase, so that they take turns
+        // at the exponent unit (a warp each: 795 us).  What the next step needs is waited for
+        // between the tiles, while the products issued last still run.
+        if (ok) ok = slot_full(1) && (NT == 1 || n < 2 || slot_full(2));
+        if (ok) clear_dead(it.next(), 0);
+        for (int j = 0; ok && j < n; ++j) {
+          const bool more = j + 1 < n;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const int buf = NT == 2 ? t : (j & 1);
-          if (!wwait(bar_p + buf, NT == 2 ? (j & 1) : ((j >> 1) & 1))) { ok = false; break; }
-          tc_fence_after();
-          issue_pv(t, buf, j);
-          if (NT == 2) {
-            if (more) {
-              issue_qk(t, t, j + 1);
-            } else {
-              if (lane == 0) tc_commit(bar_o + t);
-              __syncwarp();
+          for (int t = 0; t < NT; ++t) {
+            if (!pv_when_ready(t, t, j)) { ok = false; break; }
+            if (!more) continue;
+            if (NT == 1 && !slot_full(2 * j + 2)) { ok = false; break; }
+            issue_qk(t, t, j + 1);
+            if (t == 0) {
+              if (!slot_full(2 * j + 3)) { ok = false; break; }
+              clear_dead(it.next(), j + 1);
+            } else if (j + 2 < n && !slot_full(2 * j + 4)) {
+              ok = false;
+              break;
             }
           }
         }
-        if (!ok) break;
-        if (NT == 1) {
-          if (lane == 0) tc_commit(bar_o + (j & 1));
-          __syncwarp();
-        }
-        release(2 * j + 1);
-        if (NT == 2 && more) release(2 * j + 2);
       }
-      if (lane == 0) {
+      if (elect_one()) {
         if (!ok) fail(kDevTimeoutMma);
         tc_commit(bar_drain);
         mbar_wait(bar_drain, 0);
       }
       __syncwarp();
     }
-  }
   } else {
     // ------------------------------------------------------------ softmax --
     if constexpr (NT == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tO = tmem + lane_off + kTmemO + tile * 128;
     const bool warp_rows = __any_sync(0xffffffffu, exists);
-    // what every / any row of this warp sees (rows that do not exist bound nothing)
+    // what every row of this warp sees (rows that do not exist bound nothing), and what any does
     const int a_lo = __reduce_max_sync(0xffffffffu, exists ? lo : 0);
     const int a_hi = __reduce_min_sync(0xffffffffu, exists ? hi : 0x7fffffff);
+    const int a_plo = __reduce_max_sync(0xffffffffu, exists ? plo : 0);
     const int a_pre = __reduce_min_sync(0xffffffffu, exists ? pre : 0x7fffffff);
-    const int s_lo = __reduce_min_sync(0xffffffffu, lo < hi ? lo : 0x7fffffff);
-    const int s_hi = __reduce_max_sync(0xffffffffu, hi);
-    const int s_pre = __reduce_max_sync(0xffffffffu, pre);
-    const bool blind = !(lo < hi || pre > 0);
-    const int i_lo = __reduce_min_sync(0xffffffffu, exists && !blind ? id : 0x7fffffff);
-    const int i_hi = __reduce_max_sync(0xffffffffu, exists && !blind ? id : -1);
-    const bool any_blind = __any_sync(0xffffffffu, exists && blind);
+    const int* mine = red + (warp - W0) * 8;
+    const int s_lo = mine[0], s_hi = mine[1], s_plo = mine[2], s_pre = mine[3], i_lo = mine[4], i_hi = mine[5];
     const int q_lo = __reduce_min_sync(0xffffffffu, qpos), q_hi = __reduce_max_sync(0xffffffffu, qpos);
     float slope2 = 0.f;
     const float* trow = nullptr;
@@ -517,13 +679,13 @@ __global__ void __launch_bounds__(threads(NT), 1)
     bool ok = true;
     for (int j = 0; ok && j < n; ++j) {
       const int t = it.next();
-      const int buf = NT == 2 ? tile : (j & 1);
-      if (!wwait(bar_s + buf, NT == 2 ? (j & 1) : ((j >> 1) & 1))) { ok = false; break; }
+      const int buf = DB ? (j & 1) : tile;
+      if (!wwait(bar_s + buf, DB ? ((j >> 1) & 1) : (j & 1))) { ok = false; break; }
       tc_fence_after();
       const uint32_t tS = tmem + lane_off + buf * kBlk;
       const int p0 = tile_pos(t), pend = tile_end(t), p1 = min(p0 + kBlk, pend);
-      bool any = warp_rows && ((p0 < s_hi && p1 > s_lo) || p0 < s_pre);
-      bool full = p0 + kBlk <= pend && ((p1 <= a_hi && p0 >= a_lo) || p1 <= a_pre) && !any_blind;
+      bool any = warp_rows && ((p0 < s_hi && p1 > s_lo) || (p0 < s_pre && p1 > s_plo));
+      bool full = p0 + kBlk <= pend && ((p1 <= a_hi && p0 >= a_lo) || (p1 <= a_pre && p0 >= a_plo));
       const int32_t* kid = nullptr;
       if (krng) {
         const int2 r = krng[t - A.ntp];
@@ -534,24 +696,21 @@ __global__ void __launch_bounds__(threads(NT), 1)
         }
       }
       if (!any) {  // no key of the tile is seen: its weights are zero
-        uint32_t z[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) z[i] = 0u;
-        tmem_st32(tS, z);
-        tmem_st32(tS + 32, z);
+        for (int i = 0; i < 8; ++i) tmem_fill8(tS + 8 * i, 0u);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_p + buf);
+        if (lane == 0) {
+          mbar_arrive(bar_p + 2 * buf);
+          mbar_arrive(bar_p + 2 * buf + 1);
+        }
         continue;
       }
       float xs[128];
-      {
-        uint32_t* sr = reinterpret_cast<uint32_t*>(xs);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sr + c * 32));
-        tmem_wait_ld();
-      }
+      for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(xs + c * 32));
+      tmem_wait_ld();
       if constexpr (SCORE) {
         if (A.cap_in > 0.f) {
           // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), to 2^-22 of the cap
@@ -570,7 +729,7 @@ __global__ void __launch_bounds__(threads(NT), 1)
           for (int i = 0; i < 128; ++i) xs[i] = fmaf(-slope2, fabsf(d0 - (float)i), xs[i]);
         }
         if (tab_smem) {
-          // distances p0 - q_hi .. p0 + 127 - q_lo of this warp
+          // distances p0 - q_hi .. p0 + 127 - q_lo of this warp: all beyond the reach?
           if (p0 - q_hi >= A.reach || p0 + kBlk - 1 - q_lo <= -A.reach) {
             const float bv = tab[p0 - q_hi >= A.reach ? 2 * A.reach + kTabPad : kTabPad];
 #pragma unroll
@@ -587,10 +746,11 @@ __global__ void __launch_bounds__(threads(NT), 1)
         }
       }
       if (!full) {
-        const int e = min(hi, pend) - p0, f = lo - p0, g = min(pre, pend) - p0;
+        const int e = min(hi, pend) - p0, f = lo - p0, g = min(pre, pend) - p0, h = plo - p0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const uint32_t w = (low_bits(e - c * 32) & ~low_bits(f - c * 32)) | low_bits(g - c * 32);
+          const uint32_t w = (low_bits(e - c * 32) & ~low_bits(f - c * 32)) |
+                             (low_bits(g - c * 32) & ~low_bits(h - c * 32));
 #pragma unroll
           for (int i = 0; i < 32; ++i)
             if (!((w >> i) & 1u)) xs[c * 32 + i] = -INFINITY;
@@ -606,15 +766,16 @@ __global__ void __launch_bounds__(threads(NT), 1)
           }
         }
       }
-      float mq[4];
+      float mq[8];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float m = fmax3(xs[c * 32], xs[c * 32 + 1], xs[c * 32 + 2]);
+      for (int c = 0; c < 8; ++c) mq[c] = fmax3(xs[c], xs[c + 8], xs[c + 16]);
 #pragma unroll
-        for (int i = 3; i < 31; i += 2) m = fmax3(m, xs[c * 32 + i], xs[c * 32 + i + 1]);
-        mq[c] = fmaxf(m, xs[c * 32 + 31]);
-      }
-      float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3]));
+      for (int i = 24; i < 120; i += 16)
+#pragma unroll
+        for (int c = 0; c < 8; ++c) mq[c] = fmax3(mq[c], xs[i + c], xs[i + c + 8]);
+#pragma unroll
+      for (int c = 0; c < 8; c += 2) mq[c] = fmax3(mq[c], mq[c + 1], fmaxf(xs[120 + c], xs[121 + c]));
+      float mx = fmaxf(fmax3(mq[0], mq[2], mq[4]), mq[6]);
       if constexpr (!SCORE) mx *= A.scale;
       const float m_new = fmaxf(m_run, mx);
       // (tile rows that do not exist hold whatever shared memory held: they have no vote)
@@ -624,9 +785,9 @@ __global__ void __launch_bounds__(threads(NT), 1)
         m_run = m_new;
         l_run *= alpha;
         if (j > 0) {
-          // O holds the tiles before this one against the old maximum.  NT = 2: its last PV
-          // was issued before the product whose scores were just read; NT = 1: wait for it
-          if (NT == 1 && !wwait(bar_o + ((j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1))) { ok = false; break; }
+          // O holds the tiles before this one against the old maximum; their PV was issued
+          // before the product whose scores were just read (DB: the last one is waited for)
+          if (DB && !wwait(bar_o + ((j - 1) & 1), (uint32_t)(((j - 1) >> 1) & 1))) { ok = false; break; }
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
@@ -642,36 +803,50 @@ __global__ void __launch_bounds__(threads(NT), 1)
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
       const float sc = SCORE ? 1.f : A.scale;
       const float2 scv = make_float2(sc, sc), nm = make_float2(-m_use, -m_use);
-      float2 rs0 = make_float2(0.f, 0.f), rs1 = make_float2(0.f, 0.f);
+      // weights 2^(s - m), rounded over the scores 32 keys at a time
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[16];
 #pragma unroll
-        for (int q = 0; q < 32; ++q) {
-          const float2 xx = make_float2(xs[c * 64 + 2 * q], xs[c * 64 + 2 * q + 1]);
-          const float2 e = SCORE ? fadd2(xx, nm) : ffma2(xx, scv, nm);
-          const float2 pp = make_float2(fast_exp2(e.x), fast_exp2(e.y));
-          if (q & 1) rs1 = fadd2(rs1, pp); else rs0 = fadd2(rs0, pp);
-          w[q] = pack16<F16>(pp.x, pp.y);
+        for (int q = 0; q < 16; ++q) {
+          float2 e = make_float2(xs[c * 32 + 2 * q], xs[c * 32 + 2 * q + 1]);
+          e = SCORE ? fadd2(e, nm) : ffma2(e, scv, nm);
+          e.x = fast_exp2(e.x);
+          e.y = fast_exp2(e.y);
+          xs[c * 32 + 2 * q] = e.x;
+          xs[c * 32 + 2 * q + 1] = e.y;
+          w[q] = pack16<F16>(e.x, e.y);
         }
-        tmem_st32(tS + c * 32, w);
+        if (c == kPart / 32) {  // the stores of the first keys have landed meanwhile
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_p + 2 * buf);
+        }
+        tmem_st16(tS + c * 16, w);
       }
-      l_run += (rs0.x + rs1.x) + (rs0.y + rs1.y);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_p + buf);
+      if (lane == 0) mbar_arrive(bar_p + 2 * buf + 1);
+      // the row's sum is taken while the tensor cores go on
+      float2 rs[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) rs[c] = make_float2(xs[2 * c], xs[2 * c + 1]);
+#pragma unroll
+      for (int q = 4; q < 64; ++q) rs[q & 3] = fadd2(rs[q & 3], make_float2(xs[2 * q], xs[2 * q + 1]));
+      const float2 rt = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
+      l_run += rt.x + rt.y;
     }
     // ------------------------------------------------------------ epilogue --
-    // (the scores of tile n - 1 came after PV n - 3, so the parity names one phase)
-    if (ok && n > 0) ok = NT == 2 ? wwait(bar_o + tile, 0u) : wwait(bar_o + ((n - 1) & 1), (uint32_t)(((n - 1) >> 1) & 1));
+    // (DB: the scores of tile n - 1 came after PV n - 3, so the parity names one phase)
+    if (ok && n > 0) ok = DB ? wwait(bar_o + ((n - 1) & 1), (uint32_t)(((n - 1) >> 1) & 1)) : wwait(bar_o + tile, 0u);
+    if (n == 0) ok = wwait(bar_q, 0);  // Q's copy has landed before its memory is written
     if (!ok) fail(kDevTimeoutEpilogue);
     tc_fence_after();
     const bool zero = !ok || n == 0 || l_run == 0.f;  // NaN sums go on to the output
-    if (A.part_o != nullptr) {
-      const int s = kind ? A.splits[0] + split : split;
-      const int64_t R = (int64_t)A.B * A.Sq * A.Hq;
-      const int64_t r = (int64_t)s * R + ((int64_t)rb * A.Sq + rtok) * A.Hq + rh;
+    if (A.part_o != nullptr && (nsplit > 1 || A.items1 > 0)) {
+      const int64_t r = (kind ? A.part_off1 : 0) + (int64_t)slot * (G * T * Nb) + row;
       if (exists) A.part_ml[r] = zero ? make_float2(-INFINITY, 0.f) : make_float2(m_run, l_run);
       if (warp_rows && n > 0 && ok) {
 #pragma unroll 1
@@ -686,10 +861,12 @@ __global__ void __launch_bounds__(threads(NT), 1)
           }
         }
       }
-    } else if (warp_rows) {
+    } else {
+      // rows through the Q tile's shared memory (its last product is done) and out by TMA: a
+      // thread's own stores of 16 bytes a row took 2200 to 4000 cycles; what lies beyond the
+      // tensor is not written
       const float inv_l = zero ? 0.f : 1.0f / l_run;
-      uint8_t* dst = reinterpret_cast<uint8_t*>(A.out) +
-                     2 * ((int64_t)rb * A.os.b + (int64_t)rh * A.os.h + (int64_t)rtok * A.os.s);
+      uint8_t* so = sQ + tile * L::op + row * 128;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
@@ -697,18 +874,25 @@ __global__ void __launch_bounds__(threads(NT), 1)
           tmem_ld32(tO + c * 32, o);
           tmem_wait_ld();
         }
-        if (exists) {
+        uint8_t* dst = so + (c >> 1) * kTile;
 #pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            uint32_t w[4];
+        for (int v = 0; v < 4; ++v) {
+          uint32_t w[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              w[u] = zero ? 0u
-                          : pack16<F16>(__uint_as_float(o[8 * v + 2 * u]) * inv_l,
-                                        __uint_as_float(o[8 * v + 2 * u + 1]) * inv_l);
-            *reinterpret_cast<uint4*>(dst + c * 64 + v * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          for (int u = 0; u < 4; ++u)
+            w[u] = zero ? 0u
+                        : pack16<F16>(__uint_as_float(o[8 * v + 2 * u]) * inv_l,
+                                      __uint_as_float(o[8 * v + 2 * u + 1]) * inv_l);
+          *reinterpret_cast<uint4*>(dst + ((((c & 1) * 4 + v) ^ (row & 7)) * 16)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+      }
+      fence_async_smem();
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + tile) : "memory");
+      if (quarter == 0 && lane == 0) {
+        for (int c = 0; c < L::nb; ++c)
+          tma_store_4d(&tmo, so + c * kTile, c * 64, G > 1 ? hw * G : hw, tok0 + tile * T, b0);
+        bulk_commit();
+        bulk_wait_read<0>();
       }
     }
   }
@@ -718,40 +902,50 @@ __global__ void __launch_bounds__(threads(NT), 1)
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, L::cols);
   }
 }
 
-struct Maps { CUtensorMap q, q1, k, v, pk, pv; };
+struct Maps { CUtensorMap q, q1, o, k, v, pk, pv; };
 
-template <int D, int NT, bool F16, bool SCORE>
+template <int D, int FORM, bool F16, bool SCORE>
 static cudaError_t launch_one(const Maps& m, const Args& a, unsigned grid, cudaStream_t s) {
+  using L = Smem<D, FORM>;
   static std::atomic<uint64_t> attr{0};
-  auto kern = masked_attn_kernel<D, NT, F16, SCORE>;
-  if (NT == 2 && attr.load(std::memory_order_acquire) == 0) {
-    // the register split below must fit what the block is launched with: an inc beyond it waits for good
+  auto kern = masked_attn_kernel<D, FORM, F16, SCORE>;
+  if (FORM == kPair && attr.load(std::memory_order_acquire) == 0) {
+    // the register split must fit what the block is launched with: an inc beyond it waits for good
     cudaFuncAttributes fa;
     const cudaError_t r = cudaFuncGetAttributes(&fa, kern);
     if (r != cudaSuccess) return r;
     if (fa.numRegs * threads(2) < 128 * kRegsFew + 256 * kRegsSoftmax) return cudaErrorInvalidConfiguration;
   }
-  cudaError_t e = qf2_set_smem_once(kern, Smem<D, NT>::total, &attr);
+  cudaError_t e = qf2_set_smem_once(kern, L::total, &attr);
   if (e != cudaSuccess) return e;
-  kern<<<grid, threads(NT), Smem<D, NT>::total, s>>>(m.q, m.q1, m.k, m.v, m.pk, m.pv, a);
+  kern<<<grid, threads(L::nt), L::total, s>>>(m.q, m.q1, m.o, m.k, m.v, m.pk, m.pv, a);
   return cudaGetLastError();
 }
 
-template <int D, int NT>
-static cudaError_t launch_nt(const Maps& m, const Args& a, unsigned grid, bool f16, bool score, cudaStream_t s) {
-  if (f16) return score ? launch_one<D, NT, true, true>(m, a, grid, s) : launch_one<D, NT, true, false>(m, a, grid, s);
-  return score ? launch_one<D, NT, false, true>(m, a, grid, s) : launch_one<D, NT, false, false>(m, a, grid, s);
+template <int D, int FORM>
+static cudaError_t launch_form(const Maps& m, const Args& a, unsigned grid, bool f16, bool score, cudaStream_t s) {
+  if (f16)
+    return score ? launch_one<D, FORM, true, true>(m, a, grid, s) : launch_one<D, FORM, true, false>(m, a, grid, s);
+  return score ? launch_one<D, FORM, false, true>(m, a, grid, s) : launch_one<D, FORM, false, false>(m, a, grid, s);
+}
+
+template <int D>
+static cudaError_t launch_dim(const Maps& m, const Args& a, unsigned grid, int form, bool f16, bool score,
+                              cudaStream_t s) {
+  if (form == kPair) return launch_form<D, kPair>(m, a, grid, f16, score, s);
+  if (form == kDeep) return launch_form<D, kDeep>(m, a, grid, f16, score, s);
+  return launch_form<D, kSmall>(m, a, grid, f16, score, s);
 }
 
 // One launcher per head dim, each in its own translation unit.
-cudaError_t launch_d64(const Maps& m, const Args& a, unsigned grid, int nt, bool f16, bool score, cudaStream_t s);
-cudaError_t launch_d96(const Maps& m, const Args& a, unsigned grid, int nt, bool f16, bool score, cudaStream_t s);
-cudaError_t launch_d128(const Maps& m, const Args& a, unsigned grid, int nt, bool f16, bool score, cudaStream_t s);
-cudaError_t launch_d256(const Maps& m, const Args& a, unsigned grid, int nt, bool f16, bool score, cudaStream_t s);
+cudaError_t launch_d64(const Maps& m, const Args& a, unsigned grid, int form, bool f16, bool score, cudaStream_t s);
+cudaError_t launch_d96(const Maps& m, const Args& a, unsigned grid, int form, bool f16, bool score, cudaStream_t s);
+cudaError_t launch_d128(const Maps& m, const Args& a, unsigned grid, int form, bool f16, bool score, cudaStream_t s);
+cudaError_t launch_d256(const Maps& m, const Args& a, unsigned grid, int form, bool f16, bool score, cudaStream_t s);
 
 }  // namespace mattn
 }  // namespace qf2

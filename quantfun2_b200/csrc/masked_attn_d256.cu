@@ -5,9 +5,9 @@
 namespace qf2 {
 namespace mattn {
 
-cudaError_t launch_d256(const Maps& m, const Args& a, unsigned grid, int nt, bool f16, bool score, cudaStream_t s) {
-  (void)nt;
-  return launch_nt<256, 1>(m, a, grid, f16, score, s);
+cudaError_t launch_d256(const Maps& m, const Args& a, unsigned grid, int form, bool f16, bool score, cudaStream_t s) {
+  (void)form;
+  return launch_form<256, kDeep>(m, a, grid, f16, score, s);
 }
 
 }  // namespace mattn

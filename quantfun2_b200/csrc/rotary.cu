@@ -164,21 +164,19 @@ static cudaError_t launch(Args& a, bool half_layout, bool vec, bool copy_rest, c
 
 using namespace qf2::rotary;
 
-extern "C" int qf2_rotary_apply(const void* xq, void* xq_out, int64_t Hq, const int64_t* xq_strides,
-                                const int64_t* xq_out_strides, const void* xk, void* xk_out, int64_t Hk,
-                                const int64_t* xk_strides, const int64_t* xk_out_strides, const void* positions,
-                                const int64_t* pos_strides, int pos_is_i64, const double* inv_freq, int64_t rotary_dim,
-                                int layout, float gain, int inverse, int64_t B, int64_t S, int64_t D, int dtype,
-                                qf2_stream_t stream) {
+extern "C" int qf2_rotary_apply(const qf2_rotary_args* args) {
+  if (!args) return QF2_ERR_ARG;
+  const qf2_rotary_args& r = *args;
+  const int64_t B = r.B, S = r.S, Hq = r.Hq, Hk = r.Hk, D = r.D, rotary_dim = r.rotary_dim, layout = r.layout,
+                dtype = r.dtype;
   if (dtype != QF2_F32 && dtype != QF2_F16 && dtype != QF2_BF16) return QF2_ERR_DTYPE;
   if (layout != QF2_ROTARY_HALF && layout != QF2_ROTARY_INTERLEAVED) return QF2_ERR_ARG;
   if (B < 0 || S < 0 || Hq < 0 || Hk < 0 || D <= 0 || D > 1024) return QF2_ERR_SHAPE;
   if (rotary_dim <= 0 || rotary_dim > D || (rotary_dim & 1)) return QF2_ERR_SHAPE;
   if (Hq > 65535 || Hk > 65535 || (S > 0 && B > (int64_t)(1ll << 34) / S)) return QF2_ERR_SHAPE;
   if (B == 0 || S == 0 || Hq + Hk == 0) return QF2_OK;
-  if (!positions || !pos_strides || !inv_freq) return QF2_ERR_ARG;
-  if (Hq > 0 && (!xq || !xq_out || !xq_strides || !xq_out_strides)) return QF2_ERR_ARG;
-  if (Hk > 0 && (!xk || !xk_out || !xk_strides || !xk_out_strides)) return QF2_ERR_ARG;
+  if (!r.positions || !r.inv_freq) return QF2_ERR_ARG;
+  if ((Hq > 0 && (!r.xq || !r.xq_out)) || (Hk > 0 && (!r.xk || !r.xk_out))) return QF2_ERR_ARG;
   const int esz = dtype == QF2_F32 ? 4 : 2, V = 16 / esz;
   Args a{};
   bool vec = D % V == 0 && (layout == QF2_ROTARY_HALF ? (rotary_dim / 2) % V == 0 : rotary_dim % V == 0);
@@ -192,22 +190,22 @@ extern "C" int qf2_rotary_apply(const void* xq, void* xq_out, int64_t Hq, const 
     }
     if (x != y) in_place = false;
   };
-  if (Hq > 0) side(a.q, xq, xq_out, xq_strides, xq_out_strides);
-  if (Hk > 0) side(a.k, xk, xk_out, xk_strides, xk_out_strides);
+  if (Hq > 0) side(a.q, r.xq, r.xq_out, r.xq_strides, r.xq_out_strides);
+  if (Hk > 0) side(a.k, r.xk, r.xk_out, r.xk_strides, r.xk_out_strides);
   a.Hq = (int)Hq;
   a.H = (int)(Hq + Hk);
-  a.pos = positions;
-  a.pos_sb = pos_strides[0];
-  a.pos_ss = pos_strides[1];
-  a.pos64 = pos_is_i64;
-  a.inv_freq = inv_freq;
+  a.pos = r.positions;
+  a.pos_sb = r.pos_strides[0];
+  a.pos_ss = r.pos_strides[1];
+  a.pos64 = r.pos_is_i64 != 0;
+  a.inv_freq = r.inv_freq;
   a.half = (int)(rotary_dim / 2);
   a.D = (int)D;
   a.tokens = B * S;
   a.S = S;
-  a.gain = gain;
-  a.sin_gain = inverse ? -gain : gain;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  a.gain = (float)r.gain;
+  a.sin_gain = r.inverse ? -a.gain : a.gain;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(r.stream);
   const bool hl = layout == QF2_ROTARY_HALF, rest = !in_place;
   cudaError_t e;
   if (dtype == QF2_F32) e = launch<float>(a, hl, vec, rest, s);

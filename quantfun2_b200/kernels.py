@@ -26,7 +26,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import QF2Error, check, dtype_code, i64, on_device, require_device, stream_ptr
+from ._lib import QF2Error, check, dtype_code, i64, on_device, raw_stream, require_device, stream_ptr
 
 __all__ = [
     "copy_chunks",
@@ -158,41 +158,62 @@ def rotary_inv_freq(rotary_dim: int, base: float = 10000.0, scaling: str = "none
     return f.to(device) if device is not None else f
 
 
+_ROTARY_LAYOUTS = {"half": _lib.QF2_ROTARY_HALF, "interleaved": _lib.QF2_ROTARY_INTERLEAVED}
+_NO_STRIDES = (0, 0, 0)
+
+
 def _rotary(xq, xk, positions, inv_freq, out_q, out_k, layout, magnitude, inverse):
     require_device(xq)
-    if layout not in ("half", "interleaved"):
+    mode = _ROTARY_LAYOUTS.get(layout)
+    if mode is None:
         raise QF2Error(f"unknown rotary layout {layout!r}")
-    if xq.dim() != 4 or xq.stride(-1) != 1 or out_q.stride(-1) != 1:
-        raise QF2Error("rotary_apply expects [B, S, H, D] tensors with a contiguous last dim")
+    if xq.dim() != 4:
+        raise QF2Error("rotary_apply expects [B, S, H, D] tensors")
     B, S, Hq, D = xq.shape
-    dt = dtype_code(xq.dtype)
-    dev = xq.device
-    if xk is not None and (xk.dim() != 4 or xk.shape[0] != B or xk.shape[1] != S or xk.shape[3] != D
-                           or xk.dtype != xq.dtype or xk.device != dev or xk.stride(-1) != 1 or out_k.stride(-1) != 1):
-        raise QF2Error("xk must match xq in batch, seq, head_dim, dtype and device, with a contiguous last dim")
-    if torch.is_grad_enabled() and (xq.requires_grad or (xk is not None and xk.requires_grad)):
+    qs, qo = xq.stride(), out_q.stride()
+    dev, dtype = xq.device, xq.dtype
+    dt = dtype_code(dtype)
+    grad = xq.requires_grad
+    if xk is None:
+        kp = kop = Hk = 0
+        ks = ko = _NO_STRIDES
+    else:
+        if xk.dim() != 4:
+            raise QF2Error("rotary_apply expects [B, S, H, D] tensors")
+        Bk, Sk, Hk, Dk = xk.shape
+        ks, ko = xk.stride(), out_k.stride()
+        if Bk != B or Sk != S or Dk != D or xk.dtype != dtype or xk.device != dev or ks[3] != 1 or ko[3] != 1:
+            raise QF2Error("xk must match xq in batch, seq, head_dim, dtype and device, with a contiguous last dim")
+        kp, kop = xk.data_ptr(), out_k.data_ptr()
+        grad = grad or xk.requires_grad
+    if qs[3] != 1 or qo[3] != 1:
+        raise QF2Error("rotary_apply needs a contiguous last dim")
+    if grad and torch.is_grad_enabled():
         raise QF2Error("rotary_apply is an inference op: its inputs must not require a gradient")
-    if inv_freq.dim() != 1 or inv_freq.dtype != torch.float64 or inv_freq.device != dev or \
+    if inv_freq.dtype != torch.float64 or inv_freq.device != dev or inv_freq.dim() != 1 or \
             not inv_freq.is_contiguous():
         raise QF2Error("inv_freq must be a contiguous fp64 vector on the tensors' device")
-    if positions.device != dev or positions.dtype not in (torch.int32, torch.int64):
+    pdt = positions.dtype
+    if positions.device != dev or (pdt != torch.int64 and pdt != torch.int32):
         raise QF2Error("positions must be int32 or int64 on the tensors' device")
-    if positions.shape == (S,):
-        ps = (0, positions.stride(0))
-    elif positions.shape == (B, S) or positions.shape == (1, S):
-        ps = (positions.stride(0) if positions.shape[0] > 1 else 0, positions.stride(1))
+    psh, pst = positions.shape, positions.stride()
+    if psh == (B, S):
+        pb, pp = (pst[0] if B > 1 else 0), pst[1]
+    elif psh == (S,):
+        pb, pp = 0, pst[0]
+    elif psh == (1, S):
+        pb, pp = 0, pst[1]
     else:
-        raise QF2Error(f"positions must be [{S}] or [{B}, {S}], got {tuple(positions.shape)}")
-    st = lambda t: i64(t.stride(0), t.stride(1), t.stride(2))  # noqa: E731
-    has_k = xk is not None
+        raise QF2Error(f"positions must be [{S}] or [{B}, {S}], got {tuple(psh)}")
+    index = dev.index
+    args = _lib.ROTARY_ARGS.pack(
+        xq.data_ptr(), out_q.data_ptr(), kp, kop, positions.data_ptr(), inv_freq.data_ptr(), qs[0], qs[1], qs[2],
+        qo[0], qo[1], qo[2], ks[0], ks[1], ks[2], ko[0], ko[1], ko[2], pb, pp, pdt == torch.int64, B, S, Hq, Hk, D,
+        2 * inv_freq.shape[0], mode, bool(inverse), dt, magnitude, raw_stream(index))
     with on_device(dev):
-        check(_lib.load().qf2_rotary_apply(
-            xq.data_ptr(), out_q.data_ptr(), Hq, st(xq), st(out_q),
-            xk.data_ptr() if has_k else None, out_k.data_ptr() if has_k else None, xk.shape[2] if has_k else 0,
-            st(xk) if has_k else None, st(out_k) if has_k else None, positions.data_ptr(), i64(*ps),
-            int(positions.dtype == torch.int64), inv_freq.data_ptr(), 2 * inv_freq.shape[0],
-            _lib.QF2_ROTARY_HALF if layout == "half" else _lib.QF2_ROTARY_INTERLEAVED, float(magnitude),
-            int(bool(inverse)), B, S, D, dt, stream_ptr(dev)), "qf2_rotary_apply")
+        st = _lib.load().qf2_rotary_apply(args)
+    if st:
+        check(st, "qf2_rotary_apply")
 
 
 def rotary_apply(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,

@@ -45,20 +45,13 @@ def test_ops_refuse_host_tensors():
 
 def _call(**kw):
     """qf2_masked_attn with aligned dummy pointers: every refusal below comes before a launch."""
-    lib = _lib.load()
-    a = dict(B=1, Hq=2, Hkv=2, Sq=4, Skv=4, D=64, P=0, dtype=_lib.QF2_BF16, scale=0.1, q=1024, k=1024, v=1024, out=1024,
-             stride=64, ws=None, nbytes=0, pk=None)
-    mask = _lib.AttnMask(left=-1, right=-1)
-    for key, val in kw.items():
-        if key in a:
-            a[key] = val
-        else:
-            setattr(mask, key, val)
-    s = _lib.i64(a["stride"], a["stride"], a["stride"])
-    p = lambda x: None if x is None else ctypes.c_void_p(x)  # noqa: E731
-    return lib.qf2_masked_attn(p(a["q"]), s, p(a["k"]), s, p(a["v"]), s, p(a["out"]), s, a["B"], a["Hq"], a["Hkv"],
-                               a["Sq"], a["Skv"], a["D"], p(a["pk"]), s, p(a["pk"]), s, a["P"], mask, a["scale"],
-                               a["dtype"], p(a["ws"]), a["nbytes"], None)
+    a = dict(B=1, Hq=2, Hkv=2, Sq=4, Skv=4, D=64, dtype=_lib.QF2_BF16, sm_scale=0.1, q=1024, k=1024, v=1024, out=1024,
+             left=-1, right=-1)
+    stride = kw.pop("stride", 64)
+    a.update({f"{t}_strides": (stride,) * 3 for t in ("q", "k", "v", "out")}, prefix_k_strides=(stride,) * 2,
+             prefix_v_strides=(stride,) * 2)
+    a.update(kw)
+    return _lib.load().qf2_masked_attn(_lib.MASKED_ATTN_ARGS.pack_named(**a))
 
 
 @pytest.mark.parametrize("kw,status", [
@@ -66,9 +59,9 @@ def _call(**kw):
     (dict(B=70000), -1), (dict(Skv=(1 << 20) + 1), -1), (dict(Skv=1 << 20, P=1), -1), (dict(q=None), -8), (dict(k=None), -8),
     (dict(out=None), -8), (dict(P=4), -8), (dict(q_ids=1024), -8), (dict(k_ids=1024), -8), (dict(q_offset_mode=3), -8),
     (dict(q_offset_mode=1), -8), (dict(slopes=1024, bias_table=1024), -8), (dict(bias_table=1024, bias_reach=1025), -1),
-    (dict(softcap=-1.0), -8), (dict(softcap=math.nan), -8), (dict(scale=0.0), -8), (dict(scale=math.inf), -8),
+    (dict(softcap=-1.0), -8), (dict(softcap=math.nan), -8), (dict(sm_scale=0.0), -8), (dict(sm_scale=math.inf), -8),
     (dict(q=1032), -5), (dict(v=1032), -5), (dict(stride=60), -5), (dict(stride=0), -5),
-    (dict(q_ids=1024, k_ids=1024), -6), (dict(q_ids=1024, k_ids=1024, pk=1024, P=4), -8),
+    (dict(q_ids=1024, k_ids=1024), -6), (dict(q_ids=1024, k_ids=1024, prefix_k=1024, prefix_v=1024, P=4), -8),
 ])
 def test_attention_refusals_without_device(kw, status):
     assert _call(**kw) == status
@@ -80,10 +73,9 @@ def test_empty_batches_return_at_once():
 
 def test_workspace_plans():
     ws = _lib.load().qf2_masked_attn_workspace_bytes
-    # long queries: no split; ids: a padded copy and one range per key tile
+    # long queries: no split; ids: a padded copy of the keys', and one run of keys per query
     assert ws(1, 24, 8, 16384, 16384, 0, 128, 0) == 0
-    tiles = 16384 // 128
-    assert ws(1, 24, 8, 16384, 16384, 0, 128, 1) == tiles * 128 * 4 + tiles * 8
+    assert ws(1, 24, 8, 16384, 16384, 0, 128, 1) >= 16384 * 4 + 16384 * 8
     # single tokens on a long cache are split: fp32 rows and (max, sum) pairs of each split
     one = ws(1, 8, 8, 1, 65536, 0, 128, 0)
     assert one > 0 and (one - 0) % 256 == 0
@@ -94,12 +86,37 @@ def test_workspace_plans():
 
 def test_rotary_refusals_without_device():
     lib = _lib.load()
-    s3, s2, p = _lib.i64(64, 64, 64), _lib.i64(0, 1), ctypes.c_void_p(1024)
 
-    def call(xq=p, Hq=1, xk=None, Hk=0, pos=p, f=p, r=64, layout=0, B=1, S=1, D=64, dtype=2):
-        return lib.qf2_rotary_apply(xq, xq, Hq, s3, s3, xk, xk, Hk, s3, s3, pos, s2, 1, f, r, layout, 1.0, 0, B, S, D,
-                                    dtype, None)
+    def call(**kw):
+        a = dict(xq=1024, xq_out=1024, positions=1024, inv_freq=1024, xq_strides=(64,) * 3, xq_out_strides=(64,) * 3,
+                 pos_strides=(0, 1), pos_is_i64=1, B=1, S=1, Hq=1, Hk=0, D=64, rotary_dim=64, dtype=_lib.QF2_BF16, gain=1.0)
+        a.update(kw)
+        return lib.qf2_rotary_apply(_lib.ROTARY_ARGS.pack_named(**a))
 
-    assert call(dtype=3) == -2 and call(layout=2) == -8 and call(r=63) == -1 and call(r=66) == -1 and call(r=0) == -1
-    assert call(D=2048) == -1 and call(B=-1) == -1 and call(Hk=1) == -8 and call(xq=None) == -8 and call(pos=None) == -8
-    assert call(f=None) == -8 and call(B=0) == 0 and call(Hq=0) == 0 and call(S=0, pos=None) == 0
+    assert call(dtype=3) == -2 and call(layout=2) == -8 and call(rotary_dim=63) == -1 and call(rotary_dim=66) == -1
+    assert call(rotary_dim=0) == -1 and call(D=2048) == -1 and call(B=-1) == -1
+    assert call(Hk=1) == -8 and call(xq=None) == -8 and call(positions=None) == -8 and call(inv_freq=None) == -8
+    assert call(B=0) == 0 and call(Hq=0) == 0 and call(S=0, positions=None) == 0
+    assert lib.qf2_rotary_apply(None) == -8 and lib.qf2_masked_attn(None) == -8
+
+
+def test_argument_structs_match_the_header():
+    """The packed fields, in order, are the header's struct fields."""
+    import re
+    from pathlib import Path
+
+    text = (Path(__file__).resolve().parent.parent / "include" / "qf2b200.h").read_text()
+    for name, args in (("qf2_rotary_args", _lib.ROTARY_ARGS), ("qf2_masked_attn_args", _lib.MASKED_ATTN_ARGS)):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, re.S).group(1)
+        body = re.sub(r"/\*.*?\*/", "", body, flags=re.S)
+        fields = []
+        for decl in body.split(";"):
+            if not decl.strip():
+                continue
+            m = re.match(r"\s*((?:const )?(?:void|int64_t|int32_t|float|double|qf2_stream_t))\s*(\*?)\s*(.*)", decl, re.S)
+            base, star, names = m.group(1), m.group(2), m.group(3)
+            assert star or base in ("int64_t", "double", "qf2_stream_t"), decl      # 8 bytes each
+            for nm in names.split(","):
+                arr = re.match(r"\s*(\w+)(?:\[(\d+)\])?", nm)
+                fields.append((arr.group(1), int(arr.group(2) or 1), "d" if base == "double" and not star else "q"))
+        assert fields == [tuple(f) for f in args.fields]
