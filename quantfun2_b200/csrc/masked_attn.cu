@@ -22,6 +22,7 @@ __global__ void __launch_bounds__(128) mattn_ids_kernel(const int32_t* __restric
                                                         int* __restrict__ rising) {
   const int t = blockIdx.x, b = blockIdx.y, i = threadIdx.x;
   const int j = t * kBlk + i;
+  grid_launch_dependents();
   const int v = j < Skv ? ids[(int64_t)b * Skv + j] : -2;
   const int next = j + 1 < Skv ? ids[(int64_t)b * Skv + j + 1] : -1;
   const int fine = __syncthreads_and(j + 1 >= Skv || (uint32_t)v <= (uint32_t)next);
@@ -37,38 +38,43 @@ __global__ void __launch_bounds__(128) mattn_ids_kernel(const int32_t* __restric
   }
 }
 
-// Where a batch element's key ids are in order, the keys of each query's id are one run, found by
-// two binary searches: the attention kernel then masks by ranges (documents, padded ends) and
-// looks at no id.  grid (ceil(Sq / 128), B), 128 threads.
+// Where a batch element's key ids are in order, the keys of each query's id are one run: the
+// attention kernel then masks by ranges (documents, padded ends) and looks at no id.  A warp
+// takes 32 queries, one id among them at a time: the tiles whose first key comes before the
+// id are counted, then such keys of the last of these tiles.  grid (ceil(Sq / 128), B), 128 threads.
 __global__ void __launch_bounds__(128) mattn_runs_kernel(const int32_t* __restrict__ q_ids,
                                                          const int32_t* __restrict__ k_ids,
                                                          const int* __restrict__ rising, int Sq, int Skv, int nto,
                                                          int2* __restrict__ q_rng, int* __restrict__ sorted) {
-  const int b = blockIdx.y, i = blockIdx.x * 128 + threadIdx.x;
+  const int b = blockIdx.y, i = blockIdx.x * 128 + threadIdx.x, lane = threadIdx.x & 31;
+  const int id = i < Sq ? q_ids[(int64_t)b * Sq + i] : -1;
+  grid_launch_dependents();
+  grid_wait();
   int fine = 1;
   for (int t = threadIdx.x; t < nto; t += 128) fine &= rising[(int64_t)b * nto + t];
   fine = __syncthreads_and(fine);
   if (blockIdx.x == 0 && threadIdx.x == 0) sorted[b] = fine;
-  if (!fine || i >= Sq) return;
-  const int id = q_ids[(int64_t)b * Sq + i];
+  if (!fine) return;
   const int32_t* k = k_ids + (int64_t)b * nto * kBlk;
+  // keys of less than x (as unsigned numbers), by the warp; the pads come after every id
+  auto below = [&](uint32_t x) -> int {
+    int tiles = 0;
+    for (int t = lane; t < nto; t += 32) tiles += (uint32_t)k[(int64_t)t * kBlk] < x;
+    tiles = __reduce_add_sync(0xffffffffu, tiles);
+    if (tiles == 0) return 0;
+    const int4 v = *reinterpret_cast<const int4*>(k + (int64_t)(tiles - 1) * kBlk + 4 * lane);
+    const int n = ((uint32_t)v.x < x) + ((uint32_t)v.y < x) + ((uint32_t)v.z < x) + ((uint32_t)v.w < x);
+    return (tiles - 1) * kBlk + __reduce_add_sync(0xffffffffu, n);
+  };
   int2 r = make_int2(0, 0);
-  if (id >= 0) {
-    // first key with an id of at least `id`, first with a greater one
-    int lo = 0, hi = Skv;
-    while (lo < hi) {
-      const int m = (lo + hi) >> 1;
-      if ((uint32_t)k[m] < (uint32_t)id) lo = m + 1; else hi = m;
-    }
-    r.x = lo;
-    hi = Skv;
-    while (lo < hi) {
-      const int m = (lo + hi) >> 1;
-      if ((uint32_t)k[m] <= (uint32_t)id) lo = m + 1; else hi = m;
-    }
-    r.y = lo;
+  uint32_t left = __ballot_sync(0xffffffffu, id >= 0);
+  while (left) {
+    const int x = __shfl_sync(0xffffffffu, id, __ffs(left) - 1);
+    const int lo = below((uint32_t)x), hi = below((uint32_t)x + 1u);
+    if (id == x) r = make_int2(lo, hi);
+    left &= ~__ballot_sync(0xffffffffu, id == x);
   }
-  q_rng[(int64_t)b * Sq + i] = r;
+  if (i < Sq) q_rng[(int64_t)b * Sq + i] = r;
 }
 
 // ----------------------------------------------------------- merge splits --
@@ -82,12 +88,12 @@ __global__ void __launch_bounds__(128) mattn_merge_kernel(const __grid_constant_
   constexpr int C = D / 4, NG = 128 / C;
   __shared__ float wgt[2 * kMaxSplits];
   __shared__ float4 acc[NG][C];
-  __shared__ float redm[4], redl[4];
   const int tid = threadIdx.x;
-  const int h = blockIdx.x % A.Hq;
-  const int bt = blockIdx.x / A.Hq;
-  const int tok = bt % A.Sq, b = bt / A.Sq;
-  const int Hw = A.Hw, hw = h / A.G, g = h % A.G, T = A.T;
+  const int bt = div_of(A.by_Hq, blockIdx.x), h = blockIdx.x - bt * A.Hq;
+  const int b = div_of(A.by_Sq, bt), tok = bt - b * A.Sq;
+  const int Hw = A.Hw, hw = div_of(A.by_G, h), g = h - hw * A.G, T = A.T;
+  const int qt = div_of(A.by_T, tok), tr = tok - qt * T;
+  grid_wait();
   // own run: n0 partial rows, step0 apart, from row0
   const int64_t step0 = (int64_t)A.G * T * A.Nb[0], step1 = (int64_t)A.G * T * A.Nb[1];
   int64_t row0, row1 = 0;
@@ -99,43 +105,42 @@ __global__ void __launch_bounds__(128) mattn_merge_kernel(const __grid_constant_
   } else {
     const int nq = A.qtiles[0];
     n0 = A.splits[0];
-    row0 = ((((int64_t)b * Hw + hw) * nq + (nq - 1 - tok / T)) * n0) * step0;
+    row0 = ((((int64_t)b * Hw + hw) * nq + (nq - 1 - qt)) * n0) * step0;
   }
-  row0 += (tok % T) * A.G + g;
+  row0 += tr * A.G + g;
   if (A.items1 > 0) {
-    const int nq = A.qtiles[1], tt = (A.Sq + T - 1) / T, qt = (b / A.Nb[1]) * tt + tok / T;
+    const int nq = A.qtiles[1], nb = A.Nb[1], e = b / nb, q1 = e * A.qtiles[0] + qt;
     n1 = A.splits[1];
-    row1 = A.part_off1 + (((int64_t)hw * nq + (nq - 1 - qt)) * n1) * step1 + ((b % A.Nb[1]) * T + tok % T) * A.G + g;
+    row1 = A.part_off1 + (((int64_t)hw * nq + (nq - 1 - q1)) * n1) * step1 + ((b - e * nb) * T + tr) * A.G + g;
   }
   const int ns = n0 + n1;
   if (ns == 1) return;  // the attention kernel wrote the row
   auto part = [&](int s) -> int64_t { return s < n0 ? row0 + s * step0 : row1 + (s - n0) * step1; };
-  float m = -INFINITY;
-  for (int s = tid; s < ns; s += 128) m = fmaxf(m, A.part_ml[part(s)].x);
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if ((tid & 31) == 0) redm[tid >> 5] = m;
-  __syncthreads();
-  const float M = fmaxf(fmaxf(redm[0], redm[1]), fmaxf(redm[2], redm[3]));
+  // every warp finds the maximum and the weights by itself (one round of loads, no exchange)
+  const int lane = tid & 31;
+  float M = -INFINITY;
+  for (int i = lane; i < ns; i += 32) M = fmaxf(M, A.part_ml[part(i)].x);
+  for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
   float l = 0.f;
-  for (int s = tid; s < ns; s += 128) {
-    const float2 ml = A.part_ml[part(s)];
+  for (int i = lane; i < ns; i += 32) {
+    const float2 ml = A.part_ml[part(i)];
     // a NaN sum (its maximum may be -inf: NaN scores leave it) goes on to the output
     const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
-    wgt[s] = w;
+    wgt[i] = w;  // the same from every warp
     l += w * ml.y;
   }
   for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
-  if ((tid & 31) == 0) redl[tid >> 5] = l;
-  __syncthreads();
-  l = (redl[0] + redl[1]) + (redl[2] + redl[3]);
+  __syncwarp();
   const int grp = tid / C, c = tid % C;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   if (grp < NG) {
-#pragma unroll 4
+#pragma unroll 8
     for (int s = grp; s < ns; s += NG) {
+      // (loaded whatever its weight, so that the loads do not wait for one another; the row of a
+      // split that saw nothing was not written)
       const float w = wgt[s];
+      const float4 o = *reinterpret_cast<const float4*>(A.part_o + part(s) * D + 4 * c);
       if (w != 0.f) {
-        const float4 o = *reinterpret_cast<const float4*>(A.part_o + part(s) * D + 4 * c);
         a.x = fmaf(w, o.x, a.x); a.y = fmaf(w, o.y, a.y); a.z = fmaf(w, o.z, a.z); a.w = fmaf(w, o.w, a.w);
       }
     }
@@ -225,9 +230,11 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
       p->even = (int)(cap * (n0 / cap + 1));
     } else {
       // Split the key tiles so that the waves of CTAs are short: a wave costs its longest CTA
-      // (about 2.2 us a tile of head dim 128 with two on an SM, and 5 us to start and end); a
-      // split also writes and reads fp32 partial rows and launches the merge (about 4 us).
-      const double tile_us = D == 256 ? 2.5 : 1.3 + 0.9 * (double)D / 128.0;
+      // (a tile takes its share of the memory's rate, or the softmax of 128 rows; 5 us to start
+      // and end); a split also writes and reads fp32 partial rows and launches the merge (4 us).
+      const bool few = (int64_t)p->G * p->T <= 32;
+      const double mem_us = 1.5 * (double)D / 128.0 * (double)cap / kSms;
+      const double tile_us = few ? mem_us : std::max(mem_us, D == 256 ? 2.5 : 1.3 + 0.9 * (double)D / 128.0);
       const double row_us = (double)(B * Sq * Hq) * (double)D * 8.0 / 5.0e6;
       double best = 1e30;
       for (int64_t n = 1; n <= kSms; ++n) {
@@ -293,12 +300,11 @@ static bool make_map(CUtensorMap* m, const void* base, int64_t D, const int64_t 
 }
 
 template <bool F16>
-static void launch_merge(const Args& a, int64_t D, int64_t rows, cudaStream_t s) {
-  const unsigned grid = (unsigned)rows;
-  if (D == 64) mattn_merge_kernel<64, F16><<<grid, 128, 0, s>>>(a);
-  else if (D == 96) mattn_merge_kernel<96, F16><<<grid, 128, 0, s>>>(a);
-  else if (D == 128) mattn_merge_kernel<128, F16><<<grid, 128, 0, s>>>(a);
-  else mattn_merge_kernel<256, F16><<<grid, 128, 0, s>>>(a);
+static cudaError_t launch_merge(const Args& a, int64_t D, int64_t rows, cudaStream_t s) {
+  auto kern = D == 64 ? mattn_merge_kernel<64, F16>
+                      : D == 96 ? mattn_merge_kernel<96, F16>
+                                : D == 128 ? mattn_merge_kernel<128, F16> : mattn_merge_kernel<256, F16>;
+  return launch_after(kern, dim3((unsigned)rows), 128, 0, s, true, a);
 }
 
 }  // namespace mattn
@@ -395,6 +401,8 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   a.by_group = div(a.group);
   a.by_Hw = div(a.Hw);
   a.by_tt = div(a.qtiles[0]);
+  a.by_Hq = div(Hq);
+  a.by_Sq = div(Sq);
   for (int i = 0; i < 2; ++i) {
     a.by_qtiles[i] = div(a.qtiles[i] > 0 ? a.qtiles[i] : 1);
     a.by_splits[i] = div(a.splits[i]);
@@ -426,7 +434,7 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   const double l2e = 1.4426950408889634;
   a.scale = (float)(M.sm_scale * l2e);
   if (M.softcap > 0.0) {
-    a.cap_in = (float)(2.0 * M.sm_scale / M.softcap * l2e);
+    a.cap_in = (float)(M.sm_scale / M.softcap);
     a.cap_out = (float)(M.softcap * l2e);
   }
   a.slopes = M.slopes;
@@ -443,10 +451,9 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
           M.k_ids, (int)Skv, p.nto, k_ids, reinterpret_cast<int2*>(ws + p.rng_off), rising);
       QF2_LAUNCH_CHECK();
     }
-    mattn_runs_kernel<<<dim3((unsigned)((Sq + 127) / 128), (unsigned)B), 128, 0, s>>>(
-        M.q_ids, k_ids, rising, (int)Sq, (int)Skv, p.nto, reinterpret_cast<int2*>(ws + p.qrng_off),
-        reinterpret_cast<int*>(ws + p.sorted_off));
-    QF2_LAUNCH_CHECK();
+    QF2_CUDA_CHECK(launch_after(mattn_runs_kernel, dim3((unsigned)((Sq + 127) / 128), (unsigned)B), 128, 0, s, p.nto > 0,
+                                M.q_ids, k_ids, rising, (int)Sq, (int)Skv, p.nto,
+                                reinterpret_cast<int2*>(ws + p.qrng_off), reinterpret_cast<int*>(ws + p.sorted_off)));
   }
   const unsigned grid = (unsigned)(p.items[0] + p.items[1]);
   cudaError_t e;
@@ -456,9 +463,7 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   else e = launch_d256(m, a, grid, p.form, f16, score, s);
   QF2_CUDA_CHECK(e);
   if (p.parts) {
-    if (f16) launch_merge<true>(a, D, B * Sq * Hq, s);
-    else launch_merge<false>(a, D, B * Sq * Hq, s);
-    QF2_LAUNCH_CHECK();
+    QF2_CUDA_CHECK(f16 ? launch_merge<true>(a, D, B * Sq * Hq, s) : launch_merge<false>(a, D, B * Sq * Hq, s));
   }
   return QF2_OK;
 }

@@ -78,7 +78,7 @@ struct Args {
   // rows of a tile: G heads x T tokens x Nb batch elements ([0] own items, [1] prefix items)
   int G, T, Nb[2], qtiles[2], splits[2];
   int Hw;                             // head slots: query heads, or kv heads with their group packed
-  Div by_G, by_T, by_group, by_Hw, by_qtiles[2], by_splits[2], by_tt;  // tt: query tiles of a batch element
+  Div by_G, by_T, by_group, by_Hw, by_qtiles[2], by_splits[2], by_tt, by_Hq, by_Sq;  // tt: query tiles of a batch element
   int items1;                         // CTAs of prefix items (they come first)
   int merged;                         // own items walk the prefix tiles too
   int even;                           // > 0: CTAs of the own items, split by what each has to read
@@ -101,7 +101,7 @@ struct Args {
   const int* sorted;                  // [B] key ids in order: q_rng holds
   // scores
   float scale;                        // sm_scale * log2 e
-  float cap_in, cap_out;              // cap > 0: 2 scale log2 e / cap, cap log2 e; else 0
+  float cap_in, cap_out;              // cap > 0: scale / cap, cap log2 e; else 0
   const float* slopes;
   const float* table;                 // [Hq][2 * reach + 1]
   int reach;
@@ -155,11 +155,27 @@ QF2_DEV float bias_log2(float b) {
   return (isinf(r) && !isinf(b)) ? copysignf(3.402823466e38f, b) : r;
 }
 
+// co * tanh(ci x) of two scores by the minimax polynomial of tanh(z) / z in z^2 (Remez exchange,
+// |z| <= 3/4: to 1.9e-7 of the cap), on the FMA pipe: the quotient with an exponential and a
+// reciprocal takes the exponent unit twice as long as the softmax itself does.
+constexpr float kTanhMost = 0.75f;
+QF2_DEV float2 cap_poly(float2 x, float2 ci, float2 co) {
+  const float2 zero = make_float2(0.f, 0.f);
+  const float2 z = ffma2(x, ci, zero), t = ffma2(z, z, zero);
+  float2 p = ffma2(t, make_float2(0.0123188357f, 0.0123188357f), make_float2(-0.0492804514f, -0.0492804514f));
+  p = ffma2(p, t, make_float2(0.132260918f, 0.132260918f));
+  p = ffma2(p, t, make_float2(-0.333230765f, -0.333230765f));
+  p = ffma2(p, t, make_float2(0.999997228f, 0.999997228f));
+  return ffma2(p, ffma2(z, co, zero), zero);
+}
+
 // bits [0, n) of a 32-bit word
 QF2_DEV uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
-// The key tiles of a CTA in order: two runs [a0, a1), [b0, b1) of tile numbers, or (ids out of
-// order) the set bits of words in shared memory; every role walks the same sequence.
+// The key tiles of a CTA: two runs [a0, a0 + na), [b0, ...) of tile numbers, the last first (a
+// bias that falls with the distance has its maximum there, and the running maximum then
+// does not move: single tokens on 32768 keys with slopes 92 -> 62 us), or (ids out of order)
+// the set bits of words in shared memory; every role walks the same sequence.
 struct Tiles {
   int a0, na, b0, j;
   const uint32_t* w;  // null: runs
@@ -167,7 +183,7 @@ struct Tiles {
   uint32_t rest;
   QF2_DEV int next() {
     if (w == nullptr) {
-      const int i = j++;
+      const int i = j--;
       return i < na ? a0 + i : b0 + i - na;
     }
     while (rest == 0) rest = w[++word];
@@ -284,6 +300,9 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     b0 = e * Nb;
     tok0 = (qt - e * A.qtiles[0]) * T;
   }
+  // 32 rows or fewer: four copies of them, one for each softmax warp with a quarter of every key
+  // tile (one warp alone took longer over a tile than its keys take from memory)
+  const bool quad = FORM != kPair && G * T * Nb <= 32;
   const int t_lo = kind ? 0 : (A.merged ? 0 : A.ntp);
   const int t_hi = kind ? A.ntp : A.ntp + A.nto;
 
@@ -307,6 +326,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::misc + 4);
   int* red = reinterpret_cast<int*>(smem + L::misc + 16);  // [softmax warp][8]
 
+  grid_launch_dependents();  // the merge may take its places; it waits for this grid's end
   if (warp == 0) {
     if (lane == 0) {
       mbar_init(bar_q, 1);
@@ -324,11 +344,13 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       *abort_flag = 0;
       fence_mbar_init();
       // Q is on its way while the masks are worked out
-      mbar_arrive_expect_tx(bar_q, (uint32_t)(NT * L::nb) * 128u * (uint32_t)(G * T * Nb));
+      const int copies = quad ? 4 : 1;
+      mbar_arrive_expect_tx(bar_q, (uint32_t)(NT * L::nb * copies) * 128u * (uint32_t)(G * T * Nb));
       for (int t = 0; t < NT; ++t)
         for (int c = 0; c < L::nb; ++c)
-          tma_load_4d(sQ + t * L::op + c * kTile, kind ? &tmq1 : &tmq, c * 64, G > 1 ? hw * G : hw, tok0 + t * T, b0,
-                      bar_q);
+          for (int r = 0; r < copies; ++r)
+            tma_load_4d(sQ + t * L::op + c * kTile + r * 32 * 128, kind ? &tmq1 : &tmq, c * 64, G > 1 ? hw * G : hw,
+                        tok0 + t * T, b0, bar_q);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -341,9 +363,10 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   // [plo, pre), and where ids are out of order only those of its id
   const int tile = NT == 2 ? (warp - W0) >> 2 : 0;
   const int quarter = warp & 3;
-  const int row = quarter * 32 + lane;
+  const int row = quad ? lane : quarter * 32 + lane;
   int rb = 0, rtok = 0, rh = 0, qpos = 0, lo = 0, hi = 0, plo = 0, pre = 0, id = 0;
   bool exists = false;
+  grid_wait();  // for the kernels that prepared the ids (nothing else is still running)
   const bool by_id = A.q_ids != nullptr && A.sorted[b0] == 0;
   if (warp >= W0) {
     const int xr = div_of(A.by_G, row), g = row - xr * G;
@@ -456,7 +479,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     it.a0 = a0;
     it.na = na;
     it.b0 = c0;
-    it.j = f;
+    it.j = f + n - 1;
     it.w = nullptr;
     it.word = w_lo;
     it.rest = 0;
@@ -667,7 +690,11 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     const int a_pre = __reduce_min_sync(0xffffffffu, exists ? pre : 0x7fffffff);
     const int* mine = red + (warp - W0) * 8;
     const int s_lo = mine[0], s_hi = mine[1], s_plo = mine[2], s_pre = mine[3], i_lo = mine[4], i_hi = mine[5];
-    const int q_lo = __reduce_min_sync(0xffffffffu, qpos), q_hi = __reduce_max_sync(0xffffffffu, qpos);
+    // positions of the warp's rows (with tab_smem also of rows past the last query, whose reads of
+    // the table must stay inside it; they follow on)
+    const bool counts = exists || tab_smem;
+    const int q_lo = __reduce_min_sync(0xffffffffu, counts ? qpos : 0x7fffffff);
+    const int q_hi = __reduce_max_sync(0xffffffffu, counts ? qpos : -0x7fffffff);
     float slope2 = 0.f;
     const float* trow = nullptr;
     if constexpr (SCORE) {
@@ -677,27 +704,30 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     }
     float m_run = -INFINITY, l_run = 0.f;
     bool ok = true;
+    // KW: keys of a tile that a thread takes, from k0 on
+    auto softmax = [&](auto kw, const int k0) {
+    constexpr int KW = decltype(kw)::value;
     for (int j = 0; ok && j < n; ++j) {
       const int t = it.next();
       const int buf = DB ? (j & 1) : tile;
       if (!wwait(bar_s + buf, DB ? ((j >> 1) & 1) : (j & 1))) { ok = false; break; }
       tc_fence_after();
-      const uint32_t tS = tmem + lane_off + buf * kBlk;
-      const int p0 = tile_pos(t), pend = tile_end(t), p1 = min(p0 + kBlk, pend);
+      const uint32_t tB = tmem + lane_off + buf * kBlk, tS = tB + k0, tP = tB + k0 / 2;
+      const int p0 = tile_pos(t) + k0, pend = tile_end(t), p1 = min(p0 + KW, pend);
       bool any = warp_rows && ((p0 < s_hi && p1 > s_lo) || (p0 < s_pre && p1 > s_plo));
-      bool full = p0 + kBlk <= pend && ((p1 <= a_hi && p0 >= a_lo) || (p1 <= a_pre && p0 >= a_plo));
+      bool full = p0 + KW <= pend && ((p1 <= a_hi && p0 >= a_lo) || (p1 <= a_pre && p0 >= a_plo));
       const int32_t* kid = nullptr;
       if (krng) {
         const int2 r = krng[t - A.ntp];
         any = any && r.y >= i_lo && r.x <= i_hi;
         if (!(r.x == r.y && i_lo == i_hi && r.x == i_lo)) {
           full = false;
-          kid = A.k_ids + ((int64_t)b0 * A.nto + (t - A.ntp)) * kBlk;
+          kid = A.k_ids + ((int64_t)b0 * A.nto + (t - A.ntp)) * kBlk + k0;
         }
       }
       if (!any) {  // no key of the tile is seen: its weights are zero
 #pragma unroll
-        for (int i = 0; i < 8; ++i) tmem_fill8(tS + 8 * i, 0u);
+        for (int i = 0; i < 8; ++i) tmem_fill8(tB + 8 * i, 0u);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
@@ -707,48 +737,83 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         }
         continue;
       }
-      float xs[128];
+      float xs[KW];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(xs + c * 32));
+      for (int c = 0; c < KW / 32; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(xs + c * 32));
       tmem_wait_ld();
       if constexpr (SCORE) {
+        // the scores in log2 units: capped, then sx times the score plus the bias
+        float sx = A.scale;
         if (A.cap_in > 0.f) {
-          // cap tanh(s / cap) = cap - 2 cap / (1 + e^(2 s / cap)), to 2^-22 of the cap
+          float ma[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            const float e = fast_exp2(xs[i] * A.cap_in);
-            xs[i] = fmaf(-2.f * A.cap_out, fast_rcp(1.f + e), A.cap_out);
+          for (int i = 0; i < KW; i += 8)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) ma[c] = fmax3(ma[c], fabsf(xs[i + 2 * c]), fabsf(xs[i + 2 * c + 1]));
+          const float big = fmaxf(fmaxf(ma[0], ma[1]), fmaxf(ma[2], ma[3]));
+          if (!__any_sync(0xffffffffu, big * A.cap_in > kTanhMost)) {
+            const float2 ci = make_float2(A.cap_in, A.cap_in), co = make_float2(A.cap_out, A.cap_out);
+#pragma unroll
+            for (int i = 0; i < KW / 2; ++i) {
+              const float2 y = cap_poly(make_float2(xs[2 * i], xs[2 * i + 1]), ci, co);
+              xs[2 * i] = y.x;
+              xs[2 * i + 1] = y.y;
+            }
+          } else {
+            // cap tanh(z) = cap - 2 cap / (1 + e^(2 z)), to 2^-22 of the cap
+            const float c2 = 2.f * kLog2e * A.cap_in;
+#pragma unroll
+            for (int i = 0; i < KW; ++i)
+              xs[i] = fmaf(-2.f * A.cap_out, fast_rcp(1.f + fast_exp2(xs[i] * c2)), A.cap_out);
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 128; ++i) xs[i] *= A.scale;
+          sx = 1.f;
         }
+        const float2 sx2 = make_float2(sx, sx);
         if (A.slopes) {
           const float d0 = (float)(qpos - p0);
+          if (q_lo - p0 >= KW - 1 || q_hi <= p0) {
+            // all keys on one side of the warp's queries: the bias is linear in the key
+            const float sg = q_hi <= p0 ? -slope2 : slope2;
+            const float2 sl = make_float2(sg, sg), b = make_float2(-sg * d0, -sg * d0);
 #pragma unroll
-          for (int i = 0; i < 128; ++i) xs[i] = fmaf(-slope2, fabsf(d0 - (float)i), xs[i]);
-        }
-        if (tab_smem) {
-          // distances p0 - q_hi .. p0 + 127 - q_lo of this warp: all beyond the reach?
-          if (p0 - q_hi >= A.reach || p0 + kBlk - 1 - q_lo <= -A.reach) {
+            for (int i = 0; i < KW / 2; ++i) {
+              const float2 y = ffma2(make_float2(xs[2 * i], xs[2 * i + 1]), sx2,
+                                     ffma2(make_float2((float)(2 * i), (float)(2 * i + 1)), sl, b));
+              xs[2 * i] = y.x;
+              xs[2 * i + 1] = y.y;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < KW; ++i) xs[i] = fmaf(-slope2, fabsf(d0 - (float)i), xs[i] * sx);
+          }
+        } else if (tab_smem) {
+          // distances p0 - q_hi .. p0 + KW - 1 - q_lo of this warp: all beyond the reach?
+          const bool far = p0 - q_hi >= A.reach || p0 + KW - 1 - q_lo <= -A.reach;
+          if (far) {
             const float bv = tab[p0 - q_hi >= A.reach ? 2 * A.reach + kTabPad : kTabPad];
+            const float2 b = make_float2(bv, bv);
 #pragma unroll
-            for (int i = 0; i < 128; ++i) xs[i] += bv;
+            for (int i = 0; i < KW / 2; ++i) {
+              const float2 y = ffma2(make_float2(xs[2 * i], xs[2 * i + 1]), sx2, b);
+              xs[2 * i] = y.x;
+              xs[2 * i + 1] = y.y;
+            }
           } else {
             const float* tp = tab + (p0 - qpos + A.reach + kTabPad);
 #pragma unroll
-            for (int i = 0; i < 128; ++i) xs[i] += tp[i];
+            for (int i = 0; i < KW; ++i) xs[i] = fmaf(xs[i], sx, tp[i]);
           }
         } else if (trow) {
           const int d0 = p0 - qpos, R = A.reach;
 #pragma unroll
-          for (int i = 0; i < 128; ++i) xs[i] += bias_log2(__ldg(trow + min(max(d0 + i, -R), R) + R));
+          for (int i = 0; i < KW; ++i)
+            xs[i] = fmaf(xs[i], sx, bias_log2(__ldg(trow + min(max(d0 + i, -R), R) + R)));
         }
       }
       if (!full) {
         const int e = min(hi, pend) - p0, f = lo - p0, g = min(pre, pend) - p0, h = plo - p0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < KW / 32; ++c) {
           const uint32_t w = (low_bits(e - c * 32) & ~low_bits(f - c * 32)) |
                              (low_bits(g - c * 32) & ~low_bits(h - c * 32));
 #pragma unroll
@@ -757,7 +822,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         }
         if (kid) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < KW / 4; ++i) {
             const int4 k4 = *reinterpret_cast<const int4*>(kid + 4 * i);
             if (k4.x != id) xs[4 * i] = -INFINITY;
             if (k4.y != id) xs[4 * i + 1] = -INFINITY;
@@ -770,11 +835,11 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
 #pragma unroll
       for (int c = 0; c < 8; ++c) mq[c] = fmax3(xs[c], xs[c + 8], xs[c + 16]);
 #pragma unroll
-      for (int i = 24; i < 120; i += 16)
+      for (int i = 24; i < KW - 8; i += 16)
 #pragma unroll
         for (int c = 0; c < 8; ++c) mq[c] = fmax3(mq[c], xs[i + c], xs[i + c + 8]);
 #pragma unroll
-      for (int c = 0; c < 8; c += 2) mq[c] = fmax3(mq[c], mq[c + 1], fmaxf(xs[120 + c], xs[121 + c]));
+      for (int c = 0; c < 8; c += 2) mq[c] = fmax3(mq[c], mq[c + 1], fmaxf(xs[KW - 8 + c], xs[KW - 7 + c]));
       float mx = fmaxf(fmax3(mq[0], mq[2], mq[4]), mq[6]);
       if constexpr (!SCORE) mx *= A.scale;
       const float m_new = fmaxf(m_run, mx);
@@ -805,7 +870,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       const float2 scv = make_float2(sc, sc), nm = make_float2(-m_use, -m_use);
       // weights 2^(s - m), rounded over the scores 32 keys at a time
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
+      for (int c = 0; c < KW / 32; ++c) {
         uint32_t w[16];
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
@@ -817,35 +882,121 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
           xs[c * 32 + 2 * q + 1] = e.y;
           w[q] = pack16<F16>(e.x, e.y);
         }
-        if (c == kPart / 32) {  // the stores of the first keys have landed meanwhile
+        if (KW == kBlk && c == kPart / 32) {  // the stores of the first keys have landed meanwhile
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_p + 2 * buf);
         }
-        tmem_st16(tS + c * 16, w);
+        tmem_st16(tP + c * 16, w);
+      }
+      if constexpr (KW < kBlk) {  // the other quarters' keys weigh nothing in this copy of the rows
+#pragma unroll
+        for (int i = 0; i < kBlk / KW; ++i)
+          if (i * KW != k0) {
+            tmem_fill8(tB + i * (KW / 2), 0u);
+            tmem_fill8(tB + i * (KW / 2) + 8, 0u);
+          }
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(bar_p + 2 * buf + 1);
+      if (lane == 0) {
+        if (KW < kBlk) mbar_arrive(bar_p + 2 * buf);
+        mbar_arrive(bar_p + 2 * buf + 1);
+      }
       // the row's sum is taken while the tensor cores go on
       float2 rs[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) rs[c] = make_float2(xs[2 * c], xs[2 * c + 1]);
 #pragma unroll
-      for (int q = 4; q < 64; ++q) rs[q & 3] = fadd2(rs[q & 3], make_float2(xs[2 * q], xs[2 * q + 1]));
+      for (int q = 4; q < KW / 2; ++q) rs[q & 3] = fadd2(rs[q & 3], make_float2(xs[2 * q], xs[2 * q + 1]));
       const float2 rt = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
       l_run += rt.x + rt.y;
     }
+    };
+    if (FORM != kPair && quad)
+      softmax(Int<FORM == kPair ? kBlk : 32>{}, quarter * 32);
+    else
+      softmax(Int<kBlk>{}, 0);
     // ------------------------------------------------------------ epilogue --
     // (DB: the scores of tile n - 1 came after PV n - 3, so the parity names one phase)
     if (ok && n > 0) ok = DB ? wwait(bar_o + ((n - 1) & 1), (uint32_t)(((n - 1) >> 1) & 1)) : wwait(bar_o + tile, 0u);
     if (n == 0) ok = wwait(bar_q, 0);  // Q's copy has landed before its memory is written
     if (!ok) fail(kDevTimeoutEpilogue);
     tc_fence_after();
+    if (FORM != kPair && quad && n > 0) {
+      // the four copies' rows become one, through the memory of Q and the ring (every product and
+      // copy is done): M = max m_q, sum_q 2^(m_q - M) (l_q, O_q); then each warp has a quarter of
+      // the channels
+      constexpr int W = D / 4, pitch = D + 4;
+      float* so = reinterpret_cast<float*>(smem);
+      float2* sml = reinterpret_cast<float2*>(so + kBlk * pitch);
+      static_assert(kBlk * pitch * 4 + kBlk * 8 <= L::tab, "rows of four copies");
+      if (!ok) l_run = 0.f;
+      sml[quarter * 32 + lane] = make_float2(m_run, l_run);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      float M = -INFINITY, l = 0.f, f = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) M = fmaxf(M, sml[q * 32 + lane].x);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float2 e = sml[q * 32 + lane];
+        // (a NaN sum whose maximum is -inf goes on to the output)
+        const float w = e.y == 0.f ? 0.f : (e.x == -INFINITY ? 1.f : fast_exp2(e.x - M));
+        l += w * e.y;
+        if (q == quarter) f = w;
+      }
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32(tO + c * 32, o);
+        tmem_wait_ld();
+        float4* dst = reinterpret_cast<float4*>(so + (quarter * 32 + lane) * pitch + c * 32);
+        if (!exists) continue;
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          dst[v] = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                            : make_float4(__uint_as_float(o[4 * v]) * f, __uint_as_float(o[4 * v + 1]) * f,
+                                          __uint_as_float(o[4 * v + 2]) * f, __uint_as_float(o[4 * v + 3]) * f);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const bool none = !ok || l == 0.f;
+      if (exists) {
+        const bool parts = A.part_o != nullptr && (nsplit > 1 || A.items1 > 0);
+        const int64_t r = (kind ? A.part_off1 : 0) + (int64_t)slot * (G * T * Nb) + row;
+        if (parts && quarter == 0) A.part_ml[r] = none ? make_float2(-INFINITY, 0.f) : make_float2(M, l);
+        const float inv_l = none ? 0.f : 1.0f / l;
+        uint8_t* dst = reinterpret_cast<uint8_t*>(A.out) + 2 * ((int64_t)rb * A.os.b + (int64_t)rh * A.os.h +
+                                                                (int64_t)rtok * A.os.s + quarter * W);
+#pragma unroll 1
+        for (int c = 0; c < W / 8; ++c) {
+          float v[8];
+#pragma unroll
+          for (int u = 0; u < 8; ++u) v[u] = 0.f;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4* src = reinterpret_cast<const float4*>(so + (q * 32 + lane) * pitch + quarter * W + c * 8);
+            const float4 x0 = src[0], x1 = src[1];
+            v[0] += x0.x; v[1] += x0.y; v[2] += x0.z; v[3] += x0.w;
+            v[4] += x1.x; v[5] += x1.y; v[6] += x1.z; v[7] += x1.w;
+          }
+          if (parts) {
+            float4* po = reinterpret_cast<float4*>(A.part_o + r * D + quarter * W + c * 8);
+            if (!none) po[0] = make_float4(v[0], v[1], v[2], v[3]), po[1] = make_float4(v[4], v[5], v[6], v[7]);
+          } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) w[u] = none ? 0u : pack16<F16>(v[2 * u] * inv_l, v[2 * u + 1] * inv_l);
+            *reinterpret_cast<uint4*>(dst + c * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+    const bool joined = FORM != kPair && quad && n > 0;
     const bool zero = !ok || n == 0 || l_run == 0.f;  // NaN sums go on to the output
-    if (A.part_o != nullptr && (nsplit > 1 || A.items1 > 0)) {
+    if (joined) {
+    } else if (A.part_o != nullptr && (nsplit > 1 || A.items1 > 0)) {
       const int64_t r = (kind ? A.part_off1 : 0) + (int64_t)slot * (G * T * Nb) + row;
       if (exists) A.part_ml[r] = zero ? make_float2(-INFINITY, 0.f) : make_float2(m_run, l_run);
       if (warp_rows && n > 0 && ok) {
@@ -906,6 +1057,24 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   }
 }
 
+// A launch that, with `early`, may begin before the kernel ahead of it in the stream has ended
+// (programmatic dependent launch): it reads that kernel's results after grid_wait().
+template <typename... P, typename... V>
+static cudaError_t launch_after(void (*kern)(P...), dim3 grid, unsigned block, int smem, cudaStream_t s, bool early,
+                                const V&... args) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(block);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cfg.attrs = &at;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kern, P(args)...);
+}
+
 struct Maps { CUtensorMap q, q1, o, k, v, pk, pv; };
 
 template <int D, int FORM, bool F16, bool SCORE>
@@ -922,8 +1091,7 @@ static cudaError_t launch_one(const Maps& m, const Args& a, unsigned grid, cudaS
   }
   cudaError_t e = qf2_set_smem_once(kern, L::total, &attr);
   if (e != cudaSuccess) return e;
-  kern<<<grid, threads(L::nt), L::total, s>>>(m.q, m.q1, m.o, m.k, m.v, m.pk, m.pv, a);
-  return cudaGetLastError();
+  return launch_after(kern, grid, threads(L::nt), L::total, s, a.q_ids != nullptr, m.q, m.q1, m.o, m.k, m.v, m.pk, m.pv, a);
 }
 
 template <int D, int FORM>

@@ -48,6 +48,11 @@ QF2_DEV uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// Programmatic dependent launch: the next kernel of the stream may be placed from here on / wait
+// until the kernel ahead has ended and its writes are visible (no effect on a plain launch).
+QF2_DEV void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+QF2_DEV void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 QF2_DEV uint32_t lane_id() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%laneid;" : "=r"(r));
