@@ -103,15 +103,15 @@ __global__ void __launch_bounds__(128) mattn_merge_kernel(const __grid_constant_
     row0 = e.x * step0;
     n0 = e.y;
   } else {
-    const int nq = A.qtiles[0];
     n0 = A.splits[0];
-    row0 = ((((int64_t)b * Hw + hw) * nq + (nq - 1 - qt)) * n0) * step0;
+    row0 = (((int64_t)(A.qtiles[0] - 1 - qt) * A.heads[0] + b * Hw + hw) * n0) * step0;
   }
   row0 += tr * A.G + g;
   if (A.items1 > 0) {
-    const int nq = A.qtiles[1], nb = A.Nb[1], e = b / nb, q1 = e * A.qtiles[0] + qt;
+    const int nb = A.Nb[1], e = b / nb, q1 = e * A.qtiles[0] + qt;
     n1 = A.splits[1];
-    row1 = A.part_off1 + (((int64_t)hw * nq + (nq - 1 - q1)) * n1) * step1 + ((b - e * nb) * T + tr) * A.G + g;
+    row1 = A.part_off1 + (((int64_t)(A.qtiles[1] - 1 - q1) * A.heads[1] + hw) * n1) * step1 +
+           ((b - e * nb) * T + tr) * A.G + g;
   }
   const int ns = n0 + n1;
   if (ns == 1) return;  // the attention kernel wrote the row
@@ -224,10 +224,10 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
     const int64_t cap = deep ? kSms : 2 * kSms;  // CTAs at work at once
     // prefix items: as many splits as fill the SMs, of four tiles or more
     if (n1 > 0) p->splits[1] = (int)std::max<int64_t>(1, std::min((t1 + 3) / 4, std::min<int64_t>(cap / n1, kMaxSplits)));
-    if (p->qtiles[0] == 1 && B <= kMaxEven && t0 > 2 && n0 < 2 * cap) {
-      // one query tile per batch element: split by the keys each has (lengths are known on the
-      // device), over a grid of whole waves
-      p->even = (int)(cap * (n0 / cap + 1));
+    if (p->qtiles[0] == 1 && B <= kMaxEven && t0 > 2 && n0 < cap) {
+      // one query tile per batch element, and fewer than fill the SMs: split by the keys each has
+      // (lengths are known on the device)
+      p->even = (int)cap;
     } else {
       // Split the key tiles so that the waves of CTAs are short: a wave costs its longest CTA
       // (a tile takes its share of the memory's rate, or the softmax of 128 rows; 5 us to start
@@ -404,7 +404,8 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   a.by_Hq = div(Hq);
   a.by_Sq = div(Sq);
   for (int i = 0; i < 2; ++i) {
-    a.by_qtiles[i] = div(a.qtiles[i] > 0 ? a.qtiles[i] : 1);
+    a.heads[i] = a.Hw * (i == 0 ? a.B : 1);
+    a.by_heads[i] = div(a.heads[i]);
     a.by_splits[i] = div(a.splits[i]);
   }
   a.items1 = (int)p.items[1];

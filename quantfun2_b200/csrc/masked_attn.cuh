@@ -78,7 +78,8 @@ struct Args {
   // rows of a tile: G heads x T tokens x Nb batch elements ([0] own items, [1] prefix items)
   int G, T, Nb[2], qtiles[2], splits[2];
   int Hw;                             // head slots: query heads, or kv heads with their group packed
-  Div by_G, by_T, by_group, by_Hw, by_qtiles[2], by_splits[2], by_tt, by_Hq, by_Sq;  // tt: query tiles of a batch element
+  int heads[2];                       // head slots of all batch elements (prefix items: of one)
+  Div by_G, by_T, by_group, by_Hw, by_heads[2], by_splits[2], by_tt, by_Hq, by_Sq;  // tt: query tiles of a batch element
   int items1;                         // CTAs of prefix items (they come first)
   int merged;                         // own items walk the prefix tiles too
   int even;                           // > 0: CTAs of the own items, split by what each has to read
@@ -288,10 +289,12 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   } else {
     const int y = div_of(A.by_splits[kind], x);
     split = x - y * nsplit;
-    const int nq = A.qtiles[kind], z = div_of(A.by_qtiles[kind], y);
-    qt = nq - 1 - (y - z * nq);  // the last rows first: a causal mask gives them the most keys
-    b0 = div_of(A.by_Hw, z);
-    hw = z - b0 * Hw;
+    // the last rows of all heads first: a causal mask gives them the most keys, and the short
+    // items fill the end of the grid (heads outermost: 4352 tokens 256 against 999 us)
+    const int z = div_of(A.by_heads[kind], y), w = y - z * A.heads[kind];
+    qt = A.qtiles[kind] - 1 - z;
+    b0 = div_of(A.by_Hw, w);
+    hw = w - b0 * Hw;
   }
   const int hk = G > 1 ? hw : div_of(A.by_group, hw);
   int tok0 = qt * NT * T;
@@ -327,13 +330,73 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   int* red = reinterpret_cast<int*>(smem + L::misc + 16);  // [softmax warp][8]
 
   grid_launch_dependents();  // the merge may take its places; it waits for this grid's end
+
+  // ---------------------------------------------------------- active tiles --
+  // position of a key tile's first key, the end of its store, and the tile of a position
+  auto tile_pos = [&](int t) -> int { return t < A.ntp ? t * kBlk : A.P + (t - A.ntp) * kBlk; };
+  auto tile_end = [&](int t) -> int { return t < A.ntp ? A.P : 0x7fffffff; };
+  auto tile_at = [&](int p) -> int { return p < A.P ? p / kBlk : A.ntp + (p - A.P) / kBlk; };
+  // what any row of the CTA sees: [ulo, uhi), [uplo, upre), and (ids out of order) ids uid0 .. uid1
+  int ulo = 0x7fffffff, uhi = 0, uplo = 0x7fffffff, upre = 0, uid0 = 0x7fffffff, uid1 = -1;
+  Tiles it;
+  int n = 0;  // tiles of this CTA
+  // the two runs in order, without what they share, and this split's part of them
+  auto share = [&](int total) -> int {  // first of the split's tiles (at most 2^13 tiles and kMaxSplits splits)
+    n = total;
+    if (nsplit == 1) return 0;
+    const int f = (int)((uint32_t)(total * split) / (uint32_t)nsplit);
+    n = (int)((uint32_t)(total * (split + 1)) / (uint32_t)nsplit) - f;
+    return f;
+  };
+  auto runs = [&]() -> int {
+    int a0 = t_lo, a1 = t_lo, c0 = t_lo, c1 = t_lo;
+    if (uplo < upre) a0 = max(tile_at(uplo), t_lo), a1 = min(tile_at(upre - 1) + 1, t_hi);
+    if (ulo < uhi) c0 = max(tile_at(ulo), t_lo), c1 = min(tile_at(uhi - 1) + 1, t_hi);
+    if (a0 >= a1 || (c0 < c1 && c0 < a0)) {
+      const int s0 = a0, s1 = a1;
+      a0 = c0, a1 = c1, c0 = s0, c1 = s1;
+    }
+    c0 = max(c0, a1);
+    it.a0 = a0;
+    it.na = max(a1 - a0, 0);
+    it.b0 = c0;
+    it.w = nullptr;
+    it.word = 0;
+    it.rest = 0;
+    return it.na + max(c1 - c0, 0);
+  };
+  // Rows of one batch element without ids are consecutive positions: what they see follows from the
+  // first and the last, and the first keys are on their way before the rows are looked at.
+  const bool direct = A.q_ids == nullptr && Nb == 1;
+  if (direct) {
+    const Span s = span_of(A, b0);
+    const int first = s.off + tok0, last = s.off + min(tok0 + NT * T, A.Sq) - 1;
+    ulo = A.left < 0 ? 0 : max(first - A.left, 0);
+    uhi = A.right < 0 ? s.len : min(max(last + A.right + 1, 0), s.len);
+    uplo = 0;
+    upre = s.pre;
+    const int total = runs();
+    it.j = share(total) + n - 1;
+  }
+  // K (kv = 0) or V of the CTA's j-th tile t into its ring slot
+  auto load_kv = [&](int t, int kv, int i) {
+    const bool px = t < A.ntp;
+    const int y = (px ? t : t - A.ntp) * kBlk, sl = i % NS;
+    const CUtensorMap* m = kv ? (px ? &tmpv : &tmv) : (px ? &tmpk : &tmk);
+    uint8_t* dst = sR + sl * L::op;
+    mbar_arrive_expect_tx(bar_full + sl, L::op);
+    for (int c = 0; c < L::nb; ++c) tma_load_4d(dst + c * kTile, m, c * 64, y, hk, px ? 0 : b0, bar_full + sl);
+  };
+  int ahead = 0;  // tiles loaded before the others are there
   if (warp == 0) {
     if (lane == 0) {
       mbar_init(bar_q, 1);
+#pragma unroll 1
       for (int s = 0; s < NS; ++s) {
         mbar_init(bar_full + s, 1);
         mbar_init(bar_empty + s, 1);
       }
+#pragma unroll 1
       for (int s = 0; s < 2; ++s) {
         mbar_init(bar_s + s, 1);
         mbar_init(bar_p + 2 * s, 4);
@@ -343,16 +406,28 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       mbar_init(bar_drain, 1);
       *abort_flag = 0;
       fence_mbar_init();
-      // Q is on its way while the masks are worked out
       const int copies = quad ? 4 : 1;
       mbar_arrive_expect_tx(bar_q, (uint32_t)(NT * L::nb * copies) * 128u * (uint32_t)(G * T * Nb));
+#pragma unroll 1
       for (int t = 0; t < NT; ++t)
+#pragma unroll 1
         for (int c = 0; c < L::nb; ++c)
+#pragma unroll 1
           for (int r = 0; r < copies; ++r)
             tma_load_4d(sQ + t * L::op + c * kTile + r * 32 * 128, kind ? &tmq1 : &tmq, c * 64, G > 1 ? hw * G : hw,
                         tok0 + t * T, b0, bar_q);
     }
     __syncwarp();
+    if (direct) {
+      for (; ahead < NS / 2 && ahead < n; ++ahead) {
+        const int t = it.next();
+        if (lane == 0) {
+          load_kv(t, 0, 2 * ahead);
+          load_kv(t, 1, 2 * ahead + 1);
+        }
+      }
+      __syncwarp();
+    }
   } else if (warp == 1) {
     tmem_alloc(tmem_slot, L::cols);
     tmem_relinquish();
@@ -368,6 +443,8 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   bool exists = false;
   grid_wait();  // for the kernels that prepared the ids (nothing else is still running)
   const bool by_id = A.q_ids != nullptr && A.sorted[b0] == 0;
+  // what any row of this warp sees
+  int s_lo = 0x7fffffff, s_hi = 0, s_plo = 0x7fffffff, s_pre = 0, i_lo = 0x7fffffff, i_hi = -1;
   if (warp >= W0) {
     const int xr = div_of(A.by_G, row), g = row - xr * G;
     const int xb = div_of(A.by_T, xr);
@@ -399,11 +476,18 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     if (!sees || plo >= pre) plo = pre = 0;
     const bool blind = !(lo < hi || plo < pre);
     const int big = 0x7fffffff;
-    const int v[6] = {__reduce_min_sync(0xffffffffu, lo < hi ? lo : big), __reduce_max_sync(0xffffffffu, hi),
-                      __reduce_min_sync(0xffffffffu, plo < pre ? plo : big), __reduce_max_sync(0xffffffffu, pre),
-                      __reduce_min_sync(0xffffffffu, blind ? big : id), __reduce_max_sync(0xffffffffu, blind ? -1 : id)};
-    if (lane == 0)
-      for (int i = 0; i < 6; ++i) red[(warp - W0) * 8 + i] = v[i];
+    s_lo = __reduce_min_sync(0xffffffffu, lo < hi ? lo : big);
+    s_hi = __reduce_max_sync(0xffffffffu, hi);
+    s_plo = __reduce_min_sync(0xffffffffu, plo < pre ? plo : big);
+    s_pre = __reduce_max_sync(0xffffffffu, pre);
+    if (by_id) {
+      i_lo = __reduce_min_sync(0xffffffffu, blind ? big : id);
+      i_hi = __reduce_max_sync(0xffffffffu, blind ? -1 : id);
+    }
+    if (!direct && lane == 0) {
+      int* mine = red + (warp - W0) * 8;
+      mine[0] = s_lo, mine[1] = s_hi, mine[2] = s_plo, mine[3] = s_pre, mine[4] = i_lo, mine[5] = i_hi;
+    }
   }
   // the head's distance table with clamped pads (log2 units), where the rows of a warp are
   // consecutive positions of one head
@@ -418,43 +502,26 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  // what any row of the CTA sees: [ulo, uhi), [uplo, upre), ids uid0 .. uid1
-  int ulo = 0x7fffffff, uhi = 0, uplo = 0x7fffffff, upre = 0, uid0 = 0x7fffffff, uid1 = -1;
-#pragma unroll
-  for (int w = 0; w < 4 * NT; ++w) {
-    ulo = min(ulo, red[w * 8]);
-    uhi = max(uhi, red[w * 8 + 1]);
-    uplo = min(uplo, red[w * 8 + 2]);
-    upre = max(upre, red[w * 8 + 3]);
-    uid0 = min(uid0, red[w * 8 + 4]);
-    uid1 = max(uid1, red[w * 8 + 5]);
-  }
-
-  // ---------------------------------------------------------- active tiles --
-  // position of a key tile's first key, the end of its store, and the tile of a position
-  auto tile_pos = [&](int t) -> int { return t < A.ntp ? t * kBlk : A.P + (t - A.ntp) * kBlk; };
-  auto tile_end = [&](int t) -> int { return t < A.ntp ? A.P : 0x7fffffff; };
-  auto tile_at = [&](int p) -> int { return p < A.P ? p / kBlk : A.ntp + (p - A.P) / kBlk; };
   const int2* krng = by_id ? A.k_rng + (int64_t)b0 * A.nto : nullptr;
-  int n = 0;  // tiles of this CTA
-  Tiles it;
-  {
-    int total, w_lo = t_lo >> 5;
-    // the two runs in order, without what they share
-    int a0 = t_lo, a1 = t_lo, c0 = t_lo, c1 = t_lo;
-    if (uplo < upre) a0 = max(tile_at(uplo), t_lo), a1 = min(tile_at(upre - 1) + 1, t_hi);
-    if (ulo < uhi) c0 = max(tile_at(ulo), t_lo), c1 = min(tile_at(uhi - 1) + 1, t_hi);
-    if (a0 >= a1 || (c0 < c1 && c0 < a0)) {
-      const int s0 = a0, s1 = a1;
-      a0 = c0, a1 = c1, c0 = s0, c1 = s1;
+  if (!direct) {
+#pragma unroll 1
+    for (int w = 0; w < 4 * NT; ++w) {
+      ulo = min(ulo, red[w * 8]);
+      uhi = max(uhi, red[w * 8 + 1]);
+      uplo = min(uplo, red[w * 8 + 2]);
+      upre = max(upre, red[w * 8 + 3]);
+      uid0 = min(uid0, red[w * 8 + 4]);
+      uid1 = max(uid1, red[w * 8 + 5]);
     }
-    c0 = max(c0, a1);
-    const int na = max(a1 - a0, 0), nc = max(c1 - c0, 0);
-    if (krng) {
-      const int w_hi = (t_hi + 31) >> 5;
+    int total = runs();
+    if (!krng) {
+      it.j = share(total) + n - 1;
+    } else {
+      const int w_lo = t_lo >> 5, w_hi = (t_hi + 31) >> 5;
+      const int a1 = it.a0 + it.na, c1 = it.b0 + total - it.na;
       for (int w = w_lo + warp; w < w_hi; w += kThreads / 32) {
         const int t = w * 32 + lane;
-        bool act = (t >= a0 && t < a1) || (t >= c0 && t < c1);
+        bool act = (t >= it.a0 && t < a1) || (t >= it.b0 && t < c1);
         if (act) {
           const int2 r = krng[t - A.ntp];
           act = r.y >= uid0 && r.x <= uid1;
@@ -466,34 +533,18 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       total = 0;
       for (int w = w_lo + lane; w < w_hi; w += 32) total += __popc(bits[w]);
       total = __reduce_add_sync(0xffffffffu, total);
-    } else {
-      total = na + nc;
-    }
-    // (at most 2^13 tiles and kMaxSplits splits)
-    int f = 0;
-    n = total;
-    if (nsplit > 1) {
-      f = (int)((uint32_t)(total * split) / (uint32_t)nsplit);
-      n = (int)((uint32_t)(total * (split + 1)) / (uint32_t)nsplit) - f;
-    }
-    it.a0 = a0;
-    it.na = na;
-    it.b0 = c0;
-    it.j = f + n - 1;
-    it.w = nullptr;
-    it.word = w_lo;
-    it.rest = 0;
-    if (krng && n > 0) {
-      int skip = f, w = w_lo;
-      uint32_t rest = bits[w];
-      while (skip >= __popc(rest)) {
-        skip -= __popc(rest);
-        rest = bits[++w];
+      int skip = share(total), w = w_lo;
+      if (n > 0) {
+        uint32_t rest = bits[w];
+        while (skip >= __popc(rest)) {
+          skip -= __popc(rest);
+          rest = bits[++w];
+        }
+        for (; skip > 0; --skip) rest &= rest - 1;
+        it.w = bits;
+        it.word = w;
+        it.rest = rest;
       }
-      for (; skip > 0; --skip) rest &= rest - 1;
-      it.w = bits;
-      it.word = w;
-      it.rest = rest;
     }
   }
 
@@ -516,13 +567,11 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
     if (warp == 0) {
       // ---------------------------------------------------------- producer --
-      int issued = 0;
+      int issued = 2 * ahead;
       bool ok = true;
-      for (int j = 0; ok && j < n; ++j) {
+      for (int j = ahead; ok && j < n; ++j) {
         const int t = it.next();
-        const bool px = t < A.ntp;
-        const int y = (px ? t : t - A.ntp) * kBlk;
-#pragma unroll
+#pragma unroll 1
         for (int kv = 0; kv < 2; ++kv) {
           const int i = 2 * j + kv, s = i % NS;
           if (!wwait(bar_empty + s, ((i / NS) & 1) ^ 1)) {
@@ -530,12 +579,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
             ok = false;
             break;
           }
-          if (lane == 0) {
-            const CUtensorMap* m = kv ? (px ? &tmpv : &tmv) : (px ? &tmpk : &tmk);
-            uint8_t* dst = sR + s * L::op;
-            mbar_arrive_expect_tx(bar_full + s, L::op);
-            for (int c = 0; c < L::nb; ++c) tma_load_4d(dst + c * kTile, m, c * 64, y, hk, px ? 0 : b0, bar_full + s);
-          }
+          if (lane == 0) load_kv(t, kv, i);
           __syncwarp();
           issued = i + 1;
         }
@@ -688,8 +732,6 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     const int a_hi = __reduce_min_sync(0xffffffffu, exists ? hi : 0x7fffffff);
     const int a_plo = __reduce_max_sync(0xffffffffu, exists ? plo : 0);
     const int a_pre = __reduce_min_sync(0xffffffffu, exists ? pre : 0x7fffffff);
-    const int* mine = red + (warp - W0) * 8;
-    const int s_lo = mine[0], s_hi = mine[1], s_plo = mine[2], s_pre = mine[3], i_lo = mine[4], i_hi = mine[5];
     // positions of the warp's rows (with tab_smem also of rows past the last query, whose reads of
     // the table must stay inside it; they follow on)
     const bool counts = exists || tab_smem;
