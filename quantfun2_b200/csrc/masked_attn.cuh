@@ -378,55 +378,51 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     const int total = runs();
     it.j = share(total) + n - 1;
   }
-  // K (kv = 0) or V of the CTA's j-th tile t into its ring slot
+  // K (kv = 0) or V of key tile t into ring slot i % NS
   auto load_kv = [&](int t, int kv, int i) {
     const bool px = t < A.ntp;
     const int y = (px ? t : t - A.ntp) * kBlk, sl = i % NS;
     const CUtensorMap* m = kv ? (px ? &tmpv : &tmv) : (px ? &tmpk : &tmk);
     uint8_t* dst = sR + sl * L::op;
-    mbar_arrive_expect_tx(bar_full + sl, L::op);
-    for (int c = 0; c < L::nb; ++c) tma_load_4d(dst + c * kTile, m, c * 64, y, hk, px ? 0 : b0, bar_full + sl);
+    if (elect_one()) {
+      mbar_arrive_expect_tx(bar_full + sl, L::op);
+#pragma unroll
+      for (int c = 0; c < L::nb; ++c) tma_load_4d(dst + c * kTile, m, c * 64, y, hk, px ? 0 : b0, bar_full + sl);
+    }
+    __syncwarp();
   };
   int ahead = 0;  // tiles loaded before the others are there
   if (warp == 0) {
-    if (lane == 0) {
-      mbar_init(bar_q, 1);
-#pragma unroll 1
-      for (int s = 0; s < NS; ++s) {
-        mbar_init(bar_full + s, 1);
-        mbar_init(bar_empty + s, 1);
-      }
-#pragma unroll 1
-      for (int s = 0; s < 2; ++s) {
-        mbar_init(bar_s + s, 1);
-        mbar_init(bar_p + 2 * s, 4);
-        mbar_init(bar_p + 2 * s + 1, 4);
-        mbar_init(bar_o + s, 1);
-      }
-      mbar_init(bar_drain, 1);
+    // one barrier a lane (one lane for all: 830 cycles)
+    static_assert(L::nbars <= 32, "a barrier a lane");
+    if (lane < L::nbars) mbar_init(bars + lane, bars + lane >= bar_p && bars + lane < bar_p + 4 ? 4 : 1);
+    fence_mbar_init();
+    __syncwarp();
+    if (elect_one()) {
       *abort_flag = 0;
-      fence_mbar_init();
-      const int copies = quad ? 4 : 1;
-      mbar_arrive_expect_tx(bar_q, (uint32_t)(NT * L::nb * copies) * 128u * (uint32_t)(G * T * Nb));
-#pragma unroll 1
-      for (int t = 0; t < NT; ++t)
-#pragma unroll 1
-        for (int c = 0; c < L::nb; ++c)
-#pragma unroll 1
-          for (int r = 0; r < copies; ++r)
-            tma_load_4d(sQ + t * L::op + c * kTile + r * 32 * 128, kind ? &tmq1 : &tmq, c * 64, G > 1 ? hw * G : hw,
-                        tok0 + t * T, b0, bar_q);
+      const CUtensorMap* mq = kind ? &tmq1 : &tmq;
+      const int h0 = G > 1 ? hw * G : hw;
+      mbar_arrive_expect_tx(bar_q, (uint32_t)(NT * L::nb * (quad ? 4 : 1)) * 128u * (uint32_t)(G * T * Nb));
+      if (FORM != kPair && quad) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int c = 0; c < L::nb; ++c)
+            tma_load_4d(sQ + c * kTile + r * 32 * 128, mq, c * 64, h0, tok0, b0, bar_q);
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int c = 0; c < L::nb; ++c)
+            tma_load_4d(sQ + t * L::op + c * kTile, mq, c * 64, h0, tok0 + t * T, b0, bar_q);
+      }
     }
     __syncwarp();
-    if (direct) {
-      for (; ahead < NS / 2 && ahead < n; ++ahead) {
-        const int t = it.next();
-        if (lane == 0) {
-          load_kv(t, 0, 2 * ahead);
-          load_kv(t, 1, 2 * ahead + 1);
-        }
-      }
-      __syncwarp();
+    if (direct && n > 0) {
+      const int t = it.next();
+      load_kv(t, 0, 0);
+      load_kv(t, 1, 1);
+      ahead = 1;
     }
   } else if (warp == 1) {
     tmem_alloc(tmem_slot, L::cols);
@@ -579,8 +575,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
             ok = false;
             break;
           }
-          if (lane == 0) load_kv(t, kv, i);
-          __syncwarp();
+          load_kv(t, kv, i);
           issued = i + 1;
         }
       }
