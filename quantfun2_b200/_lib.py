@@ -6,7 +6,6 @@ an sm_100 part, every op raises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import struct
@@ -238,16 +237,14 @@ def require_device(t) -> None:
         raise QF2Error(f"device {idx} is not compute capability 10.0 (B200); sm_100a kernels only")
 
 
-_NO_GUARD = contextlib.nullcontext()
-
-
-def on_device(device):
-    """Context in which `device` is current (the library launches on the current device)."""
+def call_on(device, fn, args: bytes) -> int:
+    """fn(args) with `device` current (the library launches on the current device)."""
     import torch
 
-    if device.index is None or device.index == torch.cuda.current_device():
-        return _NO_GUARD
-    return torch.cuda.device(device)
+    if device.index == torch._C._cuda_getDevice():
+        return fn(args)
+    with torch.cuda.device(device):
+        return fn(args)
 
 
 def raw_stream(index: int) -> int:
@@ -263,13 +260,18 @@ def stream_ptr(device=None) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def dtype_code(dt) -> int:
-    import torch
+_dtype_codes: dict = {}
 
-    m = {torch.float32: QF2_F32, torch.float16: QF2_F16, torch.bfloat16: QF2_BF16}
-    if dt not in m:
+
+def dtype_code(dt) -> int:
+    if not _dtype_codes:
+        import torch
+
+        _dtype_codes.update({torch.float32: QF2_F32, torch.float16: QF2_F16, torch.bfloat16: QF2_BF16})
+    code = _dtype_codes.get(dt)
+    if code is None:
         raise QF2Error(f"unsupported dtype {dt}")
-    return m[dt]
+    return code
 
 
 def header_symbols(header: str | os.PathLike | None = None) -> list[str]:

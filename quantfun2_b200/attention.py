@@ -21,7 +21,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import QF2Error, check, i64, on_device, ptr32, raw_stream, require_device, stream_ptr
+from ._lib import QF2Error, call_on, check, i64, ptr32, raw_stream, require_device, stream_ptr
 
 __all__ = ["sageattn", "sageattn_varlen", "sage_quantize", "sage_workspace_layout", "block_topk_select",
            "blocksparse_attn", "flash_attn", "masked_attn", "shared_prefix_attn", "masked_attn_status", "do_attn",
@@ -380,8 +380,7 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
         vs[0], vs[h], vs[n], os[0], os[h], os[n], pk_h, pk_n, pv_h, pv_n, B, Hq, Hkv, Sq, Skv, P, D, dt, left, right,
         lens_p, pre_p, off_p, off, mode, qi_p, ki_p, slope_p, table_p, reach, softcap or 0.0, sm_scale,
         ws.data_ptr() if nbytes else 0, nbytes, raw_stream(dev.index))
-    with on_device(dev):
-        status = _lib.load().qf2_masked_attn(args)
+    status = call_on(dev, _lib.load().qf2_masked_attn, args)
     if status:
         check(status, "qf2_masked_attn")
     return out
@@ -435,7 +434,7 @@ def masked_attn_status(device=None) -> None:
     """Waits for the current stream of `device` and raises QF2Error if a masked_attn or
     shared_prefix_attn call on it gave up a bounded wait since the last check."""
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
-    with on_device(dev):
+    with torch.cuda.device(dev):
         check(_lib.load().qf2_masked_attn_status(stream_ptr(dev)), "masked attention")
 
 

@@ -14,56 +14,56 @@ namespace mattn {
 __device__ int g_status;
 
 // ------------------------------------------------------------- key ids --
-// Padded copy of a batch element's key ids (tiles of 128, pad -2), the least and greatest id of
-// each tile, and whether the tile's ids, and the next tile's first, do not fall (as unsigned
-// numbers: the negative ids of padding come last).  grid (nto, B), 128 threads.
-__global__ void __launch_bounds__(128) mattn_ids_kernel(const int32_t* __restrict__ ids, int Skv, int nto,
-                                                        int32_t* __restrict__ out, int2* __restrict__ rng,
-                                                        int* __restrict__ rising) {
-  const int t = blockIdx.x, b = blockIdx.y, i = threadIdx.x;
-  const int j = t * kBlk + i;
-  grid_launch_dependents();
-  const int v = j < Skv ? ids[(int64_t)b * Skv + j] : -2;
-  const int next = j + 1 < Skv ? ids[(int64_t)b * Skv + j + 1] : -1;
-  const int fine = __syncthreads_and(j + 1 >= Skv || (uint32_t)v <= (uint32_t)next);
-  out[((int64_t)b * nto + t) * kBlk + i] = v;
-  __shared__ int2 part[4];
-  const int mn = __reduce_min_sync(0xffffffffu, v), mx = __reduce_max_sync(0xffffffffu, v);
-  if ((i & 31) == 0) part[i >> 5] = make_int2(mn, mx);
-  __syncthreads();
-  if (i == 0) {
-    rng[(int64_t)b * nto + t] = make_int2(min(min(part[0].x, part[1].x), min(part[2].x, part[3].x)),
-                                          max(max(part[0].y, part[1].y), max(part[2].y, part[3].y)));
-    rising[(int64_t)b * nto + t] = fine;
-  }
-}
-
-// Where a batch element's key ids are in order, the keys of each query's id are one run: the
-// attention kernel then masks by ranges (documents, padded ends) and looks at no id.  A warp
-// takes 32 queries, one id among them at a time: the tiles whose first key comes before the
-// id are counted, then such keys of the last of these tiles.  grid (ceil(Sq / 128), B), 128 threads.
-__global__ void __launch_bounds__(128) mattn_runs_kernel(const int32_t* __restrict__ q_ids,
-                                                         const int32_t* __restrict__ k_ids,
-                                                         const int* __restrict__ rising, int Sq, int Skv, int nto,
+// What the attention kernel wants to know of ids, in one launch.  grid (kb + qb, B), 1024 threads.
+// The first kb blocks of a batch element: a padded copy of the key ids (tiles of 128, pad -2) and
+// the least and greatest id of each tile, eight tiles a block.
+// The other qb blocks, 1024 queries each: whether the key ids never fall (as unsigned numbers, so
+// that the negative ids of padding come last), which each block sees for itself; then the keys of
+// a query's id are one run, found here, and the attention kernel masks by ranges and looks at no
+// id.  A warp takes 32 queries, one id among them at a time: the tiles whose first key comes
+// before the id are counted, then such keys of the last of these tiles.
+__global__ void __launch_bounds__(1024) mattn_ids_kernel(const int32_t* __restrict__ q_ids,
+                                                         const int32_t* __restrict__ k_ids, int Sq, int Skv, int nto,
+                                                         int kb, int32_t* __restrict__ copy, int2* __restrict__ k_rng,
                                                          int2* __restrict__ q_rng, int* __restrict__ sorted) {
-  const int b = blockIdx.y, i = blockIdx.x * 128 + threadIdx.x, lane = threadIdx.x & 31;
-  const int id = i < Sq ? q_ids[(int64_t)b * Sq + i] : -1;
   grid_launch_dependents();
-  grid_wait();
+  const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int32_t* k = k_ids + (int64_t)b * Skv;
+  if ((int)blockIdx.x < kb) {
+    const int j = blockIdx.x * 1024 + threadIdx.x, t = j / kBlk;
+    const int v = j < Skv ? k[j] : -2;
+    __shared__ int2 part[32];
+    const int mn = __reduce_min_sync(0xffffffffu, v), mx = __reduce_max_sync(0xffffffffu, v);
+    if (lane == 0) part[warp] = make_int2(mn, mx);
+    __syncthreads();
+    if (t >= nto) return;
+    copy[(int64_t)b * nto * kBlk + j] = v;
+    if ((threadIdx.x & (kBlk - 1)) == 0) {
+      const int2 p0 = part[warp], p1 = part[warp + 1], p2 = part[warp + 2], p3 = part[warp + 3];
+      k_rng[(int64_t)b * nto + t] = make_int2(min(min(p0.x, p1.x), min(p2.x, p3.x)), max(max(p0.y, p1.y), max(p2.y, p3.y)));
+    }
+    return;
+  }
+  const int i = (blockIdx.x - kb) * 1024 + threadIdx.x;
+  const int id = i < Sq ? q_ids[(int64_t)b * Sq + i] : -1;
   int fine = 1;
-  for (int t = threadIdx.x; t < nto; t += 128) fine &= rising[(int64_t)b * nto + t];
+#pragma unroll 4
+  for (int j = threadIdx.x; j < Skv - 1; j += 1024) fine &= (uint32_t)k[j] <= (uint32_t)k[j + 1];
   fine = __syncthreads_and(fine);
-  if (blockIdx.x == 0 && threadIdx.x == 0) sorted[b] = fine;
+  if ((int)blockIdx.x == kb && threadIdx.x == 0) sorted[b] = fine;
   if (!fine) return;
-  const int32_t* k = k_ids + (int64_t)b * nto * kBlk;
-  // keys of less than x (as unsigned numbers), by the warp; the pads come after every id
+  // keys of less than x (as unsigned numbers), by the warp
   auto below = [&](uint32_t x) -> int {
     int tiles = 0;
     for (int t = lane; t < nto; t += 32) tiles += (uint32_t)k[(int64_t)t * kBlk] < x;
     tiles = __reduce_add_sync(0xffffffffu, tiles);
     if (tiles == 0) return 0;
-    const int4 v = *reinterpret_cast<const int4*>(k + (int64_t)(tiles - 1) * kBlk + 4 * lane);
-    const int n = ((uint32_t)v.x < x) + ((uint32_t)v.y < x) + ((uint32_t)v.z < x) + ((uint32_t)v.w < x);
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < kBlk; u += 32) {
+      const int j = (tiles - 1) * kBlk + u + lane;
+      n += j < Skv && (uint32_t)k[j] < x;
+    }
     return (tiles - 1) * kBlk + __reduce_add_sync(0xffffffffu, n);
   };
   int2 r = make_int2(0, 0);
@@ -168,7 +168,7 @@ struct Plan {
   int64_t items[2];  // CTAs of own and prefix items, splits counted
   bool parts;        // partial rows and a merge
   int64_t rows0;     // partial rows of the own items
-  int64_t ids_off, rng_off, rising_off, qrng_off, sorted_off, tab_off, ml_off, o_off, bytes;
+  int64_t ids_off, rng_off, qrng_off, sorted_off, tab_off, ml_off, o_off, bytes;
 };
 
 static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P, int64_t D,
@@ -268,7 +268,6 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   };
   p->ids_off = take(ids, B * nto * kBlk * 4);
   p->rng_off = take(ids, B * nto * 8);
-  p->rising_off = take(ids, B * nto * 4);
   p->qrng_off = take(ids, B * Sq * 8);
   p->sorted_off = take(ids, B * 4);
   p->tab_off = take(p->even > 0, B * hw * 8);
@@ -445,16 +444,12 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   const bool score = M.softcap > 0.0 || M.slopes || M.bias_table;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(M.stream);
   if (ids) {
-    int32_t* k_ids = reinterpret_cast<int32_t*>(ws + p.ids_off);
-    int* rising = reinterpret_cast<int*>(ws + p.rising_off);
-    if (p.nto > 0) {
-      mattn_ids_kernel<<<dim3((unsigned)p.nto, (unsigned)B), 128, 0, s>>>(
-          M.k_ids, (int)Skv, p.nto, k_ids, reinterpret_cast<int2*>(ws + p.rng_off), rising);
-      QF2_LAUNCH_CHECK();
-    }
-    QF2_CUDA_CHECK(launch_after(mattn_runs_kernel, dim3((unsigned)((Sq + 127) / 128), (unsigned)B), 128, 0, s, p.nto > 0,
-                                M.q_ids, k_ids, rising, (int)Sq, (int)Skv, p.nto,
-                                reinterpret_cast<int2*>(ws + p.qrng_off), reinterpret_cast<int*>(ws + p.sorted_off)));
+    const int kb = (p.nto + 7) / 8;
+    mattn_ids_kernel<<<dim3((unsigned)(kb + (Sq + 1023) / 1024), (unsigned)B), 1024, 0, s>>>(
+        M.q_ids, M.k_ids, (int)Sq, (int)Skv, p.nto, kb, reinterpret_cast<int32_t*>(ws + p.ids_off),
+        reinterpret_cast<int2*>(ws + p.rng_off), reinterpret_cast<int2*>(ws + p.qrng_off),
+        reinterpret_cast<int*>(ws + p.sorted_off));
+    QF2_LAUNCH_CHECK();
   }
   const unsigned grid = (unsigned)(p.items[0] + p.items[1]);
   cudaError_t e;

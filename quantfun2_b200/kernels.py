@@ -26,7 +26,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import QF2Error, check, dtype_code, i64, on_device, raw_stream, require_device, stream_ptr
+from ._lib import QF2Error, call_on, check, dtype_code, i64, raw_stream, require_device, stream_ptr
 
 __all__ = [
     "copy_chunks",
@@ -210,8 +210,7 @@ def _rotary(xq, xk, positions, inv_freq, out_q, out_k, layout, magnitude, invers
         xq.data_ptr(), out_q.data_ptr(), kp, kop, positions.data_ptr(), inv_freq.data_ptr(), qs[0], qs[1], qs[2],
         qo[0], qo[1], qo[2], ks[0], ks[1], ks[2], ko[0], ko[1], ko[2], pb, pp, pdt == torch.int64, B, S, Hq, Hk, D,
         2 * inv_freq.shape[0], mode, bool(inverse), dt, magnitude, raw_stream(index))
-    with on_device(dev):
-        st = _lib.load().qf2_rotary_apply(args)
+    st = call_on(dev, _lib.load().qf2_rotary_apply, args)
     if st:
         check(st, "qf2_rotary_apply")
 
