@@ -774,114 +774,144 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         }
         continue;
       }
-      float xs[KW];
+      // The scores 32 at a time, first for the maximum, then for the weights: all in registers, or
+      // (kSmall, which has fewer) out of tensor memory twice, where capped, biased or masked ones
+      // went back to.  Prompts of 64 x 512 keys take 33 us in registers and 27 us in two short
+      // loops; kPair the other way 1385 us in registers, 1438 us in loops (causal 16384 tokens).
+      constexpr bool kHeld = KW == 32 || FORM != kSmall;
+      const bool far = SCORE && tab_smem && (p0 - q_hi >= A.reach || p0 + KW - 1 - q_lo <= -A.reach);
+      const int e_hi = min(hi, pend) - p0, e_lo = lo - p0, e_pre = min(pre, pend) - p0, e_plo = plo - p0;
+      float mx = -INFINITY;
+      // N scores, the first of key c of this thread's
+      auto prepare = [&](float* x, auto count, int c) {
+        constexpr int N = decltype(count)::value;
+        if constexpr (SCORE) {
+          // the scores in log2 units: capped, then sx times the score plus the bias
+          float sx = A.scale;
+          const int q0 = p0 + c;  // position of x[0]
+          if (A.cap_in > 0.f) {
+            float ma[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int c = 0; c < KW / 32; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(xs + c * 32));
-      tmem_wait_ld();
-      if constexpr (SCORE) {
-        // the scores in log2 units: capped, then sx times the score plus the bias
-        float sx = A.scale;
-        if (A.cap_in > 0.f) {
-          float ma[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < N; i += 8)
 #pragma unroll
-          for (int i = 0; i < KW; i += 8)
+              for (int u = 0; u < 4; ++u) ma[u] = fmax3(ma[u], fabsf(x[i + 2 * u]), fabsf(x[i + 2 * u + 1]));
+            const float big = fmaxf(fmaxf(ma[0], ma[1]), fmaxf(ma[2], ma[3]));
+            if (!__any_sync(0xffffffffu, big * A.cap_in > kTanhMost)) {
+              const float2 ci = make_float2(A.cap_in, A.cap_in), co = make_float2(A.cap_out, A.cap_out);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) ma[c] = fmax3(ma[c], fabsf(xs[i + 2 * c]), fabsf(xs[i + 2 * c + 1]));
-          const float big = fmaxf(fmaxf(ma[0], ma[1]), fmaxf(ma[2], ma[3]));
-          if (!__any_sync(0xffffffffu, big * A.cap_in > kTanhMost)) {
-            const float2 ci = make_float2(A.cap_in, A.cap_in), co = make_float2(A.cap_out, A.cap_out);
+              for (int i = 0; i < N / 2; ++i) {
+                const float2 y = cap_poly(make_float2(x[2 * i], x[2 * i + 1]), ci, co);
+                x[2 * i] = y.x;
+                x[2 * i + 1] = y.y;
+              }
+            } else {
+              // cap tanh(z) = cap - 2 cap / (1 + e^(2 z)), to 2^-22 of the cap
+              const float c2 = 2.f * kLog2e * A.cap_in;
 #pragma unroll
-            for (int i = 0; i < KW / 2; ++i) {
-              const float2 y = cap_poly(make_float2(xs[2 * i], xs[2 * i + 1]), ci, co);
-              xs[2 * i] = y.x;
-              xs[2 * i + 1] = y.y;
+              for (int i = 0; i < N; ++i)
+                x[i] = fmaf(-2.f * A.cap_out, fast_rcp(1.f + fast_exp2(x[i] * c2)), A.cap_out);
             }
-          } else {
-            // cap tanh(z) = cap - 2 cap / (1 + e^(2 z)), to 2^-22 of the cap
-            const float c2 = 2.f * kLog2e * A.cap_in;
-#pragma unroll
-            for (int i = 0; i < KW; ++i)
-              xs[i] = fmaf(-2.f * A.cap_out, fast_rcp(1.f + fast_exp2(xs[i] * c2)), A.cap_out);
+            sx = 1.f;
           }
-          sx = 1.f;
+          const float2 sx2 = make_float2(sx, sx);
+          if (A.slopes) {
+            const float d0 = (float)(qpos - q0);
+            if (q_lo - q0 >= N - 1 || q_hi <= q0) {
+              // all keys on one side of the warp's queries: the bias is linear in the key
+              const float sg = q_hi <= q0 ? -slope2 : slope2;
+              const float2 sl = make_float2(sg, sg), bb = make_float2(-sg * d0, -sg * d0);
+#pragma unroll
+              for (int i = 0; i < N / 2; ++i) {
+                const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), sx2,
+                                       ffma2(make_float2((float)(2 * i), (float)(2 * i + 1)), sl, bb));
+                x[2 * i] = y.x;
+                x[2 * i + 1] = y.y;
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < N; ++i) x[i] = fmaf(-slope2, fabsf(d0 - (float)i), x[i] * sx);
+            }
+          } else if (tab_smem) {
+            if (far) {  // all distances of the warp beyond the table's reach
+              const float bv = tab[p0 - q_hi >= A.reach ? 2 * A.reach + kTabPad : kTabPad];
+              const float2 bb = make_float2(bv, bv);
+#pragma unroll
+              for (int i = 0; i < N / 2; ++i) {
+                const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), sx2, bb);
+                x[2 * i] = y.x;
+                x[2 * i + 1] = y.y;
+              }
+            } else {
+              const float* tp = tab + (q0 - qpos + A.reach + kTabPad);
+#pragma unroll
+              for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], sx, tp[i]);
+            }
+          } else if (trow) {
+            const int d0 = q0 - qpos, R = A.reach;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              x[i] = fmaf(x[i], sx, bias_log2(__ldg(trow + min(max(d0 + i, -R), R) + R)));
+          }
         }
-        const float2 sx2 = make_float2(sx, sx);
-        if (A.slopes) {
-          const float d0 = (float)(qpos - p0);
-          if (q_lo - p0 >= KW - 1 || q_hi <= p0) {
-            // all keys on one side of the warp's queries: the bias is linear in the key
-            const float sg = q_hi <= p0 ? -slope2 : slope2;
-            const float2 sl = make_float2(sg, sg), b = make_float2(-sg * d0, -sg * d0);
+        if (!full) {
 #pragma unroll
-            for (int i = 0; i < KW / 2; ++i) {
-              const float2 y = ffma2(make_float2(xs[2 * i], xs[2 * i + 1]), sx2,
-                                     ffma2(make_float2((float)(2 * i), (float)(2 * i + 1)), sl, b));
-              xs[2 * i] = y.x;
-              xs[2 * i + 1] = y.y;
-            }
-          } else {
+          for (int u = 0; u < N; u += 32) {
+            const uint32_t w = (low_bits(e_hi - c - u) & ~low_bits(e_lo - c - u)) |
+                               (low_bits(e_pre - c - u) & ~low_bits(e_plo - c - u));
 #pragma unroll
-            for (int i = 0; i < KW; ++i) xs[i] = fmaf(-slope2, fabsf(d0 - (float)i), xs[i] * sx);
+            for (int i = 0; i < 32; ++i)
+              if (!((w >> i) & 1u)) x[u + i] = -INFINITY;
           }
-        } else if (tab_smem) {
-          // distances p0 - q_hi .. p0 + KW - 1 - q_lo of this warp: all beyond the reach?
-          const bool far = p0 - q_hi >= A.reach || p0 + KW - 1 - q_lo <= -A.reach;
-          if (far) {
-            const float bv = tab[p0 - q_hi >= A.reach ? 2 * A.reach + kTabPad : kTabPad];
-            const float2 b = make_float2(bv, bv);
+          if (kid) {
 #pragma unroll
-            for (int i = 0; i < KW / 2; ++i) {
-              const float2 y = ffma2(make_float2(xs[2 * i], xs[2 * i + 1]), sx2, b);
-              xs[2 * i] = y.x;
-              xs[2 * i + 1] = y.y;
+            for (int i = 0; i < N / 4; ++i) {
+              const int4 k4 = *reinterpret_cast<const int4*>(kid + c + 4 * i);
+              if (k4.x != id) x[4 * i] = -INFINITY;
+              if (k4.y != id) x[4 * i + 1] = -INFINITY;
+              if (k4.z != id) x[4 * i + 2] = -INFINITY;
+              if (k4.w != id) x[4 * i + 3] = -INFINITY;
             }
-          } else {
-            const float* tp = tab + (p0 - qpos + A.reach + kTabPad);
-#pragma unroll
-            for (int i = 0; i < KW; ++i) xs[i] = fmaf(xs[i], sx, tp[i]);
           }
-        } else if (trow) {
-          const int d0 = p0 - qpos, R = A.reach;
+        }
+        if (!kHeld && (SCORE || !full)) tmem_st32(tS + c, *reinterpret_cast<uint32_t(*)[32]>(x));
+        float m[8];
 #pragma unroll
-          for (int i = 0; i < KW; ++i)
-            xs[i] = fmaf(xs[i], sx, bias_log2(__ldg(trow + min(max(d0 + i, -R), R) + R)));
+        for (int u = 0; u < 8; ++u) m[u] = fmax3(x[u], x[u + 8], x[u + 16]);
+#pragma unroll
+        for (int i = 24; i < N - 8; i += 16)
+#pragma unroll
+          for (int u = 0; u < 8; ++u) m[u] = fmax3(m[u], x[i + u], x[i + u + 8]);
+#pragma unroll
+        for (int u = 0; u < 8; u += 2) m[u] = fmax3(m[u], m[u + 1], fmaxf(x[N - 8 + u], x[N - 7 + u]));
+        mx = fmax3(fmax3(mx, m[0], m[2]), m[4], m[6]);
+      };
+      auto fetch = [&](float* x, int c) { tmem_ld32(tS + c, *reinterpret_cast<uint32_t(*)[32]>(x)); };
+      float xs[kHeld ? KW : 64];
+      if constexpr (kHeld) {
+#pragma unroll
+        for (int c = 0; c < KW; c += 32) fetch(xs + c, c);
+        tmem_wait_ld();
+        prepare(xs, Int<KW>{}, 0);
+      } else {
+        fetch(xs, 0);
+#pragma unroll 1
+        for (int c = 0; c < KW; c += 64) {
+          tmem_wait_ld();
+          fetch(xs + 32, c + 32);
+          prepare(xs, Int<32>{}, c);
+          tmem_wait_ld();
+          if (c + 64 < KW) fetch(xs, c + 64);
+          prepare(xs + 32, Int<32>{}, c + 32);
         }
       }
-      if (!full) {
-        const int e = min(hi, pend) - p0, f = lo - p0, g = min(pre, pend) - p0, h = plo - p0;
-#pragma unroll
-        for (int c = 0; c < KW / 32; ++c) {
-          const uint32_t w = (low_bits(e - c * 32) & ~low_bits(f - c * 32)) |
-                             (low_bits(g - c * 32) & ~low_bits(h - c * 32));
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (!((w >> i) & 1u)) xs[c * 32 + i] = -INFINITY;
-        }
-        if (kid) {
-#pragma unroll
-          for (int i = 0; i < KW / 4; ++i) {
-            const int4 k4 = *reinterpret_cast<const int4*>(kid + 4 * i);
-            if (k4.x != id) xs[4 * i] = -INFINITY;
-            if (k4.y != id) xs[4 * i + 1] = -INFINITY;
-            if (k4.z != id) xs[4 * i + 2] = -INFINITY;
-            if (k4.w != id) xs[4 * i + 3] = -INFINITY;
-          }
-        }
-      }
-      float mq[8];
-#pragma unroll
-      for (int c = 0; c < 8; ++c) mq[c] = fmax3(xs[c], xs[c + 8], xs[c + 16]);
-#pragma unroll
-      for (int i = 24; i < KW - 8; i += 16)
-#pragma unroll
-        for (int c = 0; c < 8; ++c) mq[c] = fmax3(mq[c], xs[i + c], xs[i + c + 8]);
-#pragma unroll
-      for (int c = 0; c < 8; c += 2) mq[c] = fmax3(mq[c], mq[c + 1], fmaxf(xs[KW - 8 + c], xs[KW - 7 + c]));
-      float mx = fmaxf(fmax3(mq[0], mq[2], mq[4]), mq[6]);
       if constexpr (!SCORE) mx *= A.scale;
       const float m_new = fmaxf(m_run, mx);
       // (tile rows that do not exist hold whatever shared memory held: they have no vote)
       const bool rescale = __any_sync(0xffffffffu, exists && m_new > m_run + kTau);
+      if constexpr (!kHeld) {
+        if (SCORE || !full) tmem_wait_st();
+        fetch(xs, 0);
+      }
       if (rescale) {
         const float alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
         m_run = m_new;
@@ -905,35 +935,54 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
       const float sc = SCORE ? 1.f : A.scale;
       const float2 scv = make_float2(sc, sc), nm = make_float2(-m_use, -m_use);
-      // weights 2^(s - m), rounded over the scores 32 keys at a time
-#pragma unroll
-      for (int c = 0; c < KW / 32; ++c) {
+      float2 rs0 = make_float2(0.f, 0.f), rs1 = rs0, rs2 = rs0, rs3 = rs0;
+      // weights 2^(s - m), rounded over the scores (16 columns for 32 keys: behind those read)
+      auto weigh = [&](float* x, int c) {
         uint32_t w[16];
 #pragma unroll
         for (int q = 0; q < 16; ++q) {
-          float2 e = make_float2(xs[c * 32 + 2 * q], xs[c * 32 + 2 * q + 1]);
+          float2 e = make_float2(x[2 * q], x[2 * q + 1]);
           e = SCORE ? fadd2(e, nm) : ffma2(e, scv, nm);
           e.x = fast_exp2(e.x);
           e.y = fast_exp2(e.y);
-          xs[c * 32 + 2 * q] = e.x;
-          xs[c * 32 + 2 * q + 1] = e.y;
+          if (kHeld) {
+            x[2 * q] = e.x;
+            x[2 * q + 1] = e.y;
+          } else if (q & 1) {
+            rs1 = fadd2(rs1, e);
+          } else {
+            rs0 = fadd2(rs0, e);
+          }
           w[q] = pack16<F16>(e.x, e.y);
         }
-        if (KW == kBlk && c == kPart / 32) {  // the stores of the first keys have landed meanwhile
+        if (KW == kBlk && c == kPart) {  // the stores of the first keys have landed meanwhile
           tmem_wait_st();
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(bar_p + 2 * buf);
         }
-        tmem_st16(tP + c * 16, w);
-      }
-      if constexpr (KW < kBlk) {  // the other quarters' keys weigh nothing in this copy of the rows
+        tmem_st16(tP + c / 2, w);
+      };
+      if constexpr (kHeld) {
+#pragma unroll
+        for (int c = 0; c < KW; c += 32) weigh(xs + c, c);
+        // (quarters: the other ones' keys weigh nothing in this copy of the rows)
 #pragma unroll
         for (int i = 0; i < kBlk / KW; ++i)
-          if (i * KW != k0) {
+          if (KW < kBlk && i * KW != k0) {
             tmem_fill8(tB + i * (KW / 2), 0u);
             tmem_fill8(tB + i * (KW / 2) + 8, 0u);
           }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < KW; c += 64) {
+          tmem_wait_ld();
+          fetch(xs + 32, c + 32);
+          weigh(xs, c);
+          tmem_wait_ld();
+          if (c + 64 < KW) fetch(xs, c + 64);
+          weigh(xs + 32, c + 32);
+        }
       }
       tmem_wait_st();
       tc_fence_before();
@@ -942,14 +991,18 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         if (KW < kBlk) mbar_arrive(bar_p + 2 * buf);
         mbar_arrive(bar_p + 2 * buf + 1);
       }
-      // the row's sum is taken while the tensor cores go on
-      float2 rs[4];
+      if constexpr (kHeld) {  // the row's sum is taken while the tensor cores go on
 #pragma unroll
-      for (int c = 0; c < 4; ++c) rs[c] = make_float2(xs[2 * c], xs[2 * c + 1]);
-#pragma unroll
-      for (int q = 4; q < KW / 2; ++q) rs[q & 3] = fadd2(rs[q & 3], make_float2(xs[2 * q], xs[2 * q + 1]));
-      const float2 rt = fadd2(fadd2(rs[0], rs[1]), fadd2(rs[2], rs[3]));
-      l_run += rt.x + rt.y;
+        for (int q = 0; q < KW; q += 8) {
+          rs0 = fadd2(rs0, make_float2(xs[q], xs[q + 1]));
+          rs1 = fadd2(rs1, make_float2(xs[q + 2], xs[q + 3]));
+          rs2 = fadd2(rs2, make_float2(xs[q + 4], xs[q + 5]));
+          rs3 = fadd2(rs3, make_float2(xs[q + 6], xs[q + 7]));
+        }
+        rs0 = fadd2(rs0, rs2);
+        rs1 = fadd2(rs1, rs3);
+      }
+      l_run += (rs0.x + rs1.x) + (rs0.y + rs1.y);
     }
     };
     if (FORM != kPair && quad)
