@@ -284,7 +284,9 @@ int qf2_blocksparse_attn(const void* q, const int64_t* q_strides, const void* k,
  * most 8192 key tiles of 128; R <= 1024.  Arrays on the device, contiguous.  Scores, sums
  * and outputs are fp32, probabilities are rounded to the operand type.
  * A bounded wait that gave up is reported by qf2_masked_attn_status (synchronizes the
- * stream, clears the word; one word per device for all calls). */
+ * stream, clears the word; one word per device for all calls).  Make the first call on a
+ * device before any stream capture (it loads the kernels).  The output must not overlap the
+ * inputs. */
 #define QF2_OFFSET_CONST 0
 #define QF2_OFFSET_ARRAY 1
 #define QF2_OFFSET_END 2

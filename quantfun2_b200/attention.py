@@ -342,9 +342,8 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
         qi, ki = segment_ids if isinstance(segment_ids, (tuple, list)) else (segment_ids, segment_ids)
         qi = _int32(qi, (B, Sq), "segment_ids of the queries", dev)
         ki = _int32(ki, (B, Skv), "segment_ids of the keys", dev)
-        qi_p, ki_p = qi.data_ptr(), ki.data_ptr()
-        if ki_p == 0:
-            ki_p = qi_p = 16  # no keys: never read, but ids are in use
+        if Skv:  # (without keys every row is zero, whatever its id)
+            qi_p, ki_p = qi.data_ptr(), ki.data_ptr()
     if q_offset is None:
         if kv_lens is not None and (left >= 0 or right >= 0 or slopes is not None or bias_table is not None):
             raise QF2Error("with kv_lens, give q_offset: 0 for right-padded prompts, 'end' for the last tokens of a "
@@ -373,7 +372,7 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
         table_p, reach = bias_table.data_ptr(), bias_table.shape[1] // 2
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    nbytes = _masked_workspace(B, Hq, Hkv, Sq, Skv, P, D, int(segment_ids is not None))
+    nbytes = _masked_workspace(B, Hq, Hkv, Sq, Skv, P, D, int(ki_p != 0))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     args = _lib.MASKED_ATTN_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), pkp, pvp, qs[0], qs[h], qs[n], ks[0], ks[h], ks[n],

@@ -385,19 +385,19 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   a.out = M.out;
   a.os = S3{M.out_strides[0], M.out_strides[1], M.out_strides[2]};
   a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Sq = (int)Sq; a.Skv = (int)Skv; a.P = (int)P;
-  a.ntp = p.ntp; a.nto = p.nto; a.group = (int)(Hq / Hkv);
+  a.ntp = p.ntp; a.nto = p.nto;
   a.G = p.G; a.T = p.T;
   for (int i = 0; i < 2; ++i) { a.Nb[i] = p.Nb[i]; a.qtiles[i] = p.qtiles[i]; a.splits[i] = p.splits[i]; }
   a.Hw = (int)(Hq / p.G);
   auto div = [](int64_t d) {
-    Div v{(uint32_t)d, 0, 0};
+    Div v{0, 0};
     while ((1ll << v.s) < d) ++v.s;
     v.m = (uint32_t)(((1ull << 32) * ((1ull << v.s) - (uint64_t)d)) / (uint64_t)d + 1);
     return v;
   };
   a.by_G = div(a.G);
   a.by_T = div(a.T);
-  a.by_group = div(a.group);
+  a.by_group = div(Hq / Hkv);
   a.by_Hw = div(a.Hw);
   a.by_tt = div(a.qtiles[0]);
   a.by_Hq = div(Hq);

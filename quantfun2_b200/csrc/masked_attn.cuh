@@ -25,9 +25,13 @@
 // A tile's rows are (batch element, token, query head of a group): one row per token, or all
 // query heads of a kv head packed side by side, so that single tokens read K and V once.
 //
-// Bound for long queries by one chain per tile: scores read, maximum, 128 exponentials a row
-// (the exponent unit takes 16 per SM and cycle, as long as both products), probabilities
-// stored, the last of P V and the next Q K^T.
+// Long queries are bound by one chain per tile (scores read, maximum, 128 exponentials a row,
+// probabilities stored, the last of P V, the next Q K^T: 3300 cycles for two tiles of which the
+// exponent unit works 2048 and the tensor cores 2100), and by the board's power: 16384 causal
+// tokens of 24/8 heads of 128 take 1.38 ms cold (1190 TFLOP/s) and 1.6 ms in a long run, where the
+// clock falls to 1.7 GHz.  Single tokens are bound by HBM: 16 elements on 8192 keys of 24
+// heads 6.4 TB/s.  Short calls are bound by what a CTA does once: 3 us until the first scores,
+// 2.5 us after the last.
 #pragma once
 #include "qf2_common.cuh"
 
@@ -65,7 +69,7 @@ constexpr int kRegsFew = 88, kRegsSoftmax = 208;
 
 // Division by a number known on the host: x / d = (umulhi(x, m) + x) >> s for x < 2^31.
 struct Div {
-  uint32_t d, m, s;
+  uint32_t m, s;
 };
 QF2_DEV int div_of(const Div& v, int x) { return (int)((__umulhi((uint32_t)x, v.m) + (uint32_t)x) >> v.s); }
 
@@ -74,12 +78,12 @@ struct Args {
   S3 os;
   int B, Hq, Hkv, Sq, Skv, P;       // own keys, shared prefix keys
   int ntp, nto;                       // key tiles of the prefix and of the own keys
-  int group;                          // query heads per kv head
   // rows of a tile: G heads x T tokens x Nb batch elements ([0] own items, [1] prefix items)
   int G, T, Nb[2], qtiles[2], splits[2];
   int Hw;                             // head slots: query heads, or kv heads with their group packed
   int heads[2];                       // head slots of all batch elements (prefix items: of one)
-  Div by_G, by_T, by_group, by_Hw, by_heads[2], by_splits[2], by_tt, by_Hq, by_Sq;  // tt: query tiles of a batch element
+  // (group: query heads per kv head; tt: query tiles of a batch element)
+  Div by_G, by_T, by_group, by_Hw, by_heads[2], by_splits[2], by_tt, by_Hq, by_Sq;
   int items1;                         // CTAs of prefix items (they come first)
   int merged;                         // own items walk the prefix tiles too
   int even;                           // > 0: CTAs of the own items, split by what each has to read
@@ -215,8 +219,8 @@ QF2_DEV Span span_of(const Args& A, int b) {
 template <int D, int FORM, bool F16, bool SCORE>
 __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall ? 2 : 1)
     masked_attn_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmq1,
-                       const __grid_constant__ CUtensorMap tmo,
-                       const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
+                       const __grid_constant__ CUtensorMap tmo, const __grid_constant__ CUtensorMap tmk,
+                       const __grid_constant__ CUtensorMap tmv,
                        const __grid_constant__ CUtensorMap tmpk, const __grid_constant__ CUtensorMap tmpv,
                        const __grid_constant__ Args A) {
   using L = Smem<D, FORM>;
@@ -290,7 +294,8 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     const int y = div_of(A.by_splits[kind], x);
     split = x - y * nsplit;
     // the last rows of all heads first: a causal mask gives them the most keys, and the short
-    // items fill the end of the grid (heads outermost: 4352 tokens 256 against 999 us)
+    // items fill the end of the grid (a head's rows side by side: 4352 tokens with a prefix 256 against 222 us, 16384 causal 1465
+    // against 1385)
     const int z = div_of(A.by_heads[kind], y), w = y - z * A.heads[kind];
     qt = A.qtiles[kind] - 1 - z;
     b0 = div_of(A.by_Hw, w);
@@ -443,11 +448,13 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   int s_lo = 0x7fffffff, s_hi = 0, s_plo = 0x7fffffff, s_pre = 0, i_lo = 0x7fffffff, i_hi = -1;
   if (warp >= W0) {
     const int xr = div_of(A.by_G, row), g = row - xr * G;
-    const int xb = div_of(A.by_T, xr);
+    // (rows behind the tile's last token go on from it where they are of one batch element: the
+    // distance table is indexed by consecutive positions)
+    const int xb = Nb > 1 ? div_of(A.by_T, xr) : 0;
     rtok = tok0 + tile * T + xr - xb * T;
     rb = b0 + xb;
     rh = G > 1 ? hw * G + g : hw;
-    exists = xb < Nb && rb < A.B && rtok < A.Sq;
+    exists = (Nb > 1 ? xb < Nb : xr < T) && rb < A.B && rtok < A.Sq;
     const int bc = min(rb, A.B - 1);
     const Span s = span_of(A, bc);
     qpos = s.off + rtok;

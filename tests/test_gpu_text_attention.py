@@ -212,6 +212,57 @@ def test_few_tokens_on_caches(cuda, B, Sq, Skv, Hq, Hkv, D, dtype):
     _compare(out, q, k, v, window=(77, 0), kv_lens=lens.tolist(), offsets=[n - Sq for n in lens.tolist()])
 
 
+@pytest.mark.parametrize("Sq", [1, 5, 40, 100])
+def test_distance_table_for_few_tokens_of_unlike_lengths(cuda, Sq):
+    """One head a row, several batch elements: tile rows behind the last token belong to none."""
+    from quantfun2_b200 import attention as A
+
+    B, Skv, H, D = 3, 700, 2, 64
+    q, k, v = _inputs(cuda, B, Sq, Skv, H, H, D, BF16, seed=Sq)
+    lens = torch.tensor([700, 110, 333], device=cuda)
+    for R in (3, 200):
+        table = torch.randn(H, 2 * R + 1, device=cuda)
+        out = A.masked_attn(q, k, v, window=(-1, 0), kv_lens=lens, q_offset="end", bias_table=table, tensor_layout="NHD")
+        _compare(out, q, k, v, window=(-1, 0), kv_lens=lens.tolist(), offsets=[n - Sq for n in lens.tolist()],
+                 bias_table=table)
+
+
+def test_many_batch_elements(cuda):
+    """More elements than lengths are weighed for, on caches of a few tiles."""
+    from quantfun2_b200 import attention as A
+
+    B, Skv, Hq, Hkv, D = 1500, 400, 2, 1, 64
+    q, k, v = _inputs(cuda, B, 1, Skv, Hq, Hkv, D, BF16, seed=40)
+    lens = torch.randint(0, Skv + 1, (B,), device=cuda, generator=torch.Generator(device=cuda).manual_seed(1))
+    out = A.masked_attn(q, k, v, window=(-1, 0), kv_lens=lens, q_offset="end", tensor_layout="NHD")
+    pick = [0, 1, 700, 1023, 1024, 1499]
+    _compare(out[pick], q[pick], k[pick], v[pick], window=(-1, 0), kv_lens=lens[pick].tolist(),
+             offsets=[n - 1 for n in lens[pick].tolist()])
+
+
+def test_longest_cache_and_offsets_past_32_bits(cuda):
+    """2^20 keys of 48 heads: element offsets pass 2^31, key tiles reach their limit."""
+    from quantfun2_b200 import attention as A
+
+    S, H, D = 1 << 20, 48, 64
+    q = torch.randn(1, 2, H, D, device=cuda).to(BF16)
+    k = torch.empty(1, S, H, D, device=cuda, dtype=BF16).normal_()
+    v = torch.empty(1, S, H, D, device=cuda, dtype=BF16).normal_()
+    assert k.numel() > 2 ** 31
+    lens = torch.tensor([S - 77], device=cuda)
+    ids = torch.zeros(1, S, dtype=torch.int32, device=cuda)
+    ids[0, ::3] = 1                                            # out of order: every tile is looked at by id
+    for kw, ref in ((dict(kv_lens=lens, q_offset="end", window=(-1, 0)), dict(kv_lens=[S - 77], offsets=[S - 79], window=(-1, 0))),
+                    (dict(kv_lens=lens, q_offset="end", window=(300, 0)), dict(kv_lens=[S - 77], offsets=[S - 79], window=(300, 0))),
+                    (dict(segment_ids=(ids[:, :2], ids)), dict(q_ids=ids[:, :2], k_ids=ids))):
+        out = A.masked_attn(q, k, v, tensor_layout="NHD", **kw)
+        for h in (0, H - 1):
+            sl = slice(h, h + 1)
+            # sums over 2^20 keys: the bound's 2^13 terms are for shorter ones; errors of fp32 sums
+            # over tiles add up to 2^13 tiles * 2^-24 = 2^-11 of the sum at most, already inside it
+            _compare(out[:, :, sl], q[:, :, sl], k[:, :, sl], v[:, :, sl], **ref)
+
+
 @pytest.mark.parametrize("B,S,P,Hq,Hkv,D,dtype", [
     (3, 1, 1000, 4, 2, 128, BF16), (64, 1, 3001, 6, 2, 96, FP16), (5, 40, 77, 4, 4, 64, BF16), (2, 300, 130, 2, 1, 256, BF16),
     (8, 300, 260, 24, 8, 128, BF16), (130, 1, 129, 2, 2, 64, BF16), (1, 1, 1, 1, 1, 64, FP16), (9, 3, 500, 4, 1, 128, FP16),
@@ -245,6 +296,9 @@ def test_no_keys_and_no_queries(cuda):
         q, k, v = _inputs(cuda, 2, Sq, 0, 80, 80, 64, BF16)
         out = torch.full_like(q, 7.0)
         assert A.masked_attn(q, k, v, window=(-1, 0), tensor_layout="NHD", out=out) is out and not out.any()
+        ids = (torch.zeros(2, Sq, device=cuda, dtype=torch.int32), torch.zeros(2, 0, device=cuda, dtype=torch.int32))
+        out = A.masked_attn(q, k, v, segment_ids=ids, tensor_layout="NHD")
+        assert out.shape == q.shape and not out.any()
     q, k, v, pk, pv = _inputs(cuda, 2, 5, 0, 2, 2, 64, BF16, P=30)
     out = A.shared_prefix_attn(q, pk, pv, k, v, tensor_layout="NHD")
     _compare(out, q, k, v, rows=[0, 4], offsets=[0, 0], prefix_k=pk, prefix_v=pv)
