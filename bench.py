@@ -663,7 +663,22 @@ def profile_cases(dev) -> dict:
         fr = rope_freqs(flux_position_ids(1, 512, 64, 64, dev), (16, 56, 56))
         return lambda: m(img, txt, t, y, fr)
 
-    return {"lumina_step": lumina_step, "flux_step": flux_step, "rope": rope, "qkv_norm_rope": qkv_norm_rope, "rmsnorm": rmsnorm, "softmax": softmax,
+    def rotary():        # positions -> rotated q and k of a long text
+        q, k = rn(1, 65537, 24, 128).to(bf), rn(1, 65537, 8, 128).to(bf)
+        pos, f = torch.arange(65537, device=dev), K.rotary_inv_freq(128, device=dev)
+        return lambda: K.rotary_apply(q, k, pos, f)
+
+    def masked_attn_case(q_len):  # a causal text, or single tokens on four 32768-key caches
+        def case():
+            from quantfun2_b200.attention import masked_attn
+
+            b, n = (1, q_len) if q_len > 1 else (4, 32768)
+            q, k, v = rn(b, q_len, 24, 128).to(bf), rn(b, n, 8, 128).to(bf), rn(b, n, 8, 128).to(bf)
+            return lambda: masked_attn(q, k, v, window=(-1, 0), tensor_layout="NHD")
+        return case
+
+    return {"rotary": rotary, "masked_attn": masked_attn_case(8192), "masked_attn_single": masked_attn_case(1),
+            "lumina_step": lumina_step, "flux_step": flux_step, "rope": rope, "qkv_norm_rope": qkv_norm_rope, "rmsnorm": rmsnorm, "softmax": softmax,
             "gate_residual": gate_residual, "ln_modulate": ln_modulate, "quantize_rows": quantize_rows,
             "codes_to_bf16": codes_to_bf16, "quantize_weight": quantize_weight, "copy_chunks": copy_chunks,
             "sage": sage, "sage_split": sage_split, "gemm_fp8": gemm_fp8, "gemm_bf16_glu": gemm_bf16_glu,
