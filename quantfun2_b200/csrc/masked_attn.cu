@@ -171,8 +171,28 @@ struct Plan {
   int64_t ids_off, rng_off, qrng_off, sorted_off, tab_off, ml_off, o_off, bytes;
 };
 
+// What of the mask the host knows: the window, the first query's position among all keys, and
+// whether scores are capped or biased.
+struct Known {
+  double left, right, off;  // left, right < 0: open
+  bool score;
+};
+
+// key tiles that an item of R consecutive tokens sees: the mean of eight items along the queries
+static double seen_tiles(const Known& m, int64_t Sq, double keys, double R) {
+  double sum = 0.0;
+  for (int i = 0; i < 8; ++i) {
+    const double c = m.off + (i + 0.5) / 8.0 * (double)Sq;
+    const double lo = m.left < 0 ? 0.0 : std::max(0.0, c - 0.5 * R - m.left);
+    const double hi = m.right < 0 ? keys : std::min(keys, c + 0.5 * R + m.right);
+    sum += std::max(0.0, hi - lo) / kBlk + (lo > 0.0 ? 0.5 : 0.0);  // (a band begins inside a tile)
+  }
+  return std::max(1.0, sum / 8.0);
+}
+
+// The workspace is the same whatever `known` says (null: unknown).
 static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P, int64_t D,
-                     bool ids) {
+                     bool ids, const Known* known) {
   if (D != 64 && D != 96 && D != 128 && D != 256) return QF2_ERR_SHAPE;
   if (B < 0 || Sq < 0 || Skv < 0 || P < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return QF2_ERR_SHAPE;
   if (B > 65535 || Hq > 65535 || Sq > (1 << 20)) return QF2_ERR_SHAPE;
@@ -187,24 +207,41 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   p->merged = 1;
   p->G = 1;
   if (B == 0 || Sq == 0) return QF2_OK;
-  // two query tiles per CTA where that still fills the SMs
-  const bool two = D != 256 && Sq > kBlk && B * Hq * ((Sq + 2 * kBlk - 1) / (2 * kBlk)) >= kSms;
   int64_t hw = Hq;
+  // pack a group's query heads where that makes fewer tiles
+  const int64_t tp = group <= kBlk ? std::min<int64_t>(Sq, kBlk / group) : 0;
+  if (group > 1 && tp > 0 && Hkv * ((Sq + tp - 1) / tp) < Hq * ((Sq + kBlk - 1) / kBlk)) {
+    p->G = (int)group;
+    p->T = (int)tp;
+    hw = Hkv;
+  } else {
+    p->T = (int)std::min<int64_t>(Sq, kBlk);
+  }
+  p->qtiles[0] = (int)((Sq + p->T - 1) / p->T);
+  // Two query tiles per CTA, or one in each of two CTAs per SM, where both fill the SMs.  A pair
+  // takes less time over a key tile of both, the small ones start and end under each other and
+  // leave fewer rows and keys out of sight: waves of CTAs * (tiles seen * time of one + start and
+  // end), fitted in us to 138 shapes of 256 to 4096 tokens, 0.3 % off the better of both in the
+  // mean (always pairs: 11 %, never: 5 %).  24 / 8 heads of 128, pair against small: 4 x 4096
+  // tokens 764 and 864, causal windows of 300 on them 200 and 176, 16 x 512 tokens 91 and 82,
+  // 4 x 384 tokens 24.6 and 13.4.
+  const int64_t npair = B * Hq * ((Sq + 2 * kBlk - 1) / (2 * kBlk));
+  const bool full = D != 256 && Sq > kBlk && npair >= kSms;
+  bool two = full;
+  if (full && known) {
+    const double x = (double)D / 128.0, keys = (double)(P + Skv);
+    const double pair = seen_tiles(*known, Sq, keys, 2.0 * kBlk) * (1.4 + 0.4 * x + (known->score ? 0.5 : 0.0)) + 5.0 + 2.0 * x;
+    const double one = seen_tiles(*known, Sq, keys, p->T) * (1.5 + 0.7 * x + (known->score ? 1.0 : 0.0)) + 4.5;
+    two = (double)((npair + kSms - 1) / kSms) * pair <=
+          (double)((B * hw * p->qtiles[0] + 2 * kSms - 1) / (2 * kSms)) * one;
+  }
   if (two) {
     p->form = kPair;
+    p->G = 1;
     p->T = kBlk;
+    hw = Hq;
     p->qtiles[0] = (int)((Sq + 2 * kBlk - 1) / (2 * kBlk));
   } else {
-    // pack a group's query heads where that makes fewer tiles
-    const int64_t tp = group <= kBlk ? std::min<int64_t>(Sq, kBlk / group) : 0;
-    if (group > 1 && tp > 0 && Hkv * ((Sq + tp - 1) / tp) < Hq * ((Sq + kBlk - 1) / kBlk)) {
-      p->G = (int)group;
-      p->T = (int)tp;
-      hw = Hkv;
-    } else {
-      p->T = (int)std::min<int64_t>(Sq, kBlk);
-    }
-    p->qtiles[0] = (int)((Sq + p->T - 1) / p->T);
     // rows of several batch elements share a prefix item where two or more fit a tile
     if (P > 0 && p->T == Sq) {
       const int64_t nb = std::min<int64_t>(B, kBlk / ((int64_t)p->G * p->T));
@@ -228,7 +265,7 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
       // one query tile per batch element, and fewer than fill the SMs: split by the keys each has
       // (lengths are known on the device)
       p->even = (int)cap;
-    } else {
+    } else if (!full) {
       // Split the key tiles so that the waves of CTAs are short: a wave costs its longest CTA
       // (a tile takes its share of the memory's rate, or the softmax of 128 rows; 5 us to start
       // and end); a split also writes and reads fp32 partial rows and launches the merge (4 us).
@@ -314,7 +351,7 @@ using namespace qf2::mattn;
 extern "C" int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv,
                                                    int64_t P, int64_t D, int with_ids) {
   Plan p;
-  const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids != 0);
+  const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids != 0, nullptr);
   return st != QF2_OK ? (int64_t)st : p.bytes;
 }
 
@@ -325,7 +362,10 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   if (dtype != QF2_BF16 && dtype != QF2_F16) return QF2_ERR_DTYPE;
   const bool ids = M.k_ids != nullptr;
   Plan p;
-  int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids);
+  // (positions and lengths on the device: taken for the end of the keys, and all of them)
+  const double first = (double)P + (M.q_offset_mode == QF2_OFFSET_CONST ? (double)M.q_offset : (double)Skv - (double)Sq);
+  const Known known{(double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0};
+  int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids, &known);
   if (st != QF2_OK) return st;
   if (B == 0 || Sq == 0) return QF2_OK;
   if (!M.q || !M.out) return QF2_ERR_ARG;

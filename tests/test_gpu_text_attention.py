@@ -74,7 +74,7 @@ def test_dense_and_causal(cuda, B, Sq, Hq, Hkv, D, dtype, causal):
     assert torch.equal(hnd.transpose(1, 2), out)
 
 
-# grids that fill the SMs: two query tiles per CTA (heads * batch large), spot rows
+# grids that fill the SMs (heads * batch large), spot rows
 @pytest.mark.parametrize("B,S,Hq,Hkv,D,dtype,window", [
     (4, 300, 40, 8, 64, BF16, (-1, 0)), (3, 513, 24, 8, 96, FP16, (-1, -1)), (8, 640, 24, 24, 128, BF16, (100, 0)),
     (4, 1000, 24, 8, 128, BF16, (-1, 0)), (2, 1281, 24, 8, 128, FP16, (130, 40)), (13, 257, 12, 12, 64, FP16, (0, 0)),
@@ -86,6 +86,107 @@ def test_two_tile_grids(cuda, B, S, Hq, Hkv, D, dtype, window):
     out = A.masked_attn(q, k, v, window=window, tensor_layout="NHD")
     rows = sorted({0, 1, 31, 127, 128, 129, 255, 256, S // 2, S - 2, S - 1})
     _compare(out, q, k, v, rows=rows, window=window)
+
+
+# Long key ranges and grids that fill the SMs: two query tiles in one CTA (short ranges, as in the
+# tests above, are taken by CTAs of one tile).
+PAIR_ROWS = [0, 1, 31, 127, 128, 129, 255, 256]
+
+
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hkv,D,dtype,window", [
+    (4, 390, 2600, 24, 8, 64, BF16, (-1, 0)), (4, 511, 2561, 24, 24, 96, FP16, (-1, -1)), (4, 512, 2688, 24, 8, 128, BF16, (1700, 0)),
+    (1, 2305, 2305, 18, 6, 128, FP16, (-1, -1)), (8, 450, 5000, 24, 8, 128, BF16, (-1, 300)), (2, 600, 3001, 48, 1, 96, BF16, (2200, 40)),
+])
+def test_pairs_of_query_tiles(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, window):
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, seed=Sq)
+    buf = torch.full((B, Sq + 3, Hq + 1, D), 3.0, device=cuda, dtype=dtype)
+    out = A.masked_attn(q, k, v, window=window, tensor_layout="NHD", out=buf[:, 1:Sq + 1, 1:])
+    rows = sorted({*PAIR_ROWS, Sq // 2, Sq - 2, Sq - 1})
+    _compare(out, q, k, v, rows=rows, window=window)
+    assert torch.equal(out, A.masked_attn(q, k, v, window=window, tensor_layout="NHD"))
+    buf[:, 1:Sq + 1, 1:] = 3.0
+    assert (buf == 3.0).all()                              # nothing beside the view was written
+
+
+@pytest.mark.parametrize("D,dtype", [(64, FP16), (96, BF16), (128, BF16)])
+def test_pairs_with_capped_and_biased_scores(cuda, D, dtype):
+    from quantfun2_b200 import attention as A
+
+    B, Sq, Skv, Hq = 3, 500, 2500, 32
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hq // 2, D, dtype, seed=6, amp=4.0)
+    slopes = torch.rand(Hq, device=cuda) * 0.2
+    rows = [0, 127, 128, 300, 499]
+    calls = [dict(bias_table=torch.randn(Hq, 2 * R + 1, device=cuda)) for R in (0, 40, 1024)]
+    calls += [dict(softcap=2.0, window=(-1, 0)), dict(softcap=50.0), dict(slopes=slopes), dict(slopes=slopes, window=(-1, 0)),
+              dict(softcap=50.0, slopes=slopes, window=(2100, 20), sm_scale=0.3)]
+    for kw in calls:
+        out = A.masked_attn(q, k, v, tensor_layout="NHD", **kw)
+        _compare(out, q, k, v, rows=rows, **kw)
+
+
+def test_pairs_with_prefixes_lengths_and_documents(cuda):
+    from quantfun2_b200 import attention as A
+
+    B, S, Hq, Hkv, D = 5, 500, 24, 8, 96
+    Skv = 2500
+    q, k, v = _inputs(cuda, B, S, Skv, Hq, Hkv, D, BF16, seed=7)
+    pre = torch.tensor([0, 1, 128, 1500, 9999], device=cuda)
+    lens = torch.tensor([2500, 0, 1, 129, 5000], device=cuda, dtype=torch.int32)
+    off = torch.tensor([2000, 0, -600, 50, 1], device=cuda, dtype=torch.int32)
+    rows = [0, 127, 128, 255, 256, 499]
+    out = A.masked_attn(q, k, v, window=(-1, 0), prefix_lens=pre, tensor_layout="NHD")
+    _compare(out, q, k, v, rows=rows, window=(-1, 0), prefix_lens=pre.tolist())
+    out = A.masked_attn(q, k, v, window=(1800, 0), prefix_lens=pre, kv_lens=lens, q_offset=off, tensor_layout="NHD")
+    _compare(out, q, k, v, rows=rows, window=(1800, 0), prefix_lens=pre.tolist(), kv_lens=lens.tolist(), offsets=off.tolist())
+    out = A.masked_attn(q, k, v, window=(-1, 0), kv_lens=lens, q_offset="end", tensor_layout="NHD")
+    _compare(out, q, k, v, rows=rows, window=(-1, 0), kv_lens=lens.tolist(), offsets=[min(n, Skv) - S for n in lens.tolist()])
+    ids = torch.zeros(B, Skv, dtype=torch.int64, device=cuda)
+    for cut in (1, 40, 128, 256, 300, 511, 2100, 2256, 2300):
+        ids[0, cut:] += 1                                    # packed texts
+    ids[1, 2200:] = -1                                       # padded tail
+    ids[2] = torch.randint(-1, 3, (Skv,), device=cuda)       # any order
+    ids[3] = -1                                              # nothing but padding
+    for window in ((-1, -1), (-1, 0)):
+        out = A.masked_attn(q, k, v, window=window, segment_ids=(ids[:, -S:], ids), tensor_layout="NHD")
+        _compare(out, q, k, v, rows=[*rows, 99, 100, 199, 200], window=window, q_ids=ids[:, -S:], k_ids=ids)
+        assert not out[3].any() and not out[1, 200:].any()
+
+
+def test_pairs_and_hidden_garbage(cuda):
+    from quantfun2_b200 import attention as A
+
+    B, S, Skv, H, D = 4, 500, 2600, 24, 128
+    q, k, v = _inputs(cuda, B, S, Skv, H, H // 2, D, BF16, seed=17)
+    lens = torch.tensor([2600, 2222, 700, 0], device=cuda)
+    ids = torch.zeros(B, Skv, dtype=torch.int32, device=cuda)
+    ids[0, :70], ids[1, 500:], ids[2] = -1, -1, -1
+    qid = torch.zeros(B, S, dtype=torch.int32, device=cuda)
+    left = 1500
+    j = torch.arange(Skv, device=cuda)[None]
+    for kw, bad in ((dict(kv_lens=lens), j >= lens[:, None]), (dict(segment_ids=(qid, ids)), ids < 0),
+                    (dict(window=(left, 0)), (j < Skv - S - left).expand(B, Skv))):
+        outs = []
+        for fill_k, fill_v in ((0.0, 0.0), (math.nan, math.nan), (math.inf, -math.inf)):
+            kk = torch.where(bad[:, :, None, None], fill_k, k.float()).to(BF16)
+            vv = torch.where(bad[:, :, None, None], fill_v, v.float()).to(BF16)
+            outs.append(A.masked_attn(q, kk, vv, tensor_layout="NHD", **kw))
+        assert torch.isfinite(outs[0]).all() and outs[0].any()
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (128, FP16)])
+def test_pairs_behind_a_shared_prefix(cuda, D, dtype):
+    from quantfun2_b200 import attention as A
+
+    B, S, P, Hq, Hkv = 5, 500, 2100, 24, 8
+    q, k, v, pk, pv = _inputs(cuda, B, S, S + 9, Hq, Hkv, D, dtype, seed=P, P=P)
+    lens = torch.tensor([0, 1, 300, 509, 600], device=cuda)
+    rows = [0, 127, 128, 256, 499]
+    for kw in (dict(), dict(softcap=30.0), dict(slopes=torch.rand(Hq, device=cuda) * 0.02)):
+        out = A.shared_prefix_attn(q, pk, pv, k, v, window=(-1, 0), kv_lens=lens, q_offset=9, tensor_layout="NHD", **kw)
+        _compare(out, q, k, v, rows=rows, window=(-1, 0), kv_lens=lens.tolist(), offsets=[9] * B, prefix_k=pk, prefix_v=pv, **kw)
 
 
 @pytest.mark.parametrize("Hq,two", [(2, False), (80, True)])
