@@ -83,49 +83,133 @@ __global__ void __launch_bounds__(1024) mattn_ids_kernel(const int32_t* __restri
 // D / 4 threads cover the row in 16-byte pieces, 128 / (D / 4) such groups take every
 // second, fifth, ... split, and the groups are added in a fixed order.  A row's splits are up
 // to two runs of partial rows: the own items' and the prefix items'.
+struct Row {
+  int b, tok, h, n0, n1;
+  int64_t row0, row1, step0, step1;
+  QF2_DEV int64_t part(int s) const { return s < n0 ? row0 + s * step0 : row1 + (s - n0) * step1; }
+};
+
+// the partial rows of output row r, after the attention kernel's end
+QF2_DEV Row row_of(const Args& A, int r) {
+  Row R;
+  const int bt = div_of(A.by_Hq, r);
+  R.h = r - bt * A.Hq;
+  R.b = div_of(A.by_Sq, bt);
+  R.tok = bt - R.b * A.Sq;
+  const int Hw = A.Hw, hw = div_of(A.by_G, R.h), g = R.h - hw * A.G, T = A.T;
+  const int qt = div_of(A.by_T, R.tok), tr = R.tok - qt * T;
+  grid_wait();
+  // own run: n0 partial rows, step0 apart, from row0
+  R.step0 = (int64_t)A.G * T * A.Nb[0];
+  R.step1 = (int64_t)A.G * T * A.Nb[1];
+  R.row1 = 0;
+  R.n1 = 0;
+  if (A.even > 0) {
+    const int2 e = A.part_tab[R.b * Hw + hw];
+    R.row0 = e.x * R.step0;
+    R.n0 = e.y;
+  } else {
+    R.n0 = A.splits[0];
+    R.row0 = (((int64_t)(A.qtiles[0] - 1 - qt) * A.heads[0] + R.b * Hw + hw) * R.n0) * R.step0;
+  }
+  R.row0 += tr * A.G + g;
+  if (A.items1 > 0) {
+    const int nb = A.Nb[1], e = R.b / nb, q1 = e * A.qtiles[0] + qt;
+    R.n1 = A.splits[1];
+    R.row1 = A.part_off1 + (((int64_t)(A.qtiles[1] - 1 - q1) * A.heads[1] + hw) * R.n1) * R.step1 +
+             ((R.b - e * nb) * T + tr) * A.G + g;
+  }
+  return R;
+}
+
+QF2_DEV float part_weight(float2 ml, float M) {
+  // a NaN sum (its maximum may be -inf: NaN scores leave it) goes on to the output
+  return ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
+}
+
+template <bool F16>
+QF2_DEV void store_row4(const Args& A, const Row& R, int c, float4 a, float l) {
+  const bool zero = l == 0.f;
+  const float inv = zero ? 0.f : 1.0f / l;
+  uint2 w;
+  w.x = zero ? 0u : pack16<F16>(a.x * inv, a.y * inv);
+  w.y = zero ? 0u : pack16<F16>(a.z * inv, a.w * inv);
+  *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(A.out) +
+                            2 * (R.b * A.os.b + (int64_t)R.h * A.os.h + R.tok * A.os.s + 4 * c)) = w;
+}
+
+// Many rows: one warp per row, 16-byte pieces of a lane (two splits at once where half a warp
+// covers the row).  A block a row takes 12 us for 7392 rows of two splits, 64 channels.
+template <int D, bool F16>
+__global__ void __launch_bounds__(256) mattn_merge_rows_kernel(const __grid_constant__ Args A, int rows) {
+  constexpr int C = D / 4, LC = C < 32 ? C : 32, NV = C / LC, NG = 32 / LC;
+  const int r = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (r >= rows) return;
+  const Row R = row_of(A, r);
+  const int ns = R.n0 + R.n1;
+  if (ns == 1) return;  // the attention kernel wrote the row
+  float M = -INFINITY;
+  for (int i = lane; i < ns; i += 32) M = fmaxf(M, A.part_ml[R.part(i)].x);
+  for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
+  const int grp = lane / LC, c = lane - grp * LC;
+  const bool on = grp < NG;
+  float l = 0.f;
+  float4 a[NV];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) a[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < ns; s0 += 32) {
+    float w = 0.f;
+    if (s0 + lane < ns) {
+      const float2 ml = A.part_ml[R.part(s0 + lane)];
+      w = part_weight(ml, M);
+      l += w * ml.y;
+    }
+    const int m = min(32, ns - s0);
+#pragma unroll 4
+    for (int i = 0; i < m; i += NG) {
+      const int s = min(i + min(grp, NG - 1), m - 1);  // (past the last split: again, not counted)
+      const float ws = __shfl_sync(0xffffffffu, w, s);
+      const bool counts = on && i + grp < m && ws != 0.f;  // a split that saw nothing was not written
+      const float* o = A.part_o + R.part(s0 + s) * D;
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        const float4 x = *reinterpret_cast<const float4*>(o + 4 * (v * LC + c));
+        if (counts) {
+          a[v].x = fmaf(ws, x.x, a[v].x); a[v].y = fmaf(ws, x.y, a[v].y);
+          a[v].z = fmaf(ws, x.z, a[v].z); a[v].w = fmaf(ws, x.w, a[v].w);
+        }
+      }
+    }
+  }
+  for (int d = 16; d; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    if (NG == 2) {
+      a[v].x += __shfl_xor_sync(0xffffffffu, a[v].x, 16); a[v].y += __shfl_xor_sync(0xffffffffu, a[v].y, 16);
+      a[v].z += __shfl_xor_sync(0xffffffffu, a[v].z, 16); a[v].w += __shfl_xor_sync(0xffffffffu, a[v].w, 16);
+    }
+    if (grp == 0) store_row4<F16>(A, R, v * LC + c, a[v], l);
+  }
+}
+
 template <int D, bool F16>
 __global__ void __launch_bounds__(128) mattn_merge_kernel(const __grid_constant__ Args A) {
   constexpr int C = D / 4, NG = 128 / C;
   __shared__ float wgt[2 * kMaxSplits];
   __shared__ float4 acc[NG][C];
   const int tid = threadIdx.x;
-  const int bt = div_of(A.by_Hq, blockIdx.x), h = blockIdx.x - bt * A.Hq;
-  const int b = div_of(A.by_Sq, bt), tok = bt - b * A.Sq;
-  const int Hw = A.Hw, hw = div_of(A.by_G, h), g = h - hw * A.G, T = A.T;
-  const int qt = div_of(A.by_T, tok), tr = tok - qt * T;
-  grid_wait();
-  // own run: n0 partial rows, step0 apart, from row0
-  const int64_t step0 = (int64_t)A.G * T * A.Nb[0], step1 = (int64_t)A.G * T * A.Nb[1];
-  int64_t row0, row1 = 0;
-  int n0, n1 = 0;
-  if (A.even > 0) {
-    const int2 e = A.part_tab[b * Hw + hw];
-    row0 = e.x * step0;
-    n0 = e.y;
-  } else {
-    n0 = A.splits[0];
-    row0 = (((int64_t)(A.qtiles[0] - 1 - qt) * A.heads[0] + b * Hw + hw) * n0) * step0;
-  }
-  row0 += tr * A.G + g;
-  if (A.items1 > 0) {
-    const int nb = A.Nb[1], e = b / nb, q1 = e * A.qtiles[0] + qt;
-    n1 = A.splits[1];
-    row1 = A.part_off1 + (((int64_t)(A.qtiles[1] - 1 - q1) * A.heads[1] + hw) * n1) * step1 +
-           ((b - e * nb) * T + tr) * A.G + g;
-  }
-  const int ns = n0 + n1;
+  const Row R = row_of(A, blockIdx.x);
+  const int ns = R.n0 + R.n1;
   if (ns == 1) return;  // the attention kernel wrote the row
-  auto part = [&](int s) -> int64_t { return s < n0 ? row0 + s * step0 : row1 + (s - n0) * step1; };
   // every warp finds the maximum and the weights by itself (one round of loads, no exchange)
   const int lane = tid & 31;
   float M = -INFINITY;
-  for (int i = lane; i < ns; i += 32) M = fmaxf(M, A.part_ml[part(i)].x);
+  for (int i = lane; i < ns; i += 32) M = fmaxf(M, A.part_ml[R.part(i)].x);
   for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
   float l = 0.f;
   for (int i = lane; i < ns; i += 32) {
-    const float2 ml = A.part_ml[part(i)];
-    // a NaN sum (its maximum may be -inf: NaN scores leave it) goes on to the output
-    const float w = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - M);
+    const float2 ml = A.part_ml[R.part(i)];
+    const float w = part_weight(ml, M);
     wgt[i] = w;  // the same from every warp
     l += w * ml.y;
   }
@@ -139,7 +223,7 @@ __global__ void __launch_bounds__(128) mattn_merge_kernel(const __grid_constant_
       // (loaded whatever its weight, so that the loads do not wait for one another; the row of a
       // split that saw nothing was not written)
       const float w = wgt[s];
-      const float4 o = *reinterpret_cast<const float4*>(A.part_o + part(s) * D + 4 * c);
+      const float4 o = *reinterpret_cast<const float4*>(A.part_o + R.part(s) * D + 4 * c);
       if (w != 0.f) {
         a.x = fmaf(w, o.x, a.x); a.y = fmaf(w, o.y, a.y); a.z = fmaf(w, o.z, a.z); a.w = fmaf(w, o.w, a.w);
       }
@@ -152,13 +236,7 @@ __global__ void __launch_bounds__(128) mattn_merge_kernel(const __grid_constant_
       const float4 o = acc[k][tid];
       a.x += o.x; a.y += o.y; a.z += o.z; a.w += o.w;
     }
-    const bool zero = l == 0.f;
-    const float inv = zero ? 0.f : 1.0f / l;
-    uint2 w;
-    w.x = zero ? 0u : pack16<F16>(a.x * inv, a.y * inv);
-    w.y = zero ? 0u : pack16<F16>(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2*>(reinterpret_cast<uint8_t*>(A.out) +
-                              2 * (b * A.os.b + (int64_t)h * A.os.h + tok * A.os.s + 4 * tid)) = w;
+    store_row4<F16>(A, R, tid, a, l);
   }
 }
 
@@ -171,11 +249,11 @@ struct Plan {
   int64_t ids_off, rng_off, qrng_off, sorted_off, tab_off, ml_off, o_off, bytes;
 };
 
-// What of the mask the host knows: the window, the first query's position among all keys, and
-// whether scores are capped or biased.
+// What of the mask the host knows: the window, the first query's position among all keys, whether
+// scores are capped or biased, and whether batch elements may see unlike numbers of keys.
 struct Known {
   double left, right, off;  // left, right < 0: open
-  bool score;
+  bool score, ragged;
 };
 
 // key tiles that an item of R consecutive tokens sees: the mean of eight items along the queries
@@ -190,9 +268,8 @@ static double seen_tiles(const Known& m, int64_t Sq, double keys, double R) {
   return std::max(1.0, sum / 8.0);
 }
 
-// The workspace is the same whatever `known` says (null: unknown).
 static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P, int64_t D,
-                     bool ids, const Known* known) {
+                     bool ids, const Known& known) {
   if (D != 64 && D != 96 && D != 128 && D != 256) return QF2_ERR_SHAPE;
   if (B < 0 || Sq < 0 || Skv < 0 || P < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return QF2_ERR_SHAPE;
   if (B > 65535 || Hq > 65535 || Sq > (1 << 20)) return QF2_ERR_SHAPE;
@@ -228,10 +305,11 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   const int64_t npair = B * Hq * ((Sq + 2 * kBlk - 1) / (2 * kBlk));
   const bool full = D != 256 && Sq > kBlk && npair >= kSms;
   bool two = full;
-  if (full && known) {
-    const double x = (double)D / 128.0, keys = (double)(P + Skv);
-    const double pair = seen_tiles(*known, Sq, keys, 2.0 * kBlk) * (1.4 + 0.4 * x + (known->score ? 0.5 : 0.0)) + 5.0 + 2.0 * x;
-    const double one = seen_tiles(*known, Sq, keys, p->T) * (1.5 + 0.7 * x + (known->score ? 1.0 : 0.0)) + 4.5;
+  const double x = (double)D / 128.0;
+  if (full) {
+    const double keys = (double)(P + Skv);
+    const double pair = seen_tiles(known, Sq, keys, 2.0 * kBlk) * (1.4 + 0.4 * x + (known.score ? 0.5 : 0.0)) + 5.0 + 2.0 * x;
+    const double one = seen_tiles(known, Sq, keys, p->T) * (1.5 + 0.7 * x + (known.score ? 1.0 : 0.0)) + 4.5;
     two = (double)((npair + kSms - 1) / kSms) * pair <=
           (double)((B * hw * p->qtiles[0] + 2 * kSms - 1) / (2 * kSms)) * one;
   }
@@ -254,39 +332,46 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   }
   const int64_t n0 = B * hw * p->qtiles[0], n1 = hw * p->qtiles[1];
   const int64_t t0 = (p->merged ? ntp : 0) + nto, t1 = p->merged ? 0 : ntp;
-  if (!two) {
-    // many keys for few items: one CTA per SM streams them; else two, of half the size
-    const bool deep = D == 256 || (n1 == 0 && p->qtiles[0] == 1 && n0 * t0 >= 6 * kSms && t0 >= 16);
-    p->form = deep ? kDeep : kSmall;
-    const int64_t cap = deep ? kSms : 2 * kSms;  // CTAs at work at once
-    // prefix items: as many splits as fill the SMs, of four tiles or more
-    if (n1 > 0) p->splits[1] = (int)std::max<int64_t>(1, std::min((t1 + 3) / 4, std::min<int64_t>(cap / n1, kMaxSplits)));
-    if (p->qtiles[0] == 1 && B <= kMaxEven && t0 > 2 && n0 < cap) {
-      // one query tile per batch element, and fewer than fill the SMs: split by the keys each has
-      // (lengths are known on the device)
-      p->even = (int)cap;
-    } else if (!full) {
-      // Split the key tiles so that the waves of CTAs are short: a wave costs its longest CTA
-      // (a tile takes its share of the memory's rate, or the softmax of 128 rows; 5 us to start
-      // and end); a split also writes and reads fp32 partial rows and launches the merge (4 us).
-      const bool few = (int64_t)p->G * p->T <= 32;
-      const double mem_us = 1.5 * (double)D / 128.0 * (double)cap / kSms;
-      const double tile_us = few ? mem_us : std::max(mem_us, D == 256 ? 2.5 : 1.3 + 0.9 * (double)D / 128.0);
-      const double row_us = (double)(B * Sq * Hq) * (double)D * 8.0 / 5.0e6;
-      double best = 1e30;
-      for (int64_t n = 1; n <= kSms; ++n) {
+  if (full && !two) p->form = kSmall;
+  if (!full) {
+    // Too few rows to fill the SMs with pairs.  Two forms and any number of splits of the key
+    // tiles: a wave of CTAs costs its longest one (a tile takes its latency, or its CTA's share of
+    // the memory's rate; 5 us to start and end); a split also writes and reads fp32 partial rows
+    // and launches the merge.  kDeep, one CTA per SM, takes less time over a tile than kSmall, two
+    // per SM (1.2 against 1.9 us for 128 rows, 0.9 against 1.2 us for the four copies of up to 32),
+    // and kSmall takes twice the items in a wave: 500 tokens of 24 / 8 heads of 128 9.9 us in kDeep
+    // and 13.7 us in kSmall, 64 single tokens on 4096 keys 176 and 162 us.
+    const bool few = (int64_t)p->G * p->T <= 32;
+    const double rows = (double)B * (double)Sq * (double)Hq;
+    double best = 1e30, walk = 0.0;
+    for (int form = D == 256 || n1 == 0 ? kDeep : kSmall; form >= (D == 256 ? kDeep : kSmall); --form) {
+      const int64_t cap = form == kDeep ? kSms : 2 * kSms;  // CTAs at work at once
+      double lat = form == kDeep ? (D == 256 ? 2.5 : few ? 0.5 + 0.4 * x : 1.1 + 0.1 * x)
+                                 : few ? 0.85 + 0.35 * x : 1.3 + 0.9 * x;
+      if (known.score) lat += form == kDeep ? 0.5 : 1.0;
+      for (int64_t n = 1; n <= std::min<int64_t>(std::max<int64_t>(t0, 1), kSms); n += 1 + n / 8) {
         const int64_t len = std::max<int64_t>(1, (t0 + n - 1) / n);
         const int64_t s0 = std::max<int64_t>(1, (t0 + len - 1) / len);
-        if (s0 > kMaxSplits) break;
         const int64_t ctas = n0 * s0;
-        double c = (double)((ctas + cap - 1) / cap) * ((double)len * tile_us + 5.0);
-        if (s0 > 1) c += 4.0 + row_us * (double)s0;
+        const double walk0 = (double)len * std::max(lat, 1.5 * x * (double)std::min(ctas, cap) / kSms);
+        double c = (double)((ctas + cap - 1) / cap) * (walk0 + 5.0);
+        if (s0 > 1) c += 2.5 + rows / 2000.0 + rows * (double)s0 * (double)D * 8.0 / 5.0e6;
         if (c < best) {
           best = c;
+          walk = walk0;
+          p->form = form;
           p->splits[0] = (int)s0;
         }
-        if (len == 1) break;
       }
+    }
+    const int64_t cap = p->form == kDeep ? kSms : 2 * kSms;
+    // prefix items: as many splits as fill the SMs, of four tiles or more
+    if (n1 > 0) p->splits[1] = (int)std::max<int64_t>(1, std::min((t1 + 3) / 4, std::min<int64_t>(cap / n1, kMaxSplits)));
+    // One query tile per batch element, on unlike lengths that the device knows: split by the keys
+    // each has.  That costs 1.2 us before the first load, and gains where the splits are long.
+    if (known.ragged && p->qtiles[0] == 1 && B <= kMaxEven && t0 > 2 && 2 * n0 <= cap && walk > 6.0) {
+      p->even = (int)cap;
+      p->splits[0] = 1;
     }
   }
   p->items[0] = p->even > 0 ? p->even : n0 * p->splits[0];
@@ -340,6 +425,12 @@ static cudaError_t launch_merge(const Args& a, int64_t D, int64_t rows, cudaStre
   auto kern = D == 64 ? mattn_merge_kernel<64, F16>
                       : D == 96 ? mattn_merge_kernel<96, F16>
                                 : D == 128 ? mattn_merge_kernel<128, F16> : mattn_merge_kernel<256, F16>;
+  if (rows >= 16 * kSms) {
+    auto many = D == 64 ? mattn_merge_rows_kernel<64, F16>
+                        : D == 96 ? mattn_merge_rows_kernel<96, F16>
+                                  : D == 128 ? mattn_merge_rows_kernel<128, F16> : mattn_merge_rows_kernel<256, F16>;
+    return launch_after(many, dim3((unsigned)((rows + 7) / 8)), 256, 0, s, true, a, (int)rows);
+  }
   return launch_after(kern, dim3((unsigned)rows), 128, 0, s, true, a);
 }
 
@@ -350,9 +441,15 @@ using namespace qf2::mattn;
 
 extern "C" int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv,
                                                    int64_t P, int64_t D, int with_ids) {
-  Plan p;
-  const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids != 0, nullptr);
-  return st != QF2_OK ? (int64_t)st : p.bytes;
+  // the most that any mask's plan takes (with pairs or without them no rows are split)
+  int64_t bytes = 0;
+  for (int i = 0; i < 4; ++i) {
+    Plan p;
+    const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids != 0, Known{-1.0, -1.0, 0.0, (i & 1) != 0, (i & 2) != 0});
+    if (st != QF2_OK) return st;
+    bytes = std::max(bytes, p.bytes);
+  }
+  return bytes;
 }
 
 extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
@@ -364,8 +461,9 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   Plan p;
   // (positions and lengths on the device: taken for the end of the keys, and all of them)
   const double first = (double)P + (M.q_offset_mode == QF2_OFFSET_CONST ? (double)M.q_offset : (double)Skv - (double)Sq);
-  const Known known{(double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0};
-  int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids, &known);
+  const Known known{(double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0,
+                    M.kv_lens || M.prefix_lens || M.q_offset_mode == QF2_OFFSET_ARRAY};
+  int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids, known);
   if (st != QF2_OK) return st;
   if (B == 0 || Sq == 0) return QF2_OK;
   if (!M.q || !M.out) return QF2_ERR_ARG;
