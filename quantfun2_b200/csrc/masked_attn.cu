@@ -253,7 +253,7 @@ struct Plan {
 // scores are capped or biased, and whether batch elements may see unlike numbers of keys.
 struct Known {
   double left, right, off;  // left, right < 0: open
-  bool score, ragged;
+  bool score, ragged, table;
 };
 
 // key tiles that an item of R consecutive tokens sees: the mean of eight items along the queries
@@ -285,9 +285,12 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   p->G = 1;
   if (B == 0 || Sq == 0) return QF2_OK;
   int64_t hw = Hq;
-  // pack a group's query heads where that makes fewer tiles
+  // Pack a group's query heads where that makes fewer tiles.  With a distance table only single
+  // tokens and up to 16 rows: a head's rows read it from shared memory, a group's from global
+  // memory.  24 / 8 heads of 128, packed against not: 300 tokens, reach 512, 33 and 12 us; 4 x 5
+  // tokens on 2000 keys 20 and 25; 16 single tokens on 1000 keys 26 and 41.
   const int64_t tp = group <= kBlk ? std::min<int64_t>(Sq, kBlk / group) : 0;
-  if (group > 1 && tp > 0 && Hkv * ((Sq + tp - 1) / tp) < Hq * ((Sq + kBlk - 1) / kBlk)) {
+  if ((!known.table || Sq == 1 || group * Sq <= 16) && group > 1 && tp > 0 && Hkv * ((Sq + tp - 1) / tp) < Hq * ((Sq + kBlk - 1) / kBlk)) {
     p->G = (int)group;
     p->T = (int)tp;
     hw = Hkv;
@@ -443,9 +446,9 @@ extern "C" int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_
                                                    int64_t P, int64_t D, int with_ids) {
   // the most that any mask's plan takes (with pairs or without them no rows are split)
   int64_t bytes = 0;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 8; ++i) {
     Plan p;
-    const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids != 0, Known{-1.0, -1.0, 0.0, (i & 1) != 0, (i & 2) != 0});
+    const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids != 0, Known{-1.0, -1.0, 0.0, (i & 1) != 0, (i & 2) != 0, (i & 4) != 0});
     if (st != QF2_OK) return st;
     bytes = std::max(bytes, p.bytes);
   }
@@ -462,7 +465,7 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   // (positions and lengths on the device: taken for the end of the keys, and all of them)
   const double first = (double)P + (M.q_offset_mode == QF2_OFFSET_CONST ? (double)M.q_offset : (double)Skv - (double)Sq);
   const Known known{(double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0,
-                    M.kv_lens || M.prefix_lens || M.q_offset_mode == QF2_OFFSET_ARRAY};
+                    M.kv_lens || M.prefix_lens || M.q_offset_mode == QF2_OFFSET_ARRAY, M.bias_table != nullptr};
   int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids, known);
   if (st != QF2_OK) return st;
   if (B == 0 || Sq == 0) return QF2_OK;

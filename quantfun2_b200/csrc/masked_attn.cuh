@@ -786,7 +786,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       // went back to.  Prompts of 64 x 512 keys take 33 us in registers and 27 us in two short
       // loops; kPair the other way 1385 us in registers, 1438 us in loops (causal 16384 tokens).
       constexpr bool kHeld = KW == 32 || FORM != kSmall;
-      const bool far = SCORE && tab_smem && (p0 - q_hi >= A.reach || p0 + KW - 1 - q_lo <= -A.reach);
+      const bool far = SCORE && A.table != nullptr && (p0 - q_hi >= A.reach || p0 + KW - 1 - q_lo <= -A.reach);
       const int e_hi = min(hi, pend) - p0, e_lo = lo - p0, e_pre = min(pre, pend) - p0, e_plo = plo - p0;
       float mx = -INFINITY;
       // N scores, the first of key c of this thread's
@@ -838,21 +838,20 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
 #pragma unroll
               for (int i = 0; i < N; ++i) x[i] = fmaf(-slope2, fabsf(d0 - (float)i), x[i] * sx);
             }
-          } else if (tab_smem) {
-            if (far) {  // all distances of the warp beyond the table's reach
-              const float bv = tab[p0 - q_hi >= A.reach ? 2 * A.reach + kTabPad : kTabPad];
-              const float2 bb = make_float2(bv, bv);
+          } else if (far) {  // all distances of the warp beyond the table's reach
+            const int end = p0 - q_hi >= A.reach ? 2 * A.reach : 0;
+            const float bv = tab_smem ? tab[end + kTabPad] : bias_log2(__ldg(trow + end));
+            const float2 bb = make_float2(bv, bv);
 #pragma unroll
-              for (int i = 0; i < N / 2; ++i) {
-                const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), sx2, bb);
-                x[2 * i] = y.x;
-                x[2 * i + 1] = y.y;
-              }
-            } else {
-              const float* tp = tab + (q0 - qpos + A.reach + kTabPad);
-#pragma unroll
-              for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], sx, tp[i]);
+            for (int i = 0; i < N / 2; ++i) {
+              const float2 y = ffma2(make_float2(x[2 * i], x[2 * i + 1]), sx2, bb);
+              x[2 * i] = y.x;
+              x[2 * i + 1] = y.y;
             }
+          } else if (tab_smem) {
+            const float* tp = tab + (q0 - qpos + A.reach + kTabPad);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[i] = fmaf(x[i], sx, tp[i]);
           } else if (trow) {
             const int d0 = q0 - qpos, R = A.reach;
 #pragma unroll

@@ -592,3 +592,45 @@ def test_refusals(cuda):
     with torch.no_grad():                                    # a parameter's values are fine where no gradient is wanted
         A.masked_attn(q.clone().requires_grad_(), k, v, **nhd)
     A.masked_attn_status()
+
+
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hkv,D,dtype", [
+    (2, 1, 1500, 24, 8, 64, BF16), (3, 5, 700, 6, 2, 128, FP16), (2, 6, 700, 6, 2, 128, BF16), (1, 300, 300, 6, 2, 96, BF16),
+    (2, 100, 900, 16, 1, 256, BF16), (4, 1, 2000, 40, 1, 128, FP16),
+])
+def test_distance_table_of_grouped_heads(cuda, B, Sq, Skv, Hq, Hkv, D, dtype):
+    """Tables within and beyond their reach, their last entries minus infinity or unlike each
+    other, for heads that share keys."""
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, seed=Sq + Skv)
+    rows = sorted({0, Sq // 2, Sq - 1})
+    g = torch.Generator(device=cuda).manual_seed(3)
+    for R in (0, 3, 150, 1024):
+        table = torch.randn(Hq, 2 * R + 1, device=cuda, generator=g)
+        table[:, 0] += 2.0
+        table[:, -1] -= 2.0
+        for window in ((-1, 0), (-1, -1)):
+            out = A.masked_attn(q, k, v, window=window, bias_table=table, tensor_layout="NHD")
+            _compare(out, q, k, v, rows=rows, window=window, bias_table=table)
+    table = torch.randn(Hq, 9, device=cuda, generator=g)
+    table[:, 0] = -math.inf                                  # keys 4 and more before the query are hidden
+    out = A.masked_attn(q, k, v, window=(-1, 0), bias_table=table, tensor_layout="NHD")
+    _compare(out, q, k, v, rows=rows, window=(3, 0), bias_table=torch.where(table.isinf(), 0.0, table))
+
+
+@pytest.mark.parametrize("D,dtype", [(64, BF16), (96, FP16), (128, BF16), (256, FP16)])
+def test_many_rows_of_split_keys(cuda, D, dtype):
+    """More rows than are merged by a block each; elements without keys, splits without keys."""
+    from quantfun2_b200 import attention as A
+
+    B, Sq, Skv, H = 2, 128, 6000, 12
+    q, k, v = _inputs(cuda, B, Sq, Skv, H, H, D, dtype, seed=D)
+    for lens in ([6000, 6000], [6000, 0], [200, 5000]):
+        lens = torch.tensor(lens, device=cuda)
+        out = A.masked_attn(q, k, v, window=(-1, 0), kv_lens=lens, q_offset="end", tensor_layout="NHD")
+        _compare(out, q, k, v, rows=[0, 1, 64, 127], window=(-1, 0), kv_lens=lens.tolist(),
+                 offsets=[n - Sq for n in lens.tolist()])
+    out = A.masked_attn(q, k, v, tensor_layout="NHD")
+    _compare(out, q, k, v, rows=[0, 127])
+    assert torch.equal(out, A.masked_attn(q, k, v, tensor_layout="NHD"))
