@@ -334,7 +334,12 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
     }
   }
   const int64_t n0 = B * hw * p->qtiles[0], n1 = hw * p->qtiles[1];
-  const int64_t t0 = (p->merged ? ntp : 0) + nto, t1 = p->merged ? 0 : ntp;
+  int64_t t0 = (p->merged ? ntp : 0) + nto;  // key tiles of an own item, or of its window
+  const int64_t t1 = p->merged ? 0 : ntp;
+  if (known.left >= 0.0 && known.right >= 0.0 && P == 0) {
+    const double band = ((double)p->T + known.left + known.right + kBlk - 1) / kBlk + 1.0;
+    if (band < (double)t0) t0 = std::max<int64_t>(1, (int64_t)band);
+  }
   if (full && !two) p->form = kSmall;
   if (!full) {
     // Too few rows to fill the SMs with pairs.  Two forms and any number of splits of the key
@@ -464,10 +469,19 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   Plan p;
   // (positions and lengths on the device: taken for the end of the keys, and all of them)
   const double first = (double)P + (M.q_offset_mode == QF2_OFFSET_CONST ? (double)M.q_offset : (double)Skv - (double)Sq);
-  const Known known{(double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0,
+  const Known known{M.prefix_lens ? -1.0 : (double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0,
                     M.kv_lens || M.prefix_lens || M.q_offset_mode == QF2_OFFSET_ARRAY, M.bias_table != nullptr};
   int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids, known);
   if (st != QF2_OK) return st;
+  if (known.left >= 0.0 && known.right >= 0.0) {
+    // the workspace is sized without a window: a plan that would take more gives way to that one's
+    Known open = known;
+    open.left = open.right = -1.0;
+    Plan o;
+    st = make_plan(&o, B, Hq, Hkv, Sq, Skv, P, D, ids, open);
+    if (st != QF2_OK) return st;
+    if (p.bytes > o.bytes) p = o;
+  }
   if (B == 0 || Sq == 0) return QF2_OK;
   if (!M.q || !M.out) return QF2_ERR_ARG;
   if (Skv > 0 && (!M.k || !M.v)) return QF2_ERR_ARG;

@@ -634,3 +634,19 @@ def test_many_rows_of_split_keys(cuda, D, dtype):
     out = A.masked_attn(q, k, v, tensor_layout="NHD")
     _compare(out, q, k, v, rows=[0, 127])
     assert torch.equal(out, A.masked_attn(q, k, v, tensor_layout="NHD"))
+
+
+@pytest.mark.parametrize("B,Sq,Hq,Hkv,D,dtype", [(64, 1, 24, 8, 128, BF16), (2, 16, 8, 4, 256, FP16), (1, 300, 12, 12, 64, BF16)])
+def test_narrow_windows_on_long_caches(cuda, B, Sq, Hq, Hkv, D, dtype):
+    from quantfun2_b200 import attention as A
+
+    Skv = 5000
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, seed=50)
+    lens = torch.randint(Sq, Skv + 1, (B,), device=cuda, generator=torch.Generator(device=cuda).manual_seed(2))
+    pick, rows = sorted({0, B // 2, B - 1}), sorted({0, Sq // 2, Sq - 1})
+    for window in ((0, 0), (127, 0), (700, 0), (90, 40)):
+        out = A.masked_attn(q, k, v, window=window, kv_lens=lens, q_offset="end", tensor_layout="NHD")
+        _compare(out[pick], q[pick], k[pick], v[pick], rows=rows, window=window, kv_lens=lens[pick].tolist(),
+                 offsets=[n - Sq for n in lens[pick].tolist()])
+        out = A.masked_attn(q, k, v, window=window, tensor_layout="NHD")
+        _compare(out[pick], q[pick], k[pick], v[pick], rows=rows, window=window)
