@@ -245,6 +245,9 @@ def _rows16(t: torch.Tensor):
     """t with rows a tensor map can read (contiguous channels, 16-byte aligned, no dimension
     lying on itself), and its strides."""
     st = t.stride()
+    if st[-1] == 1 and not (st[0] | st[1] | st[-2]) & 7 and st[0] > 0 and st[1] > 0 and st[-2] > 0 and \
+            not t.data_ptr() & 15:
+        return t, st  # (the common case, without a look at the shape)
     if st[-1] != 1 or t.data_ptr() % 16 or any((x % 8 or x <= 0) and n > 1 for x, n in zip(st[:-1], t.shape)):
         t = t.contiguous()
         if t.data_ptr() % 16:
