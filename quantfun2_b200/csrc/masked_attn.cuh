@@ -781,10 +781,10 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         }
         continue;
       }
-      // The scores 32 at a time, first for the maximum, then for the weights: all in registers, or
-      // (kSmall, which has fewer) out of tensor memory twice, where capped, biased or masked ones
-      // went back to.  Prompts of 64 x 512 keys take 33 us in registers and 27 us in two short
-      // loops; kPair the other way 1385 us in registers, 1438 us in loops (causal 16384 tokens).
+      // The scores, first for the maximum, then for the weights: all in registers, or (kSmall, which
+      // has fewer) 64 at a time out of tensor memory twice, where capped, biased or masked ones went
+      // back to.  16 x 512 tokens, 24 heads of 128, kSmall: 89 us in registers, 80 in loops of 32,
+      // 77 in loops of 64; kPair the other way 1385 us in registers, 1438 in loops (causal 16384).
       constexpr bool kHeld = KW == 32 || FORM != kSmall;
       const bool far = SCORE && A.table != nullptr && (p0 - q_hi >= A.reach || p0 + KW - 1 - q_lo <= -A.reach);
       const int e_hi = min(hi, pend) - p0, e_lo = lo - p0, e_pre = min(pre, pend) - p0, e_plo = plo - p0;
@@ -879,7 +879,10 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
             }
           }
         }
-        if (!kHeld && (SCORE || !full)) tmem_st32(tS + c, *reinterpret_cast<uint32_t(*)[32]>(x));
+        if (!kHeld && (SCORE || !full)) {
+          tmem_st32(tS + c, *reinterpret_cast<uint32_t(*)[32]>(x));
+          tmem_st32(tS + c + 32, *reinterpret_cast<uint32_t(*)[32]>(x + 32));
+        }
         float m[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) m[u] = fmax3(x[u], x[u + 8], x[u + 16]);
@@ -903,15 +906,11 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         tmem_wait_ld();
         prepare(xs, Int<KW>{}, 0);
       } else {
-        fetch(xs, 0);
 #pragma unroll 1
         for (int c = 0; c < KW; c += 64) {
+          tmem_ld64(tS + c, *reinterpret_cast<uint32_t(*)[64]>(xs));
           tmem_wait_ld();
-          fetch(xs + 32, c + 32);
-          prepare(xs, Int<32>{}, c);
-          tmem_wait_ld();
-          if (c + 64 < KW) fetch(xs, c + 64);
-          prepare(xs + 32, Int<32>{}, c + 32);
+          prepare(xs, Int<64>{}, c);
         }
       }
       if constexpr (!SCORE) mx *= A.scale;
@@ -920,7 +919,6 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       const bool rescale = __any_sync(0xffffffffu, exists && m_new > m_run + kTau);
       if constexpr (!kHeld) {
         if (SCORE || !full) tmem_wait_st();
-        fetch(xs, 0);
       }
       if (rescale) {
         const float alpha = m_run == -INFINITY ? 0.f : fast_exp2(m_run - m_new);
@@ -985,11 +983,9 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       } else {
 #pragma unroll 1
         for (int c = 0; c < KW; c += 64) {
+          tmem_ld64(tS + c, *reinterpret_cast<uint32_t(*)[64]>(xs));
           tmem_wait_ld();
-          fetch(xs + 32, c + 32);
           weigh(xs, c);
-          tmem_wait_ld();
-          if (c + 64 < KW) fetch(xs, c + 64);
           weigh(xs + 32, c + 32);
         }
       }
