@@ -301,18 +301,18 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   // Two query tiles per CTA, or one in each of two CTAs per SM, where both fill the SMs.  A pair
   // takes less time over a key tile of both, the small ones start and end under each other and
   // leave fewer rows and keys out of sight: waves of CTAs * (tiles seen * time of one + start and
-  // end), fitted in us to 138 shapes of 256 to 4096 tokens, 0.3 % off the better of both in the
-  // mean (always pairs: 11 %, never: 5 %).  24 / 8 heads of 128, pair against small: 4 x 4096
-  // tokens 764 and 864, causal windows of 300 on them 200 and 176, 16 x 512 tokens 91 and 82,
-  // 4 x 384 tokens 24.6 and 13.4.
+  // end), fitted in us to 204 shapes of 256 to 4096 tokens, 0.2 % off the better of both in the
+  // mean (always pairs: 12 %, never: 3 %).  24 / 8 heads of 128, pair against small: 4 x 4096
+  // tokens 758 and 826, causal windows of 300 on them 188 and 157, 16 x 512 tokens 88 and 79,
+  // 4 x 384 tokens 24.6 and 14.6.
   const int64_t npair = B * Hq * ((Sq + 2 * kBlk - 1) / (2 * kBlk));
   const bool full = D != 256 && Sq > kBlk && npair >= kSms;
   bool two = full;
   const double x = (double)D / 128.0;
   if (full) {
     const double keys = (double)(P + Skv);
-    const double pair = seen_tiles(known, Sq, keys, 2.0 * kBlk) * (1.4 + 0.4 * x + (known.score ? 0.5 : 0.0)) + 5.0 + 2.0 * x;
-    const double one = seen_tiles(known, Sq, keys, p->T) * (1.5 + 0.7 * x + (known.score ? 1.0 : 0.0)) + 4.5;
+    const double pair = seen_tiles(known, Sq, keys, 2.0 * kBlk) * (1.3 + 0.3 * x + (known.score ? 0.5 : 0.0)) + 4.5 + 2.5 * x;
+    const double one = seen_tiles(known, Sq, keys, p->T) * (1.5 + 0.5 * x + (known.score ? 0.6 : 0.0)) + 4.5;
     two = (double)((npair + kSms - 1) / kSms) * pair <=
           (double)((B * hw * p->qtiles[0] + 2 * kSms - 1) / (2 * kSms)) * one;
   }
@@ -356,7 +356,7 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
       const int64_t cap = form == kDeep ? kSms : 2 * kSms;  // CTAs at work at once
       double lat = form == kDeep ? (D == 256 ? 2.5 : few ? 0.5 + 0.4 * x : 1.1 + 0.1 * x)
                                  : few ? 0.85 + 0.35 * x : 1.3 + 0.9 * x;
-      if (known.score) lat += form == kDeep ? 0.5 : 1.0;
+      if (known.score) lat += form == kDeep ? 0.5 : 0.7;
       for (int64_t n = 1; n <= std::min<int64_t>(std::max<int64_t>(t0, 1), kSms); n += 1 + n / 8) {
         const int64_t len = std::max<int64_t>(1, (t0 + n - 1) / n);
         const int64_t s0 = std::max<int64_t>(1, (t0 + len - 1) / len);
