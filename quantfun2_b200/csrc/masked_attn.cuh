@@ -15,20 +15,20 @@
 //   warp 1      issues the products: S_t = Q_t K^T, then O_t += P_t V
 //   the rest    softmax, one thread per row, four warps per query tile
 // Three forms:
-//   kPair   long queries, NT = 2: one tile's softmax runs while the tensor cores work for the
-//           other, and K and V feed 256 rows; all of tensor memory, one CTA per SM
-//   kSmall  few query rows on few keys: half of everything, two CTAs per SM, one of which
+//   kPair   many rows that see many keys, NT = 2: one tile's softmax runs while the tensor cores
+//           work for the other, and K and V feed 256 rows; all of tensor memory, one CTA per SM
+//   kSmall  many rows that see few keys each: half of everything, two CTAs per SM, one of which
 //           starts, ends or waits for memory while the other works
-//   kDeep   few query rows on many keys, and head dim 256 (whose output takes half of tensor
+//   kDeep   few query rows, and head dim 256 (whose output takes half of tensor
 //           memory): one CTA per SM with a deep ring; the scores are double-buffered, so the
 //           next Q K^T runs under the softmax
 // A tile's rows are (batch element, token, query head of a group): one row per token, or all
 // query heads of a kv head packed side by side, so that single tokens read K and V once.
 //
 // Long queries are bound by one chain per tile (scores read, maximum, 128 exponentials a row,
-// probabilities stored, the last of P V, the next Q K^T: 3300 cycles for two tiles of which the
+// probabilities stored, the last of P V, the next Q K^T: 3100 cycles for two tiles of which the
 // exponent unit works 2048 and the tensor cores 2100), and by the board's power: 16384 causal
-// tokens of 24/8 heads of 128 take 1.38 ms cold (1190 TFLOP/s) and 1.6 ms in a long run, where the
+// tokens of 24/8 heads of 128 take 1.31 ms cold (1264 TFLOP/s) and 1.56 ms in a long run, where the
 // clock falls to 1.7 GHz.  Single tokens are bound by HBM: 16 elements on 8192 keys of 24
 // heads 6.4 TB/s.  Short calls are bound by what a CTA does once: 3 us until the first scores,
 // 2.5 us after the last.
@@ -62,7 +62,8 @@ using Int = std::integral_constant<int, N>;
 // 128 x 88 + 256 x 208 = 64512.  (88: with 56 the product warp kept its descriptors in local
 // memory.)  Two threads per row, exchanging maxima through shared memory, and a first part of
 // the exponentials taken before the maximum is known were both slower (8192 x 8192, 24 heads of
-// 128: 734 us; 772; 773), as were 1/8 to 3/8 of the exponentials on the FMA pipe.
+// 128: 734 us; 772; 773), as were 1/8 to 3/8 of the exponentials on the FMA pipe, and half key
+// tiles with products and barriers of their own (24 heads of 64: 684 us; 863).
 constexpr int threads(int nt) { return nt == 2 ? 384 : 192; }
 enum Form { kSmall = 0, kDeep = 1, kPair = 2 };
 constexpr int kRegsFew = 88, kRegsSoftmax = 208;
