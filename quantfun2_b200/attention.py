@@ -260,7 +260,8 @@ def _int32(t: torch.Tensor, shape, what: str, device) -> torch.Tensor:
     if t.device != device or t.shape != shape or t.dtype not in (torch.int32, torch.int64):
         raise QF2Error(f"{what} must be int32 (or int64) of shape {tuple(shape)} on {device}")
     if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+        # (lengths and positions beyond 32 bits are far ones, not what their low words say)
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
 
 

@@ -650,3 +650,18 @@ def test_narrow_windows_on_long_caches(cuda, B, Sq, Hq, Hkv, D, dtype):
                  offsets=[n - Sq for n in lens[pick].tolist()])
         out = A.masked_attn(q, k, v, window=window, tensor_layout="NHD")
         _compare(out[pick], q[pick], k[pick], v[pick], rows=rows, window=window)
+
+
+def test_lengths_and_offsets_in_64_bits(cuda):
+    """Beyond 32 bits: all keys, the far end; below zero: none."""
+    from quantfun2_b200 import attention as A
+
+    B, Sq, Skv = 5, 9, 300
+    q, k, v = _inputs(cuda, B, Sq, Skv, 2, 1, 64, BF16, seed=60)
+    lens = torch.tensor([2 ** 32 + 3, 2 ** 31, -2 ** 33, 2 ** 40, 5], device=cuda)
+    _compare(A.masked_attn(q, k, v, kv_lens=lens, tensor_layout="NHD"), q, k, v, kv_lens=lens.tolist())
+    off = torch.tensor([2 ** 40, -2 ** 40, 2 ** 32, 2 ** 32 - 1, 100], device=cuda)
+    out = A.masked_attn(q, k, v, window=(50, 0), q_offset=off, tensor_layout="NHD")
+    _compare(out, q, k, v, window=(50, 0), offsets=off.tolist())
+    out = A.masked_attn(q, k, v, window=(-1, 0), q_offset=off, prefix_lens=lens, tensor_layout="NHD")
+    _compare(out, q, k, v, window=(-1, 0), offsets=off.tolist(), prefix_lens=lens.tolist())

@@ -120,3 +120,12 @@ def test_argument_structs_match_the_header():
                 arr = re.match(r"\s*(\w+)(?:\[(\d+)\])?", nm)
                 fields.append((arr.group(1), int(arr.group(2) or 1), "d" if base == "double" and not star else "q"))
         assert fields == [tuple(f) for f in args.fields]
+
+
+def test_lengths_and_positions_beyond_32_bits_stay_far():
+    from quantfun2_b200.attention import _int32
+
+    x = torch.tensor([2 ** 32 + 3, 2 ** 31, 2 ** 40, -2 ** 40, -1, 7, 2 ** 31 - 1, -2 ** 31])
+    got = _int32(x, (8,), "kv_lens", x.device)
+    assert got.dtype == torch.int32
+    assert got.tolist() == [min(max(n, -2 ** 31), 2 ** 31 - 1) for n in x.tolist()]
