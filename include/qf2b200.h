@@ -271,7 +271,8 @@ int qf2_blocksparse_attn(const void* q, const int64_t* q_strides, const void* k,
  * taken as 2^29).  The query sees key j if
  *   j < kv_lens[b] (clamped to [0, Skv]; NULL: Skv)  and
  *   j < prefix_lens[b]  or  (left < 0 or j >= t_i - left) and (right < 0 or j <= t_i + right)
- *   and, with ids, q_ids[b][i] == k_ids[b][j] >= 0 (ids of documents; negative = padding).
+ *   and, with ids, q_ids[b][i] == k_ids[b][j] >= 0 (ids of documents; negative = padding;
+ *   int32, or both int64 with ids_i64 != 0, all 64 bits of which count).
  * Causal attention is right = 0.  Keys behind kv_lens, of a negative id, or outside every
  * query's band and prefix do not enter the result, whatever their bits; a NaN or infinite
  * value that some rows see may reach the others of
@@ -306,8 +307,9 @@ typedef struct qf2_masked_attn_args { /* every field 8 bytes */
   const int32_t* q_offsets;   /* [B], for QF2_OFFSET_ARRAY                               */
   int64_t q_offset;           /* for QF2_OFFSET_CONST                                    */
   int64_t q_offset_mode;
-  const int32_t* q_ids;       /* [B, Sq] or NULL                                         */
-  const int32_t* k_ids;       /* [B, Skv] or NULL, with q_ids                            */
+  const void* q_ids;          /* [B, Sq] or NULL                                         */
+  const void* k_ids;          /* [B, Skv] or NULL, with q_ids                            */
+  int64_t ids_i64;            /* 0: int32 ids                                            */
   const float* slopes;        /* [Hq] or NULL                                            */
   const float* bias_table;    /* [Hq, 2 * bias_reach + 1] or NULL, not with slopes       */
   int64_t bias_reach;
@@ -317,6 +319,7 @@ typedef struct qf2_masked_attn_args { /* every field 8 bytes */
   int64_t workspace_bytes;
   qf2_stream_t stream;
 } qf2_masked_attn_args;
+/* with_ids: 0 none, 1 int32, 2 int64 */
 int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P,
                                         int64_t D, int with_ids);
 int qf2_masked_attn(const qf2_masked_attn_args* args);

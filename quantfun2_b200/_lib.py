@@ -58,7 +58,7 @@ MASKED_ATTN_ARGS = _Args([
     ("prefix_k_strides", 2, "q"), ("prefix_v_strides", 2, "q"), ("B", 1, "q"), ("Hq", 1, "q"), ("Hkv", 1, "q"),
     ("Sq", 1, "q"), ("Skv", 1, "q"), ("P", 1, "q"), ("D", 1, "q"), ("dtype", 1, "q"), ("left", 1, "q"), ("right", 1, "q"),
     ("kv_lens", 1, "q"), ("prefix_lens", 1, "q"), ("q_offsets", 1, "q"), ("q_offset", 1, "q"), ("q_offset_mode", 1, "q"),
-    ("q_ids", 1, "q"), ("k_ids", 1, "q"), ("slopes", 1, "q"), ("bias_table", 1, "q"), ("bias_reach", 1, "q"),
+    ("q_ids", 1, "q"), ("k_ids", 1, "q"), ("ids_i64", 1, "q"), ("slopes", 1, "q"), ("bias_table", 1, "q"), ("bias_reach", 1, "q"),
     ("softcap", 1, "d"), ("sm_scale", 1, "d"), ("workspace", 1, "q"), ("workspace_bytes", 1, "q"), ("stream", 1, "q")])
 
 

@@ -256,13 +256,18 @@ def _rows16(t: torch.Tensor):
     return t, st
 
 
-def _int32(t: torch.Tensor, shape, what: str, device) -> torch.Tensor:
+def _ints(t: torch.Tensor, shape, what: str, device) -> torch.Tensor:
     if t.device != device or t.shape != shape or t.dtype not in (torch.int32, torch.int64):
         raise QF2Error(f"{what} must be int32 (or int64) of shape {tuple(shape)} on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _int32(t: torch.Tensor, shape, what: str, device) -> torch.Tensor:
+    t = _ints(t, shape, what, device)
     if t.dtype != torch.int32:
         # (lengths and positions beyond 32 bits are far ones, not what their low words say)
         t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
-    return t if t.is_contiguous() else t.contiguous()
+    return t
 
 
 def _float32(t: torch.Tensor, what: str, device) -> torch.Tensor:
@@ -335,7 +340,7 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
     left = right = -1
     if window is not None:
         left, right = max(int(window[0]), -1), max(int(window[1]), -1)
-    lens_p = pre_p = off_p = off = mode = qi_p = ki_p = slope_p = table_p = reach = 0
+    lens_p = pre_p = off_p = off = mode = qi_p = ki_p = id_words = slope_p = table_p = reach = 0
     if kv_lens is not None:
         kv_lens = _int32(kv_lens, (B,), "kv_lens", dev)
         lens_p = kv_lens.data_ptr()
@@ -344,10 +349,12 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
         pre_p = prefix_lens.data_ptr()
     if segment_ids is not None:
         qi, ki = segment_ids if isinstance(segment_ids, (tuple, list)) else (segment_ids, segment_ids)
-        qi = _int32(qi, (B, Sq), "segment_ids of the queries", dev)
-        ki = _int32(ki, (B, Skv), "segment_ids of the keys", dev)
+        qi = _ints(qi, (B, Sq), "segment_ids of the queries", dev)
+        ki = _ints(ki, (B, Skv), "segment_ids of the keys", dev)
+        if qi.dtype != ki.dtype:
+            qi, ki = qi.to(torch.int64), ki.to(torch.int64)
         if Skv:  # (without keys every row is zero, whatever its id)
-            qi_p, ki_p = qi.data_ptr(), ki.data_ptr()
+            qi_p, ki_p, id_words = qi.data_ptr(), ki.data_ptr(), 2 if qi.dtype == torch.int64 else 1
     if q_offset is None:
         if kv_lens is not None and (left >= 0 or right >= 0 or slopes is not None or bias_table is not None):
             raise QF2Error("with kv_lens, give q_offset: 0 for right-padded prompts, 'end' for the last tokens of a "
@@ -376,12 +383,12 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
         table_p, reach = bias_table.data_ptr(), bias_table.shape[1] // 2
     if sm_scale is None:
         sm_scale = 1.0 / math.sqrt(D)
-    nbytes = _masked_workspace(B, Hq, Hkv, Sq, Skv, P, D, int(ki_p != 0))
+    nbytes = _masked_workspace(B, Hq, Hkv, Sq, Skv, P, D, id_words)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     args = _lib.MASKED_ATTN_ARGS.pack(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), pkp, pvp, qs[0], qs[h], qs[n], ks[0], ks[h], ks[n],
         vs[0], vs[h], vs[n], os[0], os[h], os[n], pk_h, pk_n, pv_h, pv_n, B, Hq, Hkv, Sq, Skv, P, D, dt, left, right,
-        lens_p, pre_p, off_p, off, mode, qi_p, ki_p, slope_p, table_p, reach, softcap or 0.0, sm_scale,
+        lens_p, pre_p, off_p, off, mode, qi_p, ki_p, id_words == 2, slope_p, table_p, reach, softcap or 0.0, sm_scale,
         ws.data_ptr() if nbytes else 0, nbytes, raw_stream(dev.index))
     status = call_on(dev, _lib.load().qf2_masked_attn, args)
     if status:

@@ -15,29 +15,34 @@ __device__ int g_status;
 
 // ------------------------------------------------------------- key ids --
 // What the attention kernel wants to know of ids, in one launch.  grid (kb + qb, B), 1024 threads.
-// The first kb blocks of a batch element: a padded copy of the key ids (tiles of 128, pad -2) and
-// the least and greatest id of each tile, eight tiles a block.
+// The first kb blocks of a batch element: a padded copy of the key ids (tiles of 128, pad -2; of
+// 64-bit ids the low words, then the high ones, a negative id as -1) and the least and greatest
+// entry of each tile, eight tiles a block.
 // The other qb blocks, 1024 queries each: whether the key ids never fall (as unsigned numbers, so
 // that the negative ids of padding come last), which each block sees for itself; then the keys of
 // a query's id are one run, found here, and the attention kernel masks by ranges and looks at no
 // id.  A warp takes 32 queries, one id among them at a time: the tiles whose first key comes
 // before the id are counted, then such keys of the last of these tiles.
-__global__ void __launch_bounds__(1024) mattn_ids_kernel(const int32_t* __restrict__ q_ids,
-                                                         const int32_t* __restrict__ k_ids, int Sq, int Skv, int nto,
-                                                         int kb, int32_t* __restrict__ copy, int2* __restrict__ k_rng,
-                                                         int2* __restrict__ q_rng, int* __restrict__ sorted) {
+template <typename I>
+__global__ void __launch_bounds__(1024) mattn_ids_kernel(const I* __restrict__ q_ids, const I* __restrict__ k_ids,
+                                                         int Sq, int Skv, int nto, int kb, int32_t* __restrict__ copy,
+                                                         int64_t hi_off, int2* __restrict__ k_rng,
+                                                         int2* __restrict__ q_rng, int* __restrict__ order) {
+  using U = std::make_unsigned_t<I>;
   grid_launch_dependents();
   const int b = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int32_t* k = k_ids + (int64_t)b * Skv;
+  const I* k = k_ids + (int64_t)b * Skv;
   if ((int)blockIdx.x < kb) {
     const int j = blockIdx.x * 1024 + threadIdx.x, t = j / kBlk;
-    const int v = j < Skv ? k[j] : -2;
+    const I id = j < Skv ? k[j] : -2;
+    const int v = sizeof(I) == 8 && j < Skv && id < 0 ? -1 : (int)id;
     __shared__ int2 part[32];
     const int mn = __reduce_min_sync(0xffffffffu, v), mx = __reduce_max_sync(0xffffffffu, v);
     if (lane == 0) part[warp] = make_int2(mn, mx);
     __syncthreads();
     if (t >= nto) return;
     copy[(int64_t)b * nto * kBlk + j] = v;
+    if constexpr (sizeof(I) == 8) copy[hi_off + (int64_t)b * nto * kBlk + j] = (int)(id >> 32);
     if ((threadIdx.x & (kBlk - 1)) == 0) {
       const int2 p0 = part[warp], p1 = part[warp + 1], p2 = part[warp + 2], p3 = part[warp + 3];
       k_rng[(int64_t)b * nto + t] = make_int2(min(min(p0.x, p1.x), min(p2.x, p3.x)), max(max(p0.y, p1.y), max(p2.y, p3.y)));
@@ -45,32 +50,37 @@ __global__ void __launch_bounds__(1024) mattn_ids_kernel(const int32_t* __restri
     return;
   }
   const int i = (blockIdx.x - kb) * 1024 + threadIdx.x;
-  const int id = i < Sq ? q_ids[(int64_t)b * Sq + i] : -1;
-  int fine = 1;
+  const I id = i < Sq ? q_ids[(int64_t)b * Sq + i] : -1;
+  int fine = 1, wide = 0;
 #pragma unroll 4
-  for (int j = threadIdx.x; j < Skv - 1; j += 1024) fine &= (uint32_t)k[j] <= (uint32_t)k[j + 1];
+  for (int j = threadIdx.x; j < Skv - 1; j += 1024) {
+    fine &= (U)k[j] <= (U)k[j + 1];
+    if constexpr (sizeof(I) == 8) wide |= k[j] > 0x7fffffff;
+  }
   fine = __syncthreads_and(fine);
-  if ((int)blockIdx.x == kb && threadIdx.x == 0) sorted[b] = fine;
+  if (sizeof(I) == 8 && !fine) wide = __syncthreads_or(wide || k[Skv - 1] > 0x7fffffff);
+  // (out of order and all below 2^31, 64-bit ids are compared by their low words alone)
+  if ((int)blockIdx.x == kb && threadIdx.x == 0) order[b] = fine ? kInOrder : wide ? kMixedWide : kMixed;
   if (!fine) return;
   // keys of less than x (as unsigned numbers), by the warp
-  auto below = [&](uint32_t x) -> int {
+  auto below = [&](U x) -> int {
     int tiles = 0;
-    for (int t = lane; t < nto; t += 32) tiles += (uint32_t)k[(int64_t)t * kBlk] < x;
+    for (int t = lane; t < nto; t += 32) tiles += (U)k[(int64_t)t * kBlk] < x;
     tiles = __reduce_add_sync(0xffffffffu, tiles);
     if (tiles == 0) return 0;
     int n = 0;
 #pragma unroll
     for (int u = 0; u < kBlk; u += 32) {
       const int j = (tiles - 1) * kBlk + u + lane;
-      n += j < Skv && (uint32_t)k[j] < x;
+      n += j < Skv && (U)k[j] < x;
     }
     return (tiles - 1) * kBlk + __reduce_add_sync(0xffffffffu, n);
   };
   int2 r = make_int2(0, 0);
   uint32_t left = __ballot_sync(0xffffffffu, id >= 0);
   while (left) {
-    const int x = __shfl_sync(0xffffffffu, id, __ffs(left) - 1);
-    const int lo = below((uint32_t)x), hi = below((uint32_t)x + 1u);
+    const I x = __shfl_sync(0xffffffffu, id, __ffs(left) - 1);
+    const int lo = below((U)x), hi = below((U)x + 1u);
     if (id == x) r = make_int2(lo, hi);
     left &= ~__ballot_sync(0xffffffffu, id == x);
   }
@@ -246,7 +256,7 @@ struct Plan {
   int64_t items[2];  // CTAs of own and prefix items, splits counted
   bool parts;        // partial rows and a merge
   int64_t rows0;     // partial rows of the own items
-  int64_t ids_off, rng_off, qrng_off, sorted_off, tab_off, ml_off, o_off, bytes;
+  int64_t ids_off, rng_off, qrng_off, order_off, tab_off, ml_off, o_off, bytes;
 };
 
 // What of the mask the host knows: the window, the first query's position among all keys, whether
@@ -269,7 +279,7 @@ static double seen_tiles(const Known& m, int64_t Sq, double keys, double R) {
 }
 
 static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv, int64_t P, int64_t D,
-                     bool ids, const Known& known) {
+                     int id_words, const Known& known) {
   if (D != 64 && D != 96 && D != 128 && D != 256) return QF2_ERR_SHAPE;
   if (B < 0 || Sq < 0 || Skv < 0 || P < 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv) return QF2_ERR_SHAPE;
   if (B > 65535 || Hq > 65535 || Sq > (1 << 20)) return QF2_ERR_SHAPE;
@@ -396,10 +406,11 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
     if (want) off += (n + 255) & ~255ll;
     return at;
   };
-  p->ids_off = take(ids, B * nto * kBlk * 4);
+  const bool ids = id_words > 0;
+  p->ids_off = take(ids, B * nto * kBlk * 4 * id_words);
   p->rng_off = take(ids, B * nto * 8);
   p->qrng_off = take(ids, B * Sq * 8);
-  p->sorted_off = take(ids, B * 4);
+  p->order_off = take(ids, B * 4);
   p->tab_off = take(p->even > 0, B * hw * 8);
   p->ml_off = take(p->parts, rows * 8);
   p->o_off = take(p->parts, rows * D * 4);
@@ -449,11 +460,12 @@ using namespace qf2::mattn;
 
 extern "C" int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, int64_t Skv,
                                                    int64_t P, int64_t D, int with_ids) {
+  if (with_ids < 0 || with_ids > 2) return QF2_ERR_ARG;
   // the most that any mask's plan takes (with pairs or without them no rows are split)
   int64_t bytes = 0;
   for (int i = 0; i < 8; ++i) {
     Plan p;
-    const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids != 0, Known{-1.0, -1.0, 0.0, (i & 1) != 0, (i & 2) != 0, (i & 4) != 0});
+    const int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, with_ids, Known{-1.0, -1.0, 0.0, (i & 1) != 0, (i & 2) != 0, (i & 4) != 0});
     if (st != QF2_OK) return st;
     bytes = std::max(bytes, p.bytes);
   }
@@ -466,19 +478,20 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   const int64_t B = M.B, Hq = M.Hq, Hkv = M.Hkv, Sq = M.Sq, Skv = M.Skv, P = M.P, D = M.D, dtype = M.dtype;
   if (dtype != QF2_BF16 && dtype != QF2_F16) return QF2_ERR_DTYPE;
   const bool ids = M.k_ids != nullptr;
+  const int id_words = !ids ? 0 : M.ids_i64 ? 2 : 1;
   Plan p;
   // (positions and lengths on the device: taken for the end of the keys, and all of them)
   const double first = (double)P + (M.q_offset_mode == QF2_OFFSET_CONST ? (double)M.q_offset : (double)Skv - (double)Sq);
   const Known known{M.prefix_lens ? -1.0 : (double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0,
                     M.kv_lens || M.prefix_lens || M.q_offset_mode == QF2_OFFSET_ARRAY, M.bias_table != nullptr};
-  int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, ids, known);
+  int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, id_words, known);
   if (st != QF2_OK) return st;
   if (known.left >= 0.0 && known.right >= 0.0) {
     // the workspace is sized without a window: a plan that would take more gives way to that one's
     Known open = known;
     open.left = open.right = -1.0;
     Plan o;
-    st = make_plan(&o, B, Hq, Hkv, Sq, Skv, P, D, ids, open);
+    st = make_plan(&o, B, Hq, Hkv, Sq, Skv, P, D, id_words, open);
     if (st != QF2_OK) return st;
     if (p.bytes > o.bytes) p = o;
   }
@@ -579,12 +592,14 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   a.q_off_const = (int)std::min(std::max(M.q_offset, -far), far);
   a.left = M.left < 0 ? -1 : (int)std::min(M.left, far);
   a.right = M.right < 0 ? -1 : (int)std::min(M.right, far);
-  a.q_ids = M.q_ids;
+  a.q_ids = reinterpret_cast<const int32_t*>(M.q_ids);
+  a.id_words = id_words;
+  a.hi_off = B * (int64_t)p.nto * kBlk;
   if (ids) {
     a.k_ids = reinterpret_cast<int32_t*>(ws + p.ids_off);
     a.k_rng = reinterpret_cast<int2*>(ws + p.rng_off);
     a.q_rng = reinterpret_cast<int2*>(ws + p.qrng_off);
-    a.sorted = reinterpret_cast<int*>(ws + p.sorted_off);
+    a.order = reinterpret_cast<int*>(ws + p.order_off);
   }
   const double l2e = 1.4426950408889634;
   a.scale = (float)(M.sm_scale * l2e);
@@ -600,10 +615,16 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   cudaStream_t s = reinterpret_cast<cudaStream_t>(M.stream);
   if (ids) {
     const int kb = (p.nto + 7) / 8;
-    mattn_ids_kernel<<<dim3((unsigned)(kb + (Sq + 1023) / 1024), (unsigned)B), 1024, 0, s>>>(
-        M.q_ids, M.k_ids, (int)Sq, (int)Skv, p.nto, kb, reinterpret_cast<int32_t*>(ws + p.ids_off),
-        reinterpret_cast<int2*>(ws + p.rng_off), reinterpret_cast<int2*>(ws + p.qrng_off),
-        reinterpret_cast<int*>(ws + p.sorted_off));
+    const dim3 grid((unsigned)(kb + (Sq + 1023) / 1024), (unsigned)B);
+    auto launch = [&](auto type) {
+      using I = decltype(type);
+      mattn_ids_kernel<I><<<grid, 1024, 0, s>>>(
+          reinterpret_cast<const I*>(M.q_ids), reinterpret_cast<const I*>(M.k_ids), (int)Sq, (int)Skv, p.nto, kb,
+          reinterpret_cast<int32_t*>(ws + p.ids_off), a.hi_off, reinterpret_cast<int2*>(ws + p.rng_off),
+          reinterpret_cast<int2*>(ws + p.qrng_off), reinterpret_cast<int*>(ws + p.order_off));
+    };
+    if (M.ids_i64) launch(int64_t{});
+    else launch(int32_t{});
     QF2_LAUNCH_CHECK();
   }
   const unsigned grid = (unsigned)(p.items[0] + p.items[1]);

@@ -74,6 +74,10 @@ struct Div {
 };
 QF2_DEV int div_of(const Div& v, int x) { return (int)((__umulhi((uint32_t)x, v.m) + (uint32_t)x) >> v.s); }
 
+// Key ids of a batch element: out of order; out of order, some beyond 31 bits (compared by both
+// words); in order (q_rng holds)
+enum IdOrder { kMixed = 0, kMixedWide = 1, kInOrder = 2 };
+
 struct Args {
   void* out;
   S3 os;
@@ -100,11 +104,13 @@ struct Args {
   int q_off_mode;                     // 0 the constant, 1 the array, 2 the sequence's end
   int q_off_const;
   int left, right;                    // band, < 0 open
-  const int32_t* q_ids;
-  const int32_t* k_ids;               // padded copy [B][nto * 128] (pad -2)
-  const int2* k_rng;                  // [B][nto] least and greatest id of a key tile
+  const int32_t* q_ids;               // [B][Sq][id_words]
+  int id_words;                       // 2: 64-bit ids, the low word first
+  const int32_t* k_ids;               // padded copy [B][nto * 128] (pad -2); of 64-bit ids the low words
+  int64_t hi_off;                     // and the high words so many entries behind them
+  const int2* k_rng;                  // [B][nto] least and greatest entry of a key tile's copy
   const int2* q_rng;                  // [B][Sq] keys of the row's id, where they are in order
-  const int* sorted;                  // [B] key ids in order: q_rng holds
+  const int* order;                   // [B] IdOrder of the key ids
   // scores
   float scale;                        // sm_scale * log2 e
   float cap_in, cap_out;              // cap > 0: scale / cap, cap log2 e; else 0
@@ -444,7 +450,8 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   int rb = 0, rtok = 0, rh = 0, qpos = 0, lo = 0, hi = 0, plo = 0, pre = 0, id = 0;
   bool exists = false;
   grid_wait();  // for the kernels that prepared the ids (nothing else is still running)
-  const bool by_id = A.q_ids != nullptr && A.sorted[b0] == 0;
+  const int order = A.q_ids != nullptr ? A.order[b0] : kInOrder;
+  const bool by_id = order != kInOrder;
   // what any row of this warp sees
   int s_lo = 0x7fffffff, s_hi = 0, s_plo = 0x7fffffff, s_pre = 0, i_lo = 0x7fffffff, i_hi = -1;
   if (warp >= W0) {
@@ -466,8 +473,12 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     if (A.q_ids && exists) {
       const int64_t i = (int64_t)bc * A.Sq + rtok;
       if (by_id) {
-        id = A.q_ids[i];
+        id = A.q_ids[i * A.id_words];
         sees = id >= 0;
+        if (A.id_words == 2) {  // (a wide id among narrow keys has none)
+          const int top = A.q_ids[2 * i + 1];
+          sees = top == 0 ? order == kMixedWide || id >= 0 : order == kMixedWide && top > 0;
+        }
       } else {
         const int2 r = A.q_rng[i];
         lo = max(lo, r.x);
@@ -765,7 +776,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       if (krng) {
         const int2 r = krng[t - A.ntp];
         any = any && r.y >= i_lo && r.x <= i_hi;
-        if (!(r.x == r.y && i_lo == i_hi && r.x == i_lo)) {
+        if (!(r.x == r.y && i_lo == i_hi && r.x == i_lo) || A.order[b0] == kMixedWide) {
           full = false;
           kid = A.k_ids + ((int64_t)b0 * A.nto + (t - A.ntp)) * kBlk + k0;
         }
@@ -877,6 +888,17 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
               if (k4.y != id) x[4 * i + 1] = -INFINITY;
               if (k4.z != id) x[4 * i + 2] = -INFINITY;
               if (k4.w != id) x[4 * i + 3] = -INFINITY;
+            }
+            if (A.order[b0] == kMixedWide) {
+              const int top = exists ? A.q_ids[2 * ((int64_t)rb * A.Sq + rtok) + 1] : -1;
+#pragma unroll
+              for (int i = 0; i < N / 4; ++i) {
+                const int4 k4 = *reinterpret_cast<const int4*>(kid + A.hi_off + c + 4 * i);
+                if (k4.x != top) x[4 * i] = -INFINITY;
+                if (k4.y != top) x[4 * i + 1] = -INFINITY;
+                if (k4.z != top) x[4 * i + 2] = -INFINITY;
+                if (k4.w != top) x[4 * i + 3] = -INFINITY;
+              }
             }
           }
         }

@@ -665,3 +665,29 @@ def test_lengths_and_offsets_in_64_bits(cuda):
     _compare(out, q, k, v, window=(50, 0), offsets=off.tolist())
     out = A.masked_attn(q, k, v, window=(-1, 0), q_offset=off, prefix_lens=lens, tensor_layout="NHD")
     _compare(out, q, k, v, window=(-1, 0), offsets=off.tolist(), prefix_lens=lens.tolist())
+
+
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hkv,D,dtype", [
+    (3, 5, 300, 4, 2, 64, BF16), (3, 200, 500, 6, 2, 96, FP16), (3, 400, 900, 40, 8, 64, BF16), (3, 500, 2500, 24, 8, 128, FP16),
+    (3, 40, 300, 2, 1, 256, BF16)])
+def test_ids_in_64_bits(cuda, B, Sq, Skv, Hq, Hkv, D, dtype):
+    """Ids that share their low or their high words are unlike, in order and out of order; beside
+    int32 ones, and where only the queries' are wide."""
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, seed=61)
+    names = torch.tensor([5, 2 ** 31, 2 ** 32 + 5, 2 ** 33 + 5, 2 ** 33 + 6, 2 ** 63 - 1, -1, -2 ** 63], device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(62)
+    pick = lambda n, of: torch.randint(0, of, (B, n), device=cuda, generator=g)  # noqa: E731
+    rows = sorted({0, 1, Sq // 3, Sq // 2, Sq - 2, Sq - 1})
+    ki, qi = names[pick(Skv, 8).sort(1).values], names[pick(Sq, 8)]
+    mixed = names[pick(Skv, 8)]
+    mixed[1] = torch.where(mixed[1] > 2 ** 31 - 1, 7, mixed[1])          # an element of narrow ids
+    narrow = torch.randint(-1, 6, (B, Skv), device=cuda, generator=g)
+    for qq, kk in ((qi, ki), (qi, mixed), (qi, narrow), (qi, narrow.int()), (narrow[:, :Sq].int(), mixed), (narrow[:, :Sq], narrow)):
+        for window in ((-1, -1), (150, 30)):
+            out = A.masked_attn(q, k, v, window=window, segment_ids=(qq, kk), tensor_layout="NHD")
+            _compare(out, q, k, v, rows=rows, window=window, q_ids=qq.long(), k_ids=kk.long())
+    a = A.masked_attn(q, k, v, segment_ids=(narrow[:, :Sq], narrow), tensor_layout="NHD")
+    b = A.masked_attn(q, k, v, segment_ids=(narrow[:, :Sq].int(), narrow.int()), tensor_layout="NHD")
+    assert torch.equal(a, b)

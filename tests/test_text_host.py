@@ -129,3 +129,11 @@ def test_lengths_and_positions_beyond_32_bits_stay_far():
     got = _int32(x, (8,), "kv_lens", x.device)
     assert got.dtype == torch.int32
     assert got.tolist() == [min(max(n, -2 ** 31), 2 ** 31 - 1) for n in x.tolist()]
+
+
+def test_workspace_of_64_bit_ids():
+    ws = _lib.load().qf2_masked_attn_workspace_bytes
+    one, two = ws(2, 24, 8, 4096, 4096, 0, 128, 1), ws(2, 24, 8, 4096, 4096, 0, 128, 2)
+    assert two == one + 2 * 4096 * 4                                # the high words of the copy
+    assert ws(2, 24, 8, 4096, 4096, 0, 128, 3) == -8 and ws(2, 24, 8, 4096, 4096, 0, 128, -1) == -8
+    assert _call(q_ids=1024, k_ids=1024, ids_i64=1) == -6
