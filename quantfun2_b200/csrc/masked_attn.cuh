@@ -801,7 +801,16 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       const bool far = SCORE && A.table != nullptr && (p0 - q_hi >= A.reach || p0 + KW - 1 - q_lo <= -A.reach);
       const int e_hi = min(hi, pend) - p0, e_lo = lo - p0, e_pre = min(pre, pend) - p0, e_plo = plo - p0;
       float mx = -INFINITY;
-      // N scores, the first of key c of this thread's
+      // N scores, the first of key c of this thread's, into registers (one load: four of 32 columns,
+      // each with its own start, 677 against 641 us, 8192 x 8192 tokens, 24 heads of 64; the maximum
+      // of 32 under the next 32's load 722)
+      auto load = [&](float* x, auto count, int c) {
+        constexpr int N = decltype(count)::value;
+        if constexpr (N == 128) tmem_ld128(tS + c, *reinterpret_cast<uint32_t(*)[128]>(x));
+        else if constexpr (N == 64) tmem_ld64(tS + c, *reinterpret_cast<uint32_t(*)[64]>(x));
+        else tmem_ld32(tS + c, *reinterpret_cast<uint32_t(*)[32]>(x));
+        tmem_wait_ld();
+      };
       auto prepare = [&](float* x, auto count, int c) {
         constexpr int N = decltype(count)::value;
         if constexpr (SCORE) {
@@ -815,8 +824,10 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
 #pragma unroll
               for (int u = 0; u < 4; ++u) ma[u] = fmax3(ma[u], fabsf(x[i + 2 * u]), fabsf(x[i + 2 * u + 1]));
             const float big = fmaxf(fmaxf(ma[0], ma[1]), fmaxf(ma[2], ma[3]));
-            if (!__any_sync(0xffffffffu, big * A.cap_in > kTanhMost)) {
-              const float2 ci = make_float2(A.cap_in, A.cap_in), co = make_float2(A.cap_out, A.cap_out);
+            // Each score's formula follows from the score alone.  The vote (over hidden keys too) only
+            // spares the exponentials where no score needs them, and decides no bit of a result.
+            const float2 ci = make_float2(A.cap_in, A.cap_in), co = make_float2(A.cap_out, A.cap_out);
+            if (!__any_sync(0xffffffffu, exists && big * A.cap_in > kTanhMost)) {
 #pragma unroll
               for (int i = 0; i < N / 2; ++i) {
                 const float2 y = cap_poly(make_float2(x[2 * i], x[2 * i + 1]), ci, co);
@@ -824,11 +835,28 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
                 x[2 * i + 1] = y.y;
               }
             } else {
-              // cap tanh(z) = cap - 2 cap / (1 + e^(2 z)), to 2^-22 of the cap
+              // Beyond the polynomial's range cap tanh(z) = cap - 2 cap / (1 + e^(2 z)), to 2^-22 of the
+              // cap; within it a small score beside a great cap would be lost in that.  32 scores at a
+              // time out of tensor memory and back: with all of them and both formulas in registers
+              // 280 bytes more went to local memory, and calls that never come here took 12 % longer.
               const float c2 = 2.f * kLog2e * A.cap_in;
+#pragma unroll 1
+              for (int u = 0; u < N; u += 32) {
+                float s[32];
+                tmem_ld32(tS + c + u, *reinterpret_cast<uint32_t(*)[32]>(s));
+                tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < N; ++i)
-                x[i] = fmaf(-2.f * A.cap_out, fast_rcp(1.f + fast_exp2(x[i] * c2)), A.cap_out);
+                for (int i = 0; i < 32; i += 2) {
+                  const float2 y = cap_poly(make_float2(s[i], s[i + 1]), ci, co);
+                  const float e0 = fmaf(-2.f * A.cap_out, fast_rcp(1.f + fast_exp2(s[i] * c2)), A.cap_out);
+                  const float e1 = fmaf(-2.f * A.cap_out, fast_rcp(1.f + fast_exp2(s[i + 1] * c2)), A.cap_out);
+                  s[i] = fabsf(s[i]) * A.cap_in > kTanhMost ? e0 : y.x;
+                  s[i + 1] = fabsf(s[i + 1]) * A.cap_in > kTanhMost ? e1 : y.y;
+                }
+                tmem_st32(tS + c + u, *reinterpret_cast<uint32_t(*)[32]>(s));
+              }
+              tmem_wait_st();
+              load(x, count, c);
             }
             sx = 1.f;
           }
@@ -917,22 +945,14 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         for (int u = 0; u < 8; u += 2) m[u] = fmax3(m[u], m[u + 1], fmaxf(x[N - 8 + u], x[N - 7 + u]));
         mx = fmax3(fmax3(mx, m[0], m[2]), m[4], m[6]);
       };
-      auto fetch = [&](float* x, int c) { tmem_ld32(tS + c, *reinterpret_cast<uint32_t(*)[32]>(x)); };
       float xs[kHeld ? KW : 64];
       if constexpr (kHeld) {
-        // (one load: four of 32 columns, each with its own start, 677 against 641 us, 8192 x 8192
-        // tokens, 24 heads of 64; the maximum of 32 under the next 32's load 722)
-        if constexpr (KW == 128)
-          tmem_ld128(tS, *reinterpret_cast<uint32_t(*)[128]>(xs));
-        else
-          fetch(xs, 0);
-        tmem_wait_ld();
+        load(xs, Int<KW>{}, 0);
         prepare(xs, Int<KW>{}, 0);
       } else {
 #pragma unroll 1
         for (int c = 0; c < KW; c += 64) {
-          tmem_ld64(tS + c, *reinterpret_cast<uint32_t(*)[64]>(xs));
-          tmem_wait_ld();
+          load(xs, Int<64>{}, c);
           prepare(xs, Int<64>{}, c);
         }
       }
@@ -1006,8 +1026,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       } else {
 #pragma unroll 1
         for (int c = 0; c < KW; c += 64) {
-          tmem_ld64(tS + c, *reinterpret_cast<uint32_t(*)[64]>(xs));
-          tmem_wait_ld();
+          load(xs, Int<64>{}, c);
           weigh(xs, c);
           weigh(xs + 32, c + 32);
         }

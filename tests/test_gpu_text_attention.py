@@ -691,3 +691,43 @@ def test_ids_in_64_bits(cuda, B, Sq, Skv, Hq, Hkv, D, dtype):
     a = A.masked_attn(q, k, v, segment_ids=(narrow[:, :Sq], narrow), tensor_layout="NHD")
     b = A.masked_attn(q, k, v, segment_ids=(narrow[:, :Sq].int(), narrow.int()), tensor_layout="NHD")
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("Sq,Skv,Hq,D,dtype", [(1, 700, 4, 128, BF16), (5, 700, 4, 64, FP16), (200, 700, 4, 128, BF16), (300, 700, 80, 64, BF16),
+                                               (150, 700, 4, 256, FP16), (500, 2600, 48, 96, BF16)])
+def test_hidden_keys_choose_no_arithmetic_of_capped_scores(cuda, Sq, Skv, Hq, D, dtype):
+    """Great finite values behind the lengths, in padding and outside the window change no bit of
+    capped scores; neither does what an earlier kernel left in shared memory."""
+    from quantfun2_b200 import attention as A
+
+    B = 2
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hq // 2, D, dtype, seed=63)
+    lens = torch.tensor([Skv - 50, Skv // 2], device=cuda)
+    ids = torch.zeros(B, Skv, dtype=torch.int32, device=cuda)
+    ids[0, :70], ids[1, Skv // 2:] = -1, -1
+    qid = torch.zeros(B, Sq, dtype=torch.int32, device=cuda)
+    j = torch.arange(Skv, device=cuda)[None]
+    left = 300
+    calls = [(dict(kv_lens=lens), j >= lens[:, None]), (dict(segment_ids=(qid, ids)), ids < 0),
+             (dict(window=(left, 0)), (j < Skv - Sq - left).expand(B, Skv))]
+    for kw, hidden in calls:
+        outs = []
+        for fill in (0.0, 1e3, -1e3, math.nan):
+            kk = torch.where(hidden[:, :, None, None], fill, k.float()).to(dtype)
+            A.masked_attn(q * 30, k * 30, v, tensor_layout="NHD")        # large values in every block's memory
+            outs.append(A.masked_attn(q, kk, v, softcap=50.0, tensor_layout="NHD", **kw))
+        assert outs[0].any()
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.parametrize("cap", [0.5, 50.0, 1e3, 1e6, 1e15, 1e30, 1e38])
+@pytest.mark.parametrize("Sq,Hq,D,dtype", [(2, 2, 64, BF16), (130, 4, 128, FP16), (300, 80, 64, BF16), (70, 4, 256, BF16)])
+def test_caps_of_every_size(cuda, cap, Sq, Hq, D, dtype):
+    """A cap far above the scores leaves them as they are, in tiles with rows that do not exist
+    and beside a row whose scores reach the cap."""
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, 1, Sq, 192, Hq, Hq // 2, D, dtype, seed=64)
+    q[:, 0] *= 200
+    rows = sorted({1, Sq // 2, Sq - 1})
+    _compare(A.masked_attn(q, k, v, softcap=cap, tensor_layout="NHD"), q, k, v, rows=rows, softcap=cap)
