@@ -273,10 +273,10 @@ int qf2_blocksparse_attn(const void* q, const int64_t* q_strides, const void* k,
  *   j < prefix_lens[b]  or  (left < 0 or j >= t_i - left) and (right < 0 or j <= t_i + right)
  *   and, with ids, q_ids[b][i] == k_ids[b][j] >= 0 (ids of documents; negative = padding;
  *   int32, or both int64 with ids_i64 != 0, all 64 bits of which count).
- * Causal attention is right = 0.  Keys behind kv_lens, of a negative id, or outside every
- * query's band and prefix do not enter the result, whatever their bits; a NaN or infinite
- * value that some rows see may reach the others of
- * its tile (0 * NaN), as it does in a plain product.
+ * Causal attention is right = 0.  Keys that no query sees (behind kv_lens, of a negative id or
+ * one that no query has, outside every query's band and prefix) do not enter the result,
+ * whatever their bits; a NaN or infinite value that some rows see may reach the others of its
+ * tile (0 * NaN), as it does in a plain product.
  * prefix_k / prefix_v [P, Hkv, D] (strides {-, head, seq}): keys and values that all batch
  * elements share at positions 0 .. P - 1, read once for the rows of many batch elements;
  * the own key j, the queries and kv_lens then count from position P.  Not with ids.

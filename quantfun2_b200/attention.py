@@ -415,8 +415,9 @@ def masked_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: tuple
            or t - left <= j <= t + right)  (window = (left, right), -1 open; causal: (-1, 0))
       and their segment_ids are equal and not negative ([B, S], or a pair for queries and
                                             keys; documents, and -1 for padding).
-    A row that sees no key is zero.  What lies in keys that no row sees is not read into the
-    result, whatever its bits.  Scores: s = sm_scale q.k (default D ** -0.5), then softcap > 0:
+    A row that sees no key is zero.  What lies in keys that no query sees is not read into the
+    result, whatever its bits; a NaN or infinity in the values of a key that some queries see may
+    reach others beside them (0 * NaN, as in a plain product).  Scores: s = sm_scale q.k (default D ** -0.5), then softcap > 0:
     softcap * tanh(s / softcap), then minus slopes[h] * |t - j| (fp32 [Hq]) or plus
     bias_table[h, clamp(j - t, -R, R) + R] (fp32 [Hq, 2 R + 1], R <= 1024).  Inference only.
     `out` may be any strided view of q's shape with 16-byte aligned rows."""

@@ -600,6 +600,7 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
     a.k_rng = reinterpret_cast<int2*>(ws + p.rng_off);
     a.q_rng = reinterpret_cast<int2*>(ws + p.qrng_off);
     a.order = reinterpret_cast<int*>(ws + p.order_off);
+    a.aligned = M.q_ids == M.k_ids && Sq == Skv && M.q_offset_mode == QF2_OFFSET_CONST && M.q_offset == 0;
   }
   const double l2e = 1.4426950408889634;
   a.scale = (float)(M.sm_scale * l2e);

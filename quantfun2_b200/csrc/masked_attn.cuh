@@ -50,6 +50,7 @@ constexpr int kPart = 96;             // keys whose P V starts before the rest's
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kMaxSplits = 320;       // partial rows of one output row
 constexpr int kMaxEven = 1024;        // batch elements whose lengths a CTA weighs against each other
+constexpr int kIdSpan = 4096;         // ids of a CTA's rows that a bitmap holds
 constexpr int kSms = 148;             // B200; sizes the grids and splits (a count, not a limit)
 
 struct S3 { int64_t b, h, s; };
@@ -111,6 +112,7 @@ struct Args {
   const int2* k_rng;                  // [B][nto] least and greatest entry of a key tile's copy
   const int2* q_rng;                  // [B][Sq] keys of the row's id, where they are in order
   const int* order;                   // [B] IdOrder of the key ids
+  int aligned;                        // query i is key i: one array of ids, no offset
   // scores
   float scale;                        // sm_scale * log2 e
   float cap_in, cap_out;              // cap > 0: scale / cap, cap log2 e; else 0
@@ -136,7 +138,9 @@ struct Smem {
   static constexpr int bars = bits + kMaxTiles / 8;
   static constexpr int nbars = 1 + 2 * slots + 2 + 4 + 2 + 1;
   static constexpr int misc = bars + nbars * 8;
-  static constexpr int total = misc + 16 + 8 * 8 * 4;
+  static constexpr int idbits = misc + 16 + 8 * 8 * 4;  // ids of the rows, where ids are out of order
+  static constexpr int rows = (idbits + kIdSpan / 8 + 15) & ~15;  // what each row sees, where rows are unlike
+  static constexpr int total = rows + nt * kBlk * 24;
   // TMEM: 512 columns where one CTA has the SM (no second fits beside it), else 256 each
   static constexpr int cols = two ? 256 : 512;
   static_assert(total <= (two ? 113 : 227) * 1024, "shared memory");
@@ -340,6 +344,9 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::misc + 4);
   int* red = reinterpret_cast<int*>(smem + L::misc + 16);  // [softmax warp][8]
+  uint32_t* idbits = reinterpret_cast<uint32_t*>(smem + L::idbits);
+  int4* row_sees = reinterpret_cast<int4*>(smem + L::rows);  // [row] lo, hi, plo, pre
+  int2* row_id = reinterpret_cast<int2*>(row_sees + NT * kBlk);
 
   grid_launch_dependents();  // the merge may take its places; it waits for this grid's end
 
@@ -478,6 +485,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         if (A.id_words == 2) {  // (a wide id among narrow keys has none)
           const int top = A.q_ids[2 * i + 1];
           sees = top == 0 ? order == kMixedWide || id >= 0 : order == kMixedWide && top > 0;
+          row_id[tile * kBlk + quarter * 32 + lane].y = top;
         }
       } else {
         const int2 r = A.q_rng[i];
@@ -498,6 +506,12 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     if (by_id) {
       i_lo = __reduce_min_sync(0xffffffffu, blind ? big : id);
       i_hi = __reduce_max_sync(0xffffffffu, blind ? -1 : id);
+    }
+    if (!direct && (by_id || !A.aligned)) {
+      const int r = tile * kBlk + quarter * 32 + lane;
+      row_sees[r] = make_int4(lo, hi, plo, pre);
+      row_id[r].x = id;
+      if (r < kIdSpan / 32) idbits[r] = 0u;
     }
     if (!direct && lane == 0) {
       int* mine = red + (warp - W0) * 8;
@@ -532,6 +546,8 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     if (!krng) {
       it.j = share(total) + n - 1;
     } else {
+      const uint32_t nth = (uint32_t)id - (uint32_t)uid0;
+      if (warp >= W0 && (lo < hi || plo < pre) && nth < (uint32_t)kIdSpan) atomicOr(idbits + (nth >> 5), 1u << (nth & 31));
       const int w_lo = t_lo >> 5, w_hi = (t_hi + 31) >> 5;
       const int a1 = it.a0 + it.na, c1 = it.b0 + total - it.na;
       for (int w = w_lo + warp; w < w_hi; w += kThreads / 32) {
@@ -651,9 +667,54 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         }
         __syncwarp();
       };
-      // keys that no row of the CTA sees weigh nothing, yet 0 * NaN would reach every row:
-      // their V rows are cleared (a cache's unused end, padding, another text)
-      auto clear_dead = [&](int t, int j) {
+      // Keys that no row of the CTA sees weigh nothing, yet 0 * NaN would reach every row: their V
+      // rows are cleared (a cache's unused end, padding, another text).  These are the keys outside
+      // of what bounds all rows' ranges and ids, and between them (`look`)
+      //   0  none: ranges that follow on each other, one id
+      //   1  those of an id that no row has, by a bitmap: every row sees all keys of its id, or all up
+      //      to its own, and the keys behind the tile's first row are its rows
+      //   2  any: V is looked through for values that are not finite, and their keys are held
+      //      against each row (2 x 4000 tokens of ids out of order 707 -> 1093 us, so not where 1 does)
+      int look = 0;
+      auto choose_look = [&]() {
+        if (direct) return;
+        const bool wide = krng && A.order[b0] == kMixedWide, many = krng && (uid0 != uid1 || wide);
+        if (A.aligned && !many) return;
+        if (many && !wide && (uint32_t)uid1 - (uint32_t)uid0 < (uint32_t)kIdSpan && A.left < 0 &&
+            (A.right < 0 || (A.aligned && A.right == 0))) {
+          look = 1;
+          return;
+        }
+        if (many) {
+          look = 2;
+          return;
+        }
+        // no key is missed between ranges that all hold or touch one key, nor where each touches
+        // the next row's
+        int lo_m = 0, hi_m = 0x7fffffff, lo_p = 0, hi_p = 0x7fffffff, starts = 0;
+        bool apart = false;
+#pragma unroll 1
+        for (int r = lane; r < (quad ? 32 : NT * kBlk); r += 32) {
+          const int4 a = row_sees[r];
+          const int2 b = r > 0 ? *reinterpret_cast<const int2*>(row_sees + r - 1) : make_int2(0, 0);
+          const bool live = a.x < a.y, before = b.x < b.y;
+          if (live) lo_m = max(lo_m, a.x), hi_m = min(hi_m, a.y);
+          if (a.z < a.w) lo_p = max(lo_p, a.z), hi_p = min(hi_p, a.w);
+          starts += live && !before;
+          apart = apart || (live && before && max(a.x, b.x) > min(a.y, b.y));
+        }
+        const unsigned all = 0xffffffffu;
+        if ((__reduce_max_sync(all, lo_m) > __reduce_min_sync(all, hi_m) &&
+             (__any_sync(all, apart) || __reduce_add_sync(all, starts) > 1)) ||
+            __reduce_max_sync(all, lo_p) > __reduce_min_sync(all, hi_p))
+          look = 2;
+      };
+      auto clear_row = [&](uint8_t* v, int r) {
+        for (int c = 0; c < L::nb; ++c)
+          for (int u = 0; u < 8; ++u)
+            *reinterpret_cast<uint4*>(v + c * kTile + r * 128 + ((u + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+      };
+      auto clear_dead = [&](int t, int j, auto looks) {
         const int p0 = tile_pos(t), p1 = min(p0 + kBlk, tile_end(t));
         bool all = (p1 <= uhi && p0 >= ulo) || (p1 <= upre && p0 >= uplo);
         const int32_t* ids = nullptr;
@@ -662,16 +723,49 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
           all = all && r.x >= uid0 && r.y <= uid1;
           ids = A.k_ids + ((int64_t)b0 * A.nto + (t - A.ntp)) * kBlk;
         }
-        if (all) return;
+        if (all && !decltype(looks)::value) return;
         uint8_t* v = sR + ((2 * j + 1) % NS) * L::op;
         for (int r = lane; r < kBlk; r += 32) {
           const int p = p0 + r;
           bool dead = !((p < uhi && p >= ulo) || (p < upre && p >= uplo)) || p >= p1;
-          if (ids) dead = dead || ids[r] < uid0 || ids[r] > uid1;
-          if (dead)
+          if (ids) {
+            const int id = ids[r];
+            dead = dead || id < uid0 || id > uid1;
+            if (decltype(looks)::value && look == 1 && !dead) dead = !((idbits[(id - uid0) >> 5] >> ((id - uid0) & 31)) & 1u);
+          }
+          if (dead) clear_row(v, r);
+        }
+        if (decltype(looks)::value && look == 2) {
+#pragma unroll 1
+          for (int r = lane; r < kBlk; r += 32) {
+            uint32_t top = 0;  // the sign bits of halves whose exponent is all ones (cleared rows have none)
+            constexpr uint32_t kExp = F16 ? 0x7c007c00u : 0x7f807f80u, kOne = F16 ? 0x04000400u : 0x00800080u;
+#pragma unroll 1
             for (int c = 0; c < L::nb; ++c)
-              for (int u = 0; u < 8; ++u)
-                *reinterpret_cast<uint4*>(v + c * kTile + r * 128 + ((u + lane) & 7) * 16) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+              for (int u = 0; u < 8; ++u) {
+                const uint4 w = *reinterpret_cast<const uint4*>(v + c * kTile + r * 128 + ((u + lane) & 7) * 16);
+                top |= ((w.x & kExp) + kOne) | ((w.y & kExp) + kOne) | ((w.z & kExp) + kOne) | ((w.w & kExp) + kOne);
+              }
+            uint32_t odd = __ballot_sync(0xffffffffu, (top & 0x80008000u) != 0);
+#pragma unroll 1
+            while (odd) {
+              const int kl = __ffs(odd) - 1, kr = r - lane + kl;
+              odd &= odd - 1;
+              bool seen = false;
+#pragma unroll 1
+              for (int i = lane; i < (quad ? 32 : NT * kBlk); i += 32) {
+                const int4 m = row_sees[i];
+                bool s = (p0 + kr >= m.x && p0 + kr < m.y) || (p0 + kr >= m.z && p0 + kr < m.w);
+                if (ids) {
+                  s = s && row_id[i].x == ids[kr];
+                  if (A.order[b0] == kMixedWide) s = s && row_id[i].y == ids[A.hi_off + kr];
+                }
+                seen = seen || s;
+              }
+              if (!__any_sync(0xffffffffu, seen) && lane == kl) clear_row(v, r);
+            }
+          }
         }
         fence_async_smem();
         __syncwarp();
@@ -691,43 +785,50 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       if (ok) {
         tc_fence_after();
         for (int t = 0; t < NT; ++t) issue_qk(t, t, 0);
+        choose_look();
       }
-      if constexpr (DB) {
-        for (int j = 0; ok && j < n; ++j) {
-          if (j + 1 < n) {
-            // the other buffer's P was read by the PV of tile j - 1, issued before this product
-            if (!slot_full(2 * j + 2)) { ok = false; break; }
-            tc_fence_after();
-            issue_qk(0, (j + 1) & 1, j + 1);
+      // (the rare looks have a loop of their own: their registers in the one for all calls cost 3 to 6 %
+      // of the pair form's time)
+      auto steps = [&](auto looks) {
+        if constexpr (DB) {
+          for (int j = 0; ok && j < n; ++j) {
+            if (j + 1 < n) {
+              // the other buffer's P was read by the PV of tile j - 1, issued before this product
+              if (!slot_full(2 * j + 2)) { ok = false; break; }
+              tc_fence_after();
+              issue_qk(0, (j + 1) & 1, j + 1);
+            }
+            if (!slot_full(2 * j + 1)) { ok = false; break; }
+            clear_dead(it.next(), j, looks);
+            if (!pv_when_ready(0, j & 1, j)) { ok = false; break; }
           }
-          if (!slot_full(2 * j + 1)) { ok = false; break; }
-          clear_dead(it.next(), j);
-          if (!pv_when_ready(0, j & 1, j)) { ok = false; break; }
-        }
-      } else {
-        // One warp for both tiles keeps their softmaxes out of phase, so that they take turns
-        // at the exponent unit (a warp each: 795 us).  What the next step needs is waited for
-        // between the tiles, while the products issued last still run.
-        if (ok) ok = slot_full(1) && (NT == 1 || n < 2 || slot_full(2));
-        if (ok) clear_dead(it.next(), 0);
-        for (int j = 0; ok && j < n; ++j) {
-          const bool more = j + 1 < n;
+        } else {
+          // One warp for both tiles keeps their softmaxes out of phase, so that they take turns
+          // at the exponent unit (a warp each: 795 us).  What the next step needs is waited for
+          // between the tiles, while the products issued last still run.
+          if (ok) ok = slot_full(1) && (NT == 1 || n < 2 || slot_full(2));
+          if (ok) clear_dead(it.next(), 0, looks);
+          for (int j = 0; ok && j < n; ++j) {
+            const bool more = j + 1 < n;
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            if (!pv_when_ready(t, t, j)) { ok = false; break; }
-            if (!more) continue;
-            if (NT == 1 && !slot_full(2 * j + 2)) { ok = false; break; }
-            issue_qk(t, t, j + 1);
-            if (t == 0) {
-              if (!slot_full(2 * j + 3)) { ok = false; break; }
-              clear_dead(it.next(), j + 1);
-            } else if (j + 2 < n && !slot_full(2 * j + 4)) {
-              ok = false;
-              break;
+            for (int t = 0; t < NT; ++t) {
+              if (!pv_when_ready(t, t, j)) { ok = false; break; }
+              if (!more) continue;
+              if (NT == 1 && !slot_full(2 * j + 2)) { ok = false; break; }
+              issue_qk(t, t, j + 1);
+              if (t == 0) {
+                if (!slot_full(2 * j + 3)) { ok = false; break; }
+                clear_dead(it.next(), j + 1, looks);
+              } else if (j + 2 < n && !slot_full(2 * j + 4)) {
+                ok = false;
+                break;
+              }
             }
           }
         }
-      }
+      };
+      if (look == 0) steps(std::false_type{});
+      else steps(std::true_type{});
       if (elect_one()) {
         if (!ok) fail(kDevTimeoutMma);
         tc_commit(bar_drain);

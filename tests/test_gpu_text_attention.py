@@ -731,3 +731,65 @@ def test_caps_of_every_size(cuda, cap, Sq, Hq, D, dtype):
     q[:, 0] *= 200
     rows = sorted({1, Sq // 2, Sq - 1})
     _compare(A.masked_attn(q, k, v, softcap=cap, tensor_layout="NHD"), q, k, v, rows=rows, softcap=cap)
+
+
+@pytest.mark.parametrize("Sq,Hq,Hkv,D,dtype", [(2, 2, 1, 64, BF16), (2, 40, 20, 128, FP16), (200, 4, 2, 96, BF16), (200, 4, 2, 256, FP16), (300, 80, 40, 64, FP16),
+                                               (600, 40, 40, 128, BF16)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_keys_of_ids_without_queries_hold_garbage(cuda, Sq, Hq, Hkv, D, dtype, wide):
+    """Keys of an id between two ids of a tile's queries, that no query has, do not enter: the bits
+    of the result are those with zeros there.  In order and out of order; 64-bit ids with equal low words."""
+    from quantfun2_b200 import attention as A
+
+    B, Skv = 3, 700
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, seed=70)
+    g = torch.Generator(device=cuda).manual_seed(71)
+    ki = torch.arange(Skv, device=cuda)[None].expand(B, Skv) * 7 // Skv              # 0 .. 6, in order
+    qi = torch.randint(0, 4, (B, Sq), device=cuda, generator=g) * 2                  # even ones
+    if Sq > 2:
+        qi[1, 50:] = -1                                                              # few queries, others padding
+    qi[0] = qi[0].sort().values
+    perm = torch.randperm(Skv, device=cuda, generator=g)
+    name = (lambda x: torch.where(x < 0, x, 5 + x * 2 ** 32)) if wide else (lambda x: x.int())
+    for kid in (ki, ki[:, perm]):
+        hidden = torch.stack([~torch.isin(kid[b], qi[b]) for b in range(B)])
+        assert hidden.any(1).all()
+        outs = []
+        for fill in (0.0, math.nan, math.inf, -math.inf):
+            vv = torch.where(hidden[:, :, None, None], fill, v.float()).to(dtype)
+            outs.append(A.masked_attn(q, k, vv, segment_ids=(name(qi), name(kid)), tensor_layout="NHD"))
+        assert torch.isfinite(outs[0]).all() and outs[0].any()
+        assert all(torch.equal(outs[0], o) for o in outs[1:])
+        rows = sorted({0, Sq // 2, Sq - 1})
+        vv = torch.where(hidden[:, :, None, None], 0.0, v.float()).to(dtype)
+        _compare(outs[0], q, k, vv, rows=rows, q_ids=qi, k_ids=kid)
+
+
+def test_keys_between_bands_hold_garbage(cuda):
+    """Queries with padding between them and narrow windows; batch elements at far positions of one
+    shared prefix: what lies between their bands does not enter."""
+    from quantfun2_b200 import attention as A
+
+    for Hq, D in ((2, 64), (24, 128)):
+        S = 300
+        q, k, v = _inputs(cuda, 2, S, S, Hq, Hq, D, BF16, seed=72)
+        qi = torch.full((2, S), -1, device=cuda, dtype=torch.int32)
+        qi[0, [5, 6, 100, 290]] = 0
+        qi[1, [0, 299]] = 3
+        for ki in (torch.tensor([0, 3], device=cuda, dtype=torch.int32)[:, None].expand(2, S),
+                   torch.where(torch.arange(S, device=cuda) % 50 == 0, -1, torch.tensor([0, 3], device=cuda)[:, None]).int()):
+            t = torch.arange(S, device=cuda)
+            band = (t[:, None] - t[None]).abs() <= 2                       # [queries, keys]
+            hidden = torch.stack([~(band & (qi[b, :, None] == ki[b][None]) & (qi[b, :, None] >= 0)).any(0) for b in range(2)])
+            outs = [A.masked_attn(q, k, torch.where(hidden[:, :, None, None], f, v.float()).to(BF16), window=(2, 2),
+                                  segment_ids=(qi, ki), tensor_layout="NHD") for f in (0.0, math.nan, math.inf)]
+            assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and outs[0].any()
+        B, P = 6, 900
+        q, k, v, pk, pv = _inputs(cuda, B, 1, 4, Hq, Hq, D, BF16, seed=73, P=P)
+        at = torch.tensor([10, 890, 130, 500, 10, 2], device=cuda)         # positions in the prefix
+        for dist in (3, 60):
+            j = torch.arange(P, device=cuda)
+            hidden = ~((j[None] <= at[:, None]) & (j[None] >= at[:, None] - dist)).any(0)
+            outs = [A.shared_prefix_attn(q, pk, torch.where(hidden[:, None, None], f, pv.float()).to(BF16), k, v, window=(dist, 0),
+                                         q_offset=at - P, tensor_layout="NHD") for f in (0.0, math.nan, -math.inf)]
+            assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and outs[0].any()
