@@ -499,6 +499,10 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     if (!sees || plo >= pre) plo = pre = 0;
     const bool blind = !(lo < hi || plo < pre);
     const int big = 0x7fffffff;
+    // A linear bias counts from the nearest key in sight: a row's weights are the same, and those of
+    // keys far from the query (|t - j| beyond 2^20 steps, say) do not drown in the bias's rounding.
+    if (SCORE && A.slopes && !blind)
+      qpos = min(max(qpos, min(lo < hi ? lo : big, plo < pre ? plo : big)), max(hi, pre) - 1);
     s_lo = __reduce_min_sync(0xffffffffu, lo < hi ? lo : big);
     s_hi = __reduce_max_sync(0xffffffffu, hi);
     s_plo = __reduce_min_sync(0xffffffffu, plo < pre ? plo : big);

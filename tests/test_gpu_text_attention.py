@@ -793,3 +793,26 @@ def test_keys_between_bands_hold_garbage(cuda):
             outs = [A.shared_prefix_attn(q, pk, torch.where(hidden[:, None, None], f, pv.float()).to(BF16), k, v, window=(dist, 0),
                                          q_offset=at - P, tensor_layout="NHD") for f in (0.0, math.nan, -math.inf)]
             assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2]) and outs[0].any()
+
+
+@pytest.mark.parametrize("Sq,Skv,Hq,Hkv,D,dtype", [(1, 3000, 4, 2, 64, BF16), (5, 300, 4, 2, 128, FP16), (140, 500, 4, 4, 96, BF16), (300, 700, 80, 80, 64, BF16),
+                                                    (500, 2600, 48, 48, 128, FP16)])
+def test_slopes_of_far_queries(cuda, Sq, Skv, Hq, Hkv, D, dtype):
+    """Queries millions of positions from their keys, on both sides: the weights follow from the
+    keys' distances to each other."""
+    from quantfun2_b200 import attention as A
+
+    B = 3
+    q, k, v = _inputs(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, seed=74)
+    slopes = torch.rand(Hq, device=cuda) * 0.5 + 0.01
+    rows = sorted({0, Sq // 2, Sq - 1})
+    for off in ([2 ** 22, 2 ** 28 + 3, 10 ** 6], [-2 ** 28, -10 ** 6 - 1, -2 ** 22], [Skv, -Sq, 0]):
+        at = torch.tensor(off, device=cuda)
+        lens = torch.tensor([Skv, Skv // 2, Skv - 1], device=cuda)
+        for kw in (dict(), dict(kv_lens=lens), dict(prefix_lens=torch.tensor([7, 200, 0], device=cuda), window=(50, 50))):
+            out = A.masked_attn(q, k, v, slopes=slopes, q_offset=at, tensor_layout="NHD", **kw)
+            _compare(out, q, k, v, rows=rows, slopes=slopes, offsets=off, **{n: x.tolist() if hasattr(x, "tolist") else x for n, x in kw.items()})
+    P = 700
+    pk, pv = torch.randn(P, Hkv, D, device=cuda).to(dtype), torch.randn(P, Hkv, D, device=cuda).to(dtype)
+    out = A.shared_prefix_attn(q, pk, pv, k, v, slopes=slopes, q_offset=2 ** 27, tensor_layout="NHD")
+    _compare(out, q, k, v, rows=rows, slopes=slopes, offsets=[2 ** 27] * B, prefix_k=pk, prefix_v=pv)
