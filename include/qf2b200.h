@@ -314,7 +314,7 @@ typedef struct qf2_masked_attn_args { /* every field 8 bytes */
   const float* bias_table;    /* [Hq, 2 * bias_reach + 1] or NULL, not with slopes       */
   int64_t bias_reach;
   double softcap;             /* 0: none                                                 */
-  double sm_scale;
+  double sm_scale;            /* times log2 e finite in fp32                             */
   void* workspace;            /* qf2_masked_attn_workspace_bytes                         */
   int64_t workspace_bytes;
   qf2_stream_t stream;

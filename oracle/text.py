@@ -65,7 +65,7 @@ def attention(q, k, v, window=(-1, -1), prefix_lens=None, q_ids=None, k_ids=None
             qq = q[b, i].double().view(Hkv, G, D)
             s = torch.einsum("hgd,nhd->hgn", qq, kk).reshape(Hq, -1) * scale
             if softcap:
-                s = softcap * torch.tanh(s / softcap)
+                s = softcap * torch.tanh(s / torch.full_like(s, softcap))  # (a scalar goes by its reciprocal, which may overflow)
             if slopes is not None:
                 s = s - slopes.double()[:, None] * (t - j).abs().double()[None]
             if bias_table is not None:

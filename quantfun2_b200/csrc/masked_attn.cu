@@ -505,7 +505,8 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
     return QF2_ERR_ARG;
   if (M.slopes && M.bias_table) return QF2_ERR_ARG;
   if (M.bias_table && (M.bias_reach < 0 || M.bias_reach > kMaxReach)) return QF2_ERR_SHAPE;
-  if (!(M.softcap >= 0.0) || !(M.sm_scale > 0.0) || M.softcap > FLT_MAX || M.sm_scale > FLT_MAX) return QF2_ERR_ARG;
+  const double l2e = 1.4426950408889634;
+  if (!(M.softcap >= 0.0) || !(M.sm_scale > 0.0) || M.softcap > FLT_MAX || M.sm_scale * l2e > FLT_MAX) return QF2_ERR_ARG;
   if (!al16(M.q) || !al16(M.out) || (Skv > 0 && (!al16(M.k) || !al16(M.v))) ||
       (P > 0 && (!al16(M.prefix_k) || !al16(M.prefix_v))))
     return QF2_ERR_ALIGN;
@@ -602,10 +603,9 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
     a.order = reinterpret_cast<int*>(ws + p.order_off);
     a.aligned = M.q_ids == M.k_ids && Sq == Skv && M.q_offset_mode == QF2_OFFSET_CONST && M.q_offset == 0;
   }
-  const double l2e = 1.4426950408889634;
   a.scale = (float)(M.sm_scale * l2e);
   if (M.softcap > 0.0) {
-    a.cap_in = (float)(M.sm_scale / M.softcap);
+    a.cap_in = (float)std::min(M.sm_scale / M.softcap, 1e37);  // (finite; every score but zero takes the cap)
     a.cap_out = (float)(M.softcap * l2e);
   }
   a.slopes = M.slopes;

@@ -816,3 +816,14 @@ def test_slopes_of_far_queries(cuda, Sq, Skv, Hq, Hkv, D, dtype):
     pk, pv = torch.randn(P, Hkv, D, device=cuda).to(dtype), torch.randn(P, Hkv, D, device=cuda).to(dtype)
     out = A.shared_prefix_attn(q, pk, pv, k, v, slopes=slopes, q_offset=2 ** 27, tensor_layout="NHD")
     _compare(out, q, k, v, rows=rows, slopes=slopes, offsets=[2 ** 27] * B, prefix_k=pk, prefix_v=pv)
+
+
+@pytest.mark.parametrize("cap", [5e-324, 1e-42, 1e-38, 1e-20])
+def test_caps_near_zero(cuda, cap):
+    """All scores but zeros are at the cap, which is nothing: an even softmax, with zero rows of q too."""
+    from quantfun2_b200 import attention as A
+
+    for Sq, Hq in ((2, 2), (300, 80)):
+        q, k, v = _inputs(cuda, 1, Sq, 200, Hq, Hq, 64, BF16, seed=75)
+        q[:, 0] = 0.0
+        _compare(A.masked_attn(q, k, v, softcap=cap, tensor_layout="NHD"), q, k, v, rows=[0, Sq - 1], softcap=cap)

@@ -137,3 +137,8 @@ def test_workspace_of_64_bit_ids():
     assert two == one + 2 * 4096 * 4                                # the high words of the copy
     assert ws(2, 24, 8, 4096, 4096, 0, 128, 3) == -8 and ws(2, 24, 8, 4096, 4096, 0, 128, -1) == -8
     assert _call(q_ids=1024, k_ids=1024, ids_i64=1) == -6
+
+
+def test_scales_beyond_fp32_are_refused():
+    assert _call(sm_scale=3e38) == -8 and _call(sm_scale=2.4e38, softcap=1.0) == -8
+    assert _call(sm_scale=1e-300, B=0) == 0
