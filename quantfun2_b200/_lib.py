@@ -7,6 +7,7 @@ an sm_100 part, every op raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import struct
 from ctypes import c_float, c_int, c_int64, c_void_p, POINTER
@@ -258,6 +259,53 @@ def stream_ptr(device=None) -> c_void_p:
     import torch
 
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
+
+
+def overlaps_itself(t) -> bool:
+    """Whether elements of t may share memory (expanded or unfolded views)."""
+    return not t.is_contiguous() and _folded(t.stride(), t.shape)
+
+
+def overlap(a, b) -> bool:
+    """Whether an element of a may lie on one of b."""
+    pa, pb = a.data_ptr(), b.data_ptr()
+    if pa <= pb and a.is_contiguous() and pa + a.nbytes <= pb or pb <= pa and b.is_contiguous() and pb + b.nbytes <= pa:
+        return False  # (the common case)
+    return _overlap(pb - pa, a.stride(), a.shape, a.element_size(), b.stride(), b.shape, b.element_size())
+
+
+@functools.lru_cache(maxsize=1024)
+def _folded(strides, shape) -> bool:
+    ext = 1
+    for s, n in sorted(zip(strides, shape)):
+        if n == 0:
+            return False
+        if n > 1:
+            if s < ext:
+                return 0 not in shape
+            ext += s * (n - 1)
+    return False
+
+
+@functools.lru_cache(maxsize=1024)
+def _overlap(delta, sa, na, ea, sb, nb, eb) -> bool:
+    """b begins delta bytes behind a; strides and sizes, bytes of an element.  Slices of one
+    buffer are told apart by a stride of theirs: all strides from it on are its multiples, and
+    within one step of it a and b lie side by side."""
+    if 0 in na or 0 in nb:
+        return False
+    da = [(s * ea, n - 1) for s, n in zip(sa, na) if n > 1]
+    db = [(s * eb, n - 1) for s, n in zip(sb, nb) if n > 1]
+    if ea + sum(s * n for s, n in da) <= delta or eb + sum(s * n for s, n in db) <= -delta:
+        return False
+    strides = {s for s, _ in da + db if s}
+    for p in strides:
+        if any(s > p and s % p for s in strides):
+            continue
+        ia, ib = (e + sum(s * n for s, n in d if s < p) for e, d in ((ea, da), (eb, db)))
+        if ia <= delta % p and delta % p + ib <= p:
+            return False
+    return True
 
 
 _dtype_codes: dict = {}

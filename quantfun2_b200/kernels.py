@@ -26,7 +26,8 @@ import math
 import torch
 
 from . import _lib
-from ._lib import QF2Error, call_on, check, dtype_code, i64, raw_stream, require_device, stream_ptr
+from ._lib import (QF2Error, call_on, check, dtype_code, i64, overlap, overlaps_itself, raw_stream, require_device,
+                   stream_ptr)
 
 __all__ = [
     "copy_chunks",
@@ -233,10 +234,9 @@ def rotary_apply(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Ten
 def rotary_apply_(xq: torch.Tensor, xk: torch.Tensor | None, positions: torch.Tensor, inv_freq: torch.Tensor,
                   layout: str = "half", magnitude: float = 1.0, inverse: bool = False):
     """rotary_apply in place; returns the same tensors.  Tensors whose elements share memory
-    (expanded views) are refused."""
-    for t in (xq, xk):
-        if t is not None and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
-            raise QF2Error("rotary_apply_ needs tensors whose elements do not share memory")
+    (expanded views, or xq and xk that overlap) are refused."""
+    if overlaps_itself(xq) or (xk is not None and (overlaps_itself(xk) or overlap(xq, xk))):
+        raise QF2Error("rotary_apply_ needs tensors whose elements do not share memory")
     _rotary(xq, xk, positions, inv_freq, xq, xk, layout, magnitude, inverse)
     return xq, xk
 

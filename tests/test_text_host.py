@@ -142,3 +142,55 @@ def test_workspace_of_64_bit_ids():
 def test_scales_beyond_fp32_are_refused():
     assert _call(sm_scale=3e38) == -8 and _call(sm_scale=2.4e38, softcap=1.0) == -8
     assert _call(sm_scale=1e-300, B=0) == 0
+
+
+def test_overlap_of_views():
+    """Against the elements themselves, on views of one buffer."""
+    import random
+
+    from quantfun2_b200._lib import overlap, overlaps_itself
+
+    def places(t):
+        p = torch.zeros(t.shape, dtype=torch.int64) + t.storage_offset()
+        for d, (n, s) in enumerate(zip(t.shape, t.stride())):
+            p = p + (torch.arange(n) * s).view([-1] + [1] * (t.dim() - d - 1))
+        return p.flatten().tolist()
+
+    joint = torch.zeros(2, 50, 8, 64)
+    q, k, v = joint[:, :, :5], joint[:, :, 5:7], joint[:, :, 7:]
+    assert not overlap(q, k) and not overlap(k, q) and not overlap(q, v) and not overlaps_itself(q)
+    assert overlap(q, q) and overlap(joint, k) and overlap(q[:, 3:], q[:, :4]) and not overlap(q[:, 4:], q[:, :4])
+    hnd = torch.zeros(2, 8, 50, 64).transpose(1, 2)
+    assert not overlap(hnd[:, :, :3], hnd[:, :, 3:]) and overlap(hnd[:, :, :4], hnd[:, :, 3:])
+    assert not overlap(joint[..., :32], joint[..., 32:]) and overlap(joint[..., :33], joint[..., 32:])
+    assert overlaps_itself(torch.zeros(1, 3).expand(4, 3)) and overlaps_itself(torch.zeros(9).as_strided((3, 4), (2, 1)))
+    assert not overlap(torch.zeros(4), torch.zeros(4)) and not overlap(joint[:0], joint)
+    rng = random.Random(0)
+    buf = torch.zeros(400)
+    told = 0
+    for _ in range(3000):
+        def view():
+            dims = [rng.randint(1, 4) for _ in range(3)]
+            strides = [rng.choice([0, 1, 2, 4, 8, 12, 24, 48]) for _ in range(3)]
+            return buf.as_strided(dims, strides, rng.randint(0, 20))
+        a, b = view(), view()
+        pa, pb = places(a), places(b)
+        if set(pa) & set(pb):
+            assert overlap(a, b)
+        told += not overlap(a, b)
+        if len(set(pa)) < len(pa):
+            assert overlaps_itself(a)
+    assert told > 100
+
+
+def test_rotary_in_place_refuses_shared_memory():
+    from quantfun2_b200 import kernels
+
+    x = torch.zeros(1, 4, 6, 64)
+    pos, f = torch.arange(4), kernels.rotary_inv_freq(64)
+    for xq, xk in ((x, x), (x, x[:, :, 2:4]), (x[:, :, :3], x[:, :, 2:]), (x.as_strided((1, 4, 6, 64), (0, 320, 64, 1)), None),
+                   (x[:, :, :2], x[:, :1, 2:3].expand(1, 4, 1, 64))):
+        with pytest.raises(QF2Error, match="share memory"):
+            kernels.rotary_apply_(xq, xk, pos, f)
+    with pytest.raises(QF2Error, match="CUDA"):                     # slices side by side come as far as the device
+        kernels.rotary_apply_(x[:, :, :4], x[:, :, 4:], pos, f)
