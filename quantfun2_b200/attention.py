@@ -21,7 +21,8 @@ import math
 import torch
 
 from . import _lib
-from ._lib import QF2Error, call_on, check, i64, ptr32, raw_stream, require_device, stream_ptr
+from ._lib import (QF2Error, call_on, check, i64, overlap, overlaps_itself, ptr32, raw_stream, require_device,
+                   stream_ptr)
 
 __all__ = ["sageattn", "sageattn_varlen", "sage_quantize", "sage_workspace_layout", "block_topk_select",
            "blocksparse_attn", "flash_attn", "masked_attn", "shared_prefix_attn", "masked_attn_status", "do_attn",
@@ -317,6 +318,7 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
         for t in (q, k, v, prefix_k, prefix_v, slopes, bias_table):
             if t is not None and t.requires_grad:
                 raise QF2Error("masked attention is an inference op: its inputs must not require a gradient")
+    given = None
     if out is None:
         out = torch.empty_like(q)
         os = out.stride()
@@ -325,9 +327,15 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
             os = out.stride()
     else:
         os = out.stride()
-        if out.shape != q.shape or out.dtype != dtype or out.device != dev or os[3] != 1 or \
-                any(x == 0 and m > 1 for x, m in zip(os, out.shape)):
-            raise QF2Error("out must match q's shape, dtype and device, with a contiguous last dim")
+        if out.shape != q.shape or out.dtype != dtype or out.device != dev or os[3] != 1 or overlaps_itself(out):
+            raise QF2Error("out must match q's shape, dtype and device, with a contiguous last dim and elements that "
+                           "share no memory")
+        # (q itself is fine: a row's q is read before its result is written)
+        inputs = (k, v) if prefix_k is None else (k, v, prefix_k, prefix_v)
+        if any(overlap(out, t) for t in inputs) or (
+                (out.data_ptr() != q.data_ptr() or os != q.stride()) and overlap(out, q)):
+            given, out = out, torch.empty(q.shape, dtype=dtype, device=dev)
+            os = out.stride()
     q, qs = _rows16(q)
     k, ks = _rows16(k)
     v, vs = _rows16(v)
@@ -393,6 +401,8 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
     status = call_on(dev, _lib.load().qf2_masked_attn, args)
     if status:
         check(status, "qf2_masked_attn")
+    if given is not None:
+        return given.copy_(out)
     return out
 
 
@@ -420,7 +430,8 @@ def masked_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: tuple
     reach others beside them (0 * NaN, as in a plain product).  Scores: s = sm_scale q.k (default D ** -0.5), then softcap > 0:
     softcap * tanh(s / softcap), then minus slopes[h] * |t - j| (fp32 [Hq]) or plus
     bias_table[h, clamp(j - t, -R, R) + R] (fp32 [Hq, 2 R + 1], R <= 1024).  Inference only.
-    `out` may be any strided view of q's shape with 16-byte aligned rows."""
+    `out` may be any strided view of q's shape with 16-byte aligned rows, q itself among them;
+    where it overlaps an input in another way the result is made beside it and copied."""
     return _masked(q, None, None, k, v, window, prefix_lens, segment_ids, kv_lens, q_offset, softcap, slopes,
                    bias_table, sm_scale, tensor_layout, out)
 

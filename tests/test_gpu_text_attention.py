@@ -827,3 +827,35 @@ def test_caps_near_zero(cuda, cap):
         q, k, v = _inputs(cuda, 1, Sq, 200, Hq, Hq, 64, BF16, seed=75)
         q[:, 0] = 0.0
         _compare(A.masked_attn(q, k, v, softcap=cap, tensor_layout="NHD"), q, k, v, rows=[0, Sq - 1], softcap=cap)
+
+
+@pytest.mark.parametrize("B,S,H,D,dtype", [(2, 1, 4, 64, BF16), (1, 40, 4, 128, FP16), (3, 300, 40, 64, BF16), (2, 2500, 24, 128, BF16), (2, 300, 4, 256, BF16)])
+def test_out_over_the_inputs(cuda, B, S, H, D, dtype):
+    """Into q, k or v themselves, into parts of them, and beside them in one buffer."""
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, B, S, S, H, H, D, dtype, seed=76)
+    kw = dict(window=(-1, 0), tensor_layout="NHD")
+    want = A.masked_attn(q, k, v, **kw)
+    for n in range(3):
+        t = [x.clone() for x in (q, k, v)]
+        assert A.masked_attn(*t, out=t[n], **kw) is t[n] and torch.equal(t[n], want)
+    joint = torch.cat([q, k, v, v], 2)
+    for n in range(4):                                                # q's, k's, v's and the last heads
+        j = joint.clone()
+        qq, kk, vv, rest = j.split(H, 2)
+        out = (qq, kk, vv, rest)[n]
+        assert A.masked_attn(qq, kk, vv, out=out, **kw) is out and torch.equal(out, want)
+        keep = [m for m in range(4) if m != n]
+        assert all(torch.equal(j.split(H, 2)[m], joint.split(H, 2)[m]) for m in keep)
+    j = joint.clone()
+    qq, kk, vv, _ = j.split(H, 2)
+    out = j[:, :, H // 2:H // 2 + H]                                  # half over q, half over k
+    assert torch.equal(A.masked_attn(qq, kk, vv, out=out, **kw), want)
+    P = 200
+    pk, pv = torch.randn(B * S + P, H, D, device=cuda).to(dtype), torch.randn(P, H, D, device=cuda).to(dtype)
+    want = A.shared_prefix_attn(q, pk[:P], pv, k, v, **kw)
+    out = pk[:B * S].view(B, S, H, D)                                 # over the prefix's keys
+    assert torch.equal(A.shared_prefix_attn(q, pk[:P], pv, k, v, out=out, **kw), want)
+    with pytest.raises(A.QF2Error):
+        A.masked_attn(q, k, v, out=torch.empty(B * S * H * D, device=cuda, dtype=dtype).as_strided(q.shape, (0 if B > 1 else H * D, H * D, D // 2, 1)), **kw)
