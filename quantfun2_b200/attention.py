@@ -523,7 +523,7 @@ def do_attn(attn, xq: torch.Tensor, xk: torch.Tensor, xv: torch.Tensor, attn_mas
             raise QF2Error("the bf16 attention path takes unpadded batches; use ATTN='b200' for padded ones")
         return flash_attn(xq, xk, xv, softmax_scale, tensor_layout="NHD")
     if ATTN == "masked":
-        ids = None if attn_mask is None else attn_mask.to(torch.int32) - 1
+        ids = None if attn_mask is None else attn_mask.to(torch.bool).to(torch.int32) - 1
         return masked_attn(xq, xk, xv, segment_ids=ids, sm_scale=softmax_scale, tensor_layout="NHD")
     if ATTN not in ("b200", "sage"):
         raise QF2Error(f"unknown ATTN backend {ATTN!r}")

@@ -859,3 +859,18 @@ def test_out_over_the_inputs(cuda, B, S, H, D, dtype):
     assert torch.equal(A.shared_prefix_attn(q, pk[:P], pv, k, v, out=out, **kw), want)
     with pytest.raises(A.QF2Error):
         A.masked_attn(q, k, v, out=torch.empty(B * S * H * D, device=cuda, dtype=dtype).as_strided(q.shape, (0 if B > 1 else H * D, H * D, D // 2, 1)), **kw)
+
+
+def test_do_attn_masked_takes_masks_of_any_type(cuda):
+    """What is not zero is a token, as for the other backends."""
+    from quantfun2_b200 import attention as A
+
+    q, k, v = _inputs(cuda, 2, 90, 90, 4, 2, 64, BF16, seed=77)
+    mask = torch.rand(2, 90, device=cuda) < 0.7
+    A.ATTN = "masked"
+    try:
+        want = A.do_attn(None, q, k, v, mask)
+        for m in (mask.int(), mask.float() * 0.5, mask.to(torch.uint8) * torch.arange(1, 91, device=cuda, dtype=torch.uint8), -mask.long()):
+            assert torch.equal(A.do_attn(None, q, k, v, m), want)
+    finally:
+        A.ATTN = "b200"
