@@ -261,6 +261,21 @@ def stream_ptr(device=None) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def wants_derivative(*tensors) -> bool:
+    """Whether a gradient would be asked of any of the tensors (None among them), or one carries
+    a forward-mode tangent: the ops have neither, and must not drop them."""
+    import torch
+    from torch.autograd import forward_ad
+
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    if forward_ad._current_level < 0:
+        return False
+    return any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def overlaps_itself(t) -> bool:
     """Whether elements of t may share memory (expanded or unfolded views)."""
     return not t.is_contiguous() and _folded(t.stride(), t.shape)

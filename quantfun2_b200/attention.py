@@ -22,7 +22,7 @@ import torch
 
 from . import _lib
 from ._lib import (QF2Error, call_on, check, i64, overlap, overlaps_itself, ptr32, raw_stream, require_device,
-                   stream_ptr)
+                   stream_ptr, wants_derivative)
 
 __all__ = ["sageattn", "sageattn_varlen", "sage_quantize", "sage_workspace_layout", "block_topk_select",
            "blocksparse_attn", "flash_attn", "masked_attn", "shared_prefix_attn", "masked_attn_status", "do_attn",
@@ -314,10 +314,8 @@ def _masked(q, prefix_k, prefix_v, k, v, window, prefix_lens, segment_ids, kv_le
                 raise QF2Error("prefix_k and prefix_v must be alike, three-dimensional, with the own keys' dtype, "
                                "device, heads and head dim")
         P = prefix_k.shape[n - 1]
-    if torch.is_grad_enabled():
-        for t in (q, k, v, prefix_k, prefix_v, slopes, bias_table):
-            if t is not None and t.requires_grad:
-                raise QF2Error("masked attention is an inference op: its inputs must not require a gradient")
+    if wants_derivative(q, k, v, prefix_k, prefix_v, slopes, bias_table, out):
+        raise QF2Error("masked attention is an inference op: its inputs must not require a gradient or carry a tangent")
     given = None
     if out is None:
         out = torch.empty_like(q)

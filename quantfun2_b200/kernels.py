@@ -27,7 +27,7 @@ import torch
 
 from . import _lib
 from ._lib import (QF2Error, call_on, check, dtype_code, i64, overlap, overlaps_itself, raw_stream, require_device,
-                   stream_ptr)
+                   stream_ptr, wants_derivative)
 
 __all__ = [
     "copy_chunks",
@@ -174,7 +174,6 @@ def _rotary(xq, xk, positions, inv_freq, out_q, out_k, layout, magnitude, invers
     qs, qo = xq.stride(), out_q.stride()
     dev, dtype = xq.device, xq.dtype
     dt = dtype_code(dtype)
-    grad = xq.requires_grad
     if xk is None:
         kp = kop = Hk = 0
         ks = ko = _NO_STRIDES
@@ -186,11 +185,10 @@ def _rotary(xq, xk, positions, inv_freq, out_q, out_k, layout, magnitude, invers
         if Bk != B or Sk != S or Dk != D or xk.dtype != dtype or xk.device != dev or ks[3] != 1 or ko[3] != 1:
             raise QF2Error("xk must match xq in batch, seq, head_dim, dtype and device, with a contiguous last dim")
         kp, kop = xk.data_ptr(), out_k.data_ptr()
-        grad = grad or xk.requires_grad
     if qs[3] != 1 or qo[3] != 1:
         raise QF2Error("rotary_apply needs a contiguous last dim")
-    if grad and torch.is_grad_enabled():
-        raise QF2Error("rotary_apply is an inference op: its inputs must not require a gradient")
+    if wants_derivative(xq, xk, inv_freq):
+        raise QF2Error("rotary_apply is an inference op: its inputs must not require a gradient or carry a tangent")
     if inv_freq.dtype != torch.float64 or inv_freq.device != dev or inv_freq.dim() != 1 or \
             not inv_freq.is_contiguous():
         raise QF2Error("inv_freq must be a contiguous fp64 vector on the tensors' device")

@@ -152,3 +152,32 @@ def test_agrees_with_rope_apply(cuda):
     # both round a value known to 2^-20 of the row's greatest
     tol = 2 * (2.0 ** -8 * a.double().abs() + 2.0 ** -20 * x.double().abs().amax())
     assert ((a.double() - b.double()).abs() <= tol).all()
+
+
+def test_derivatives_are_refused(cuda):
+    """Neither a gradient nor a forward tangent is dropped without a word."""
+    from torch.autograd import forward_ad
+
+    from quantfun2_b200 import attention as A
+    from quantfun2_b200 import kernels as K
+
+    x = torch.randn(1, 4, 2, 64, device=cuda)
+    h = x.bfloat16()
+    pos, f = torch.arange(4, device=cuda), K.rotary_inv_freq(64, device=cuda)
+    calls = [lambda t: K.rotary_apply(t, None, pos, f), lambda t: K.rotary_apply(x, t, pos, f), lambda t: K.rotary_apply_(t, None, pos, f),
+             lambda t: A.masked_attn(t.bfloat16(), h, h), lambda t: A.masked_attn(h, h, t.bfloat16()),
+             lambda t: A.masked_attn(h, h, h, slopes=t[0, :, 0, 0].contiguous())]
+    for call in calls:
+        call(x.clone())
+        with forward_ad.dual_level():
+            with pytest.raises(K.QF2Error, match="tangent"):
+                call(forward_ad.make_dual(x.clone(), torch.ones_like(x)))
+            call(x.clone())                                              # no tangent of its own
+        with pytest.raises(Exception):
+            torch.func.jvp(lambda t: call(t), (x.clone(),), (torch.ones_like(x),))
+        with pytest.raises(Exception):
+            torch.func.grad(lambda t: call(t)[0].float().sum())(x.clone())
+    with pytest.raises(K.QF2Error, match="gradient"):
+        K.rotary_apply(x, None, pos, f.clone().requires_grad_())
+    with pytest.raises(K.QF2Error, match="gradient"):
+        A.masked_attn(h, h, h, out=h.clone().requires_grad_())

@@ -194,3 +194,18 @@ def test_rotary_in_place_refuses_shared_memory():
             kernels.rotary_apply_(xq, xk, pos, f)
     with pytest.raises(QF2Error, match="CUDA"):                     # slices side by side come as far as the device
         kernels.rotary_apply_(x[:, :, :4], x[:, :, 4:], pos, f)
+
+
+def test_derivatives_are_noticed():
+    from torch.autograd import forward_ad
+
+    from quantfun2_b200._lib import wants_derivative
+
+    x, w = torch.zeros(3), torch.zeros(3, requires_grad=True)
+    assert wants_derivative(x, None, w) and not wants_derivative(x, None)
+    with torch.no_grad():
+        assert not wants_derivative(w)
+        with forward_ad.dual_level():
+            d = forward_ad.make_dual(torch.zeros(3), torch.ones(3))
+            assert wants_derivative(x, d) and wants_derivative(d * 2) and not wants_derivative(x, None)
+    assert not wants_derivative(x)
