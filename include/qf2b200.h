@@ -324,6 +324,12 @@ int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int6
                                         int64_t D, int with_ids);
 int qf2_masked_attn(const qf2_masked_attn_args* args);
 int qf2_masked_attn_status(qf2_stream_t stream);
+/* How a call would be computed (on the host, from sizes and the mask's kind; pointers only say
+ * what is there): plan[8] = {kernel form (0 single query tiles, two blocks per SM; 1 single tiles,
+ * one block per SM; 2 pairs of tiles), query heads and tokens of a tile, splits of the own keys,
+ * blocks that share them by the elements' lengths (0: splits as given), batch elements of a prefix
+ * tile (0: none of its own), splits of the prefix, workspace bytes}. */
+int qf2_masked_attn_plan(const qf2_masked_attn_args* args, int64_t* plan);
 
 /* ------------------------------------------------------ quantized linears --
  * Replace the torchao weight subclasses the reference swaps into nn.Linear.weight

@@ -418,6 +418,27 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
   return QF2_OK;
 }
 
+// The plan of a call (a window may change it: what of the mask the host knows).
+static int plan_of(Plan* p, const qf2_masked_attn_args& M) {
+  const int id_words = M.k_ids == nullptr ? 0 : M.ids_i64 ? 2 : 1;
+  // (positions and lengths on the device: taken for the end of the keys, and all of them)
+  const double first = (double)M.P + (M.q_offset_mode == QF2_OFFSET_CONST ? (double)M.q_offset : (double)M.Skv - (double)M.Sq);
+  const Known known{M.prefix_lens ? -1.0 : (double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0,
+                    M.kv_lens || M.prefix_lens || M.q_offset_mode == QF2_OFFSET_ARRAY, M.bias_table != nullptr};
+  int st = make_plan(p, M.B, M.Hq, M.Hkv, M.Sq, M.Skv, M.P, M.D, id_words, known);
+  if (st != QF2_OK) return st;
+  if (known.left >= 0.0 && known.right >= 0.0) {
+    // the workspace is sized without a window: a plan that would take more gives way to that one's
+    Known open = known;
+    open.left = open.right = -1.0;
+    Plan o;
+    st = make_plan(&o, M.B, M.Hq, M.Hkv, M.Sq, M.Skv, M.P, M.D, id_words, open);
+    if (st != QF2_OK) return st;
+    if (p->bytes > o.bytes) *p = o;
+  }
+  return QF2_OK;
+}
+
 static bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // strides {batch, head, seq}; a dimension of one element has no stride to speak of
@@ -472,6 +493,16 @@ extern "C" int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_
   return bytes;
 }
 
+extern "C" int qf2_masked_attn_plan(const qf2_masked_attn_args* args, int64_t* plan) {
+  if (!args || !plan) return QF2_ERR_ARG;
+  Plan p;
+  const int st = plan_of(&p, *args);
+  if (st != QF2_OK) return st;
+  const int64_t v[8] = {p.form, p.G, p.T, p.splits[0], p.even, p.items[1] > 0 ? p.Nb[1] : 0, p.splits[1], p.bytes};
+  for (int i = 0; i < 8; ++i) plan[i] = v[i];
+  return QF2_OK;
+}
+
 extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   if (!args) return QF2_ERR_ARG;
   const qf2_masked_attn_args& M = *args;
@@ -480,21 +511,8 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   const bool ids = M.k_ids != nullptr;
   const int id_words = !ids ? 0 : M.ids_i64 ? 2 : 1;
   Plan p;
-  // (positions and lengths on the device: taken for the end of the keys, and all of them)
-  const double first = (double)P + (M.q_offset_mode == QF2_OFFSET_CONST ? (double)M.q_offset : (double)Skv - (double)Sq);
-  const Known known{M.prefix_lens ? -1.0 : (double)M.left, (double)M.right, first, M.slopes || M.bias_table || M.softcap > 0.0,
-                    M.kv_lens || M.prefix_lens || M.q_offset_mode == QF2_OFFSET_ARRAY, M.bias_table != nullptr};
-  int st = make_plan(&p, B, Hq, Hkv, Sq, Skv, P, D, id_words, known);
+  int st = plan_of(&p, M);
   if (st != QF2_OK) return st;
-  if (known.left >= 0.0 && known.right >= 0.0) {
-    // the workspace is sized without a window: a plan that would take more gives way to that one's
-    Known open = known;
-    open.left = open.right = -1.0;
-    Plan o;
-    st = make_plan(&o, B, Hq, Hkv, Sq, Skv, P, D, id_words, open);
-    if (st != QF2_OK) return st;
-    if (p.bytes > o.bytes) p = o;
-  }
   if (B == 0 || Sq == 0) return QF2_OK;
   if (!M.q || !M.out) return QF2_ERR_ARG;
   if (Skv > 0 && (!M.k || !M.v)) return QF2_ERR_ARG;

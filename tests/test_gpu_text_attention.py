@@ -668,7 +668,7 @@ def test_lengths_and_offsets_in_64_bits(cuda):
 
 
 @pytest.mark.parametrize("B,Sq,Skv,Hq,Hkv,D,dtype", [
-    (3, 5, 300, 4, 2, 64, BF16), (3, 200, 500, 6, 2, 96, FP16), (3, 400, 900, 40, 8, 64, BF16), (3, 500, 2500, 24, 8, 128, FP16),
+    (3, 5, 300, 4, 2, 64, BF16), (3, 200, 500, 6, 2, 96, FP16), (3, 400, 900, 40, 8, 64, BF16), (4, 500, 2500, 24, 8, 128, FP16),
     (3, 40, 300, 2, 1, 256, BF16)])
 def test_ids_in_64_bits(cuda, B, Sq, Skv, Hq, Hkv, D, dtype):
     """Ids that share their low or their high words are unlike, in order and out of order; beside

@@ -170,3 +170,52 @@ def test_every_key_behind_a_shared_prefix(cuda, B, Sq, Skv, P, Hq, Hkv, D, dtype
     for window in ((-1, 0), (P // 2, 0)):
         call = lambda k, v, pk, pv: A.shared_prefix_attn(q, pk, pv, k, v, window=window, kv_lens=dlens, q_offset=Skv - Sq, tensor_layout="NHD")  # noqa: E731,B023
         _check(call, _seen(cuda, B, Sq, Skv, P, window=window, offsets=[Skv - Sq] * B, kv_lens=lens.tolist()), Hkv, D, dtype, P)
+
+
+# splits by what each element has to read, decided on the device
+UNLIKE = [(16, 1, 4000, 12, 4, 64, BF16, 0), (2, 100, 20000, 12, 4, 64, FP16, 0), (8, 5, 8000, 8, 8, 128, BF16, 0), (4, 1, 20000, 24, 8, 128, BF16, 0),
+          (3, 1, 30000, 4, 4, 96, FP16, 0), (2, 5, 9000, 8, 4, 256, BF16, 0), (2, 100, 9000, 4, 4, 128, FP16, 0), (5, 1, 20000, 8, 8, 64, BF16, 700),
+          (5, 40, 9000, 2, 2, 128, FP16, 700), (30, 1, 4000, 6, 2, 96, BF16, 700)]
+
+
+def _unlike(B, Skv):
+    lens = torch.randint(0, Skv + 1, (B,), generator=torch.Generator().manual_seed(B))
+    lens[0], lens[B // 2] = Skv, 1
+    if B > 2:
+        lens[1] = 0
+    return lens.tolist()
+
+
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hkv,D,dtype,P", UNLIKE)
+def test_every_key_of_unlike_lengths(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, P):
+    from quantfun2_b200 import attention as A
+
+    q = _zero(cuda, B, Sq, Hq, D, dtype)
+    for lens in (_unlike(B, Skv), [Skv] * B, [Skv] + [0] * (B - 1), [0] * B):
+        dlens, end = torch.tensor(lens, device=cuda), [n - Sq for n in lens]
+        for window, score in (((-1, 0), {}), ((-1, 0), dict(softcap=30.0)), ((Skv // 2, 0), {})):
+            kw = dict(window=window, kv_lens=dlens, q_offset="end", tensor_layout="NHD", **score)
+            call = (lambda k, v, pk, pv: A.shared_prefix_attn(q, pk, pv, k, v, **kw)) if P else (  # noqa: B023
+                lambda k, v, pk, pv: A.masked_attn(q, k, v, **kw))  # noqa: B023
+            _check(call, _seen(cuda, B, Sq, Skv, P, window=window, offsets=end, kv_lens=lens), Hkv, D, dtype, P)
+
+
+@pytest.mark.parametrize("B,Sq,Skv,Hq,Hkv,D,dtype,P", UNLIKE)
+def test_caches_of_unlike_lengths(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, P):
+    """Against the formula, with and without a bias; the bits of a second call."""
+    from quantfun2_b200 import attention as A
+    from test_gpu_text_attention import _compare, _inputs
+
+    made = _inputs(cuda, B, Sq, Skv, Hq, Hkv, D, dtype, seed=80, P=P)
+    (q, k, v), pre = made[:3], made[3:]
+    lens = _unlike(B, Skv)
+    pick, rows = sorted({0, B // 2, B - 1}), sorted({0, Sq - 1})
+    off = [n - Sq for n in lens]
+    for more in (dict(), dict(slopes=torch.rand(Hq, device=cuda) * 0.01), dict(softcap=20.0)):
+        kw = dict(window=(-1, 0), kv_lens=torch.tensor(lens, device=cuda), q_offset="end", tensor_layout="NHD", **more)
+        call = (lambda: A.shared_prefix_attn(q, *pre, k, v, **kw)) if P else (lambda: A.masked_attn(q, k, v, **kw))  # noqa: B023
+        out = call()
+        ref = dict(prefix_k=pre[0], prefix_v=pre[1]) if P else {}
+        _compare(out[pick], q[pick], k[pick], v[pick], rows=rows, window=(-1, 0), kv_lens=[lens[b] for b in pick],
+                 offsets=[off[b] for b in pick], **more, **ref)
+        assert torch.equal(out, call())
