@@ -324,6 +324,12 @@ int64_t qf2_masked_attn_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int6
                                         int64_t D, int with_ids);
 int qf2_masked_attn(const qf2_masked_attn_args* args);
 int qf2_masked_attn_status(qf2_stream_t stream);
+/* Failure injection for tests of the bounded waits, as qf2_sage_fault_injection, for every later
+ * masked attention launch of the process: waits are bounded to about wait_limit_us (<= 0: the
+ * default, about 2 s), and with skip_kv_tile >= 0 that key tile of each block is never loaded, so
+ * that the waits on it run out; qf2_masked_attn_status then returns QF2_ERR_TIMEOUT, the output
+ * of the call is undefined and the context stays usable.  (0, -1) restores normal operation. */
+int qf2_masked_attn_fault_injection(int64_t wait_limit_us, int skip_kv_tile);
 /* How a call would be computed (on the host, from sizes and the mask's kind; pointers only say
  * what is there): plan[8] = {kernel form (0 single query tiles, two blocks per SM; 1 single tiles,
  * one block per SM; 2 pairs of tiles), query heads and tokens of a tile, splits of the own keys,

@@ -131,6 +131,7 @@ SIGNATURES = {
         c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int]),
     "qf2_masked_attn": (c_int, [ctypes.c_char_p]),
     "qf2_masked_attn_status": (c_int, [c_void_p]),
+    "qf2_masked_attn_fault_injection": (c_int, [c_int64, c_int]),
     "qf2_masked_attn_plan": (c_int, [ctypes.c_char_p, _P64]),
     "qf2_quantize_rows": (
         c_int, [c_void_p, c_int64, c_int, c_int64, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p]),

@@ -13,6 +13,10 @@ namespace mattn {
 // It lives in the module, zero when loaded, so that a call needs no launch to clear one.
 __device__ int g_status;
 
+// Failure-injection settings of the launches (qf2_masked_attn_fault_injection).
+static std::atomic<long long> g_wait_clocks{kWaitClocks};
+static std::atomic<int> g_skip_kv{-1};
+
 // ------------------------------------------------------------- key ids --
 // What the attention kernel wants to know of ids, in one launch.  grid (kb + qb, B), 1024 threads.
 // The first kb blocks of a batch element: a padded copy of the key ids (tiles of 128, pad -2; of
@@ -630,6 +634,8 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   a.table = M.bias_table;
   a.reach = (int)M.bias_reach;
   a.status = reinterpret_cast<int*>(status);
+  a.wait_clocks = g_wait_clocks.load(std::memory_order_relaxed);
+  a.skip_kv = g_skip_kv.load(std::memory_order_relaxed);
   const bool score = M.softcap > 0.0 || M.slopes || M.bias_table;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(M.stream);
   if (ids) {
@@ -656,6 +662,13 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   if (p.parts) {
     QF2_CUDA_CHECK(f16 ? launch_merge<true>(a, D, B * Sq * Hq, s) : launch_merge<false>(a, D, B * Sq * Hq, s));
   }
+  return QF2_OK;
+}
+
+extern "C" int qf2_masked_attn_fault_injection(int64_t wait_limit_us, int skip_kv_tile) {
+  // SM clocks per microsecond: the B200's 1965 MHz maximum rounded up
+  g_wait_clocks.store(wait_limit_us > 0 ? wait_limit_us * 2000 : qf2::kWaitClocks, std::memory_order_relaxed);
+  g_skip_kv.store(skip_kv_tile >= 0 ? skip_kv_tile : -1, std::memory_order_relaxed);
   return QF2_OK;
 }
 

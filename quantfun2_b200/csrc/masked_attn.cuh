@@ -120,6 +120,8 @@ struct Args {
   const float* table;                 // [Hq][2 * reach + 1]
   int reach;
   int* status;
+  long long wait_clocks;              // bound of each wait (kWaitClocks but in tests of it)
+  int skip_kv;                        // key tile of a CTA that is never loaded, for such tests; else -1
 };
 
 template <int D, int FORM>
@@ -401,6 +403,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
   auto load_kv = [&](int t, int kv, int i) {
     const bool px = t < A.ntp;
     const int y = (px ? t : t - A.ntp) * kBlk, sl = i % NS;
+    if (i / 2 == A.skip_kv) return;
     const CUtensorMap* m = kv ? (px ? &tmpv : &tmv) : (px ? &tmpk : &tmk);
     uint8_t* dst = sR + sl * L::op;
     if (elect_one()) {
@@ -594,15 +597,16 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
     const long long t0 = clock64();
     while (true) {
       if (__all_sync(0xffffffffu, mbar_try_wait(a, parity))) return true;
-      if (__any_sync(0xffffffffu, *abort_flag != 0 || clock64() - t0 > kWaitClocks)) return false;
+      if (__any_sync(0xffffffffu, *abort_flag != 0 || clock64() - t0 > A.wait_clocks)) return false;
     }
   };
 
+  int issued = 0;  // warp 0: copies into the ring
   if (warp < W0) {
     if constexpr (NT == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsFew));
     if (warp == 0) {
       // ---------------------------------------------------------- producer --
-      int issued = 2 * ahead;
+      issued = 2 * ahead;
       bool ok = true;
       for (int j = ahead; ok && j < n; ++j) {
         const int t = it.next();
@@ -619,11 +623,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         }
       }
       // copies in flight land before the CTA ends (Q also where no key tile was active)
-      if (lane == 0) {
-        mbar_wait(bar_q, 0);
-        if (*abort_flag)
-          for (int i = issued > NS ? issued - NS : 0; i < issued; ++i) mbar_wait(bar_full + (i % NS), (i / NS) & 1);
-      }
+      if (lane == 0) mbar_wait(bar_q, 0, A.wait_clocks);
       __syncwarp();
     } else if (warp == 1 && n > 0) {
       // ---------------------------------------------------------- products --
@@ -836,7 +836,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
       if (elect_one()) {
         if (!ok) fail(kDevTimeoutMma);
         tc_commit(bar_drain);
-        mbar_wait(bar_drain, 0);
+        mbar_wait(bar_drain, 0, A.wait_clocks);
       }
       __syncwarp();
     }
@@ -1294,6 +1294,9 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
 
   tc_fence_before();
   __syncthreads();
+  // (after a wait that gave up nobody has waited for the last copies)
+  if (warp == 0 && lane == 0 && *abort_flag)
+    for (int i = issued > NS ? issued - NS : 0; i < issued; ++i) mbar_wait(bar_full + (i % NS), (i / NS) & 1, A.wait_clocks);
   if (warp == 1) {
     __syncwarp();
     tc_fence_after();
