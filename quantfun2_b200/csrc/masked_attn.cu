@@ -580,23 +580,17 @@ extern "C" int qf2_masked_attn(const qf2_masked_attn_args* args) {
   a.G = p.G; a.T = p.T;
   for (int i = 0; i < 2; ++i) { a.Nb[i] = p.Nb[i]; a.qtiles[i] = p.qtiles[i]; a.splits[i] = p.splits[i]; }
   a.Hw = (int)(Hq / p.G);
-  auto div = [](int64_t d) {
-    Div v{0, 0};
-    while ((1ll << v.s) < d) ++v.s;
-    v.m = (uint32_t)(((1ull << 32) * ((1ull << v.s) - (uint64_t)d)) / (uint64_t)d + 1);
-    return v;
-  };
-  a.by_G = div(a.G);
-  a.by_T = div(a.T);
-  a.by_group = div(Hq / Hkv);
-  a.by_Hw = div(a.Hw);
-  a.by_tt = div(a.qtiles[0]);
-  a.by_Hq = div(Hq);
-  a.by_Sq = div(Sq);
+  a.by_G = qf2::make_div(a.G);
+  a.by_T = qf2::make_div(a.T);
+  a.by_group = qf2::make_div(Hq / Hkv);
+  a.by_Hw = qf2::make_div(a.Hw);
+  a.by_tt = qf2::make_div(a.qtiles[0]);
+  a.by_Hq = qf2::make_div(Hq);
+  a.by_Sq = qf2::make_div(Sq);
   for (int i = 0; i < 2; ++i) {
     a.heads[i] = a.Hw * (i == 0 ? a.B : 1);
-    a.by_heads[i] = div(a.heads[i]);
-    a.by_splits[i] = div(a.splits[i]);
+    a.by_heads[i] = qf2::make_div(a.heads[i]);
+    a.by_splits[i] = qf2::make_div(a.splits[i]);
   }
   a.items1 = (int)p.items[1];
   a.merged = p.merged;

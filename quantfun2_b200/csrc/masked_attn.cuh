@@ -69,12 +69,6 @@ constexpr int threads(int nt) { return nt == 2 ? 384 : 192; }
 enum Form { kSmall = 0, kDeep = 1, kPair = 2 };
 constexpr int kRegsFew = 88, kRegsSoftmax = 208;
 
-// Division by a number known on the host: x / d = (umulhi(x, m) + x) >> s for x < 2^31.
-struct Div {
-  uint32_t m, s;
-};
-QF2_DEV int div_of(const Div& v, int x) { return (int)((__umulhi((uint32_t)x, v.m) + (uint32_t)x) >> v.s); }
-
 // Key ids of a batch element: out of order; out of order, some beyond 31 bits (compared by both
 // words); in order (q_rng holds)
 enum IdOrder { kMixed = 0, kMixedWide = 1, kInOrder = 2 };

@@ -48,6 +48,18 @@ QF2_DEV uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
 
+// Division by a number known on the host: x / d = (umulhi(x, m) + x) >> s for x < 2^31.
+struct Div {
+  uint32_t m, s;
+};
+QF2_DEV int div_of(const Div& v, int x) { return (int)((__umulhi((uint32_t)x, v.m) + (uint32_t)x) >> v.s); }
+inline Div make_div(int64_t d) {
+  Div v{0, 0};
+  while ((1ll << v.s) < d) ++v.s;
+  v.m = (uint32_t)(((1ull << 32) * ((1ull << v.s) - (uint64_t)d)) / (uint64_t)d + 1);
+  return v;
+}
+
 // Programmatic dependent launch: the next kernel of the stream may be placed from here on / wait
 // until the kernel ahead has ended and its writes are visible (no effect on a plain launch).
 QF2_DEV void grid_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -468,15 +480,6 @@ QF2_DEV void tmem_ld128(uint32_t taddr, uint32_t (&r)[128]) {
       : "r"(taddr));
 }
 
-QF2_DEV void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
 QF2_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -484,12 +487,6 @@ QF2_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
       "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
-}
-
-QF2_DEV void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
-               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
-               : "memory");
 }
 
 QF2_DEV void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {

@@ -24,12 +24,6 @@ struct Side {
   int64_t ob, os, oh;  // output strides
 };
 
-// Division by a number known on the host: x / d = (umulhi(x, m) + x) >> s for x < 2^31.
-struct Div {
-  uint32_t m, s;
-};
-QF2_DEV int div_of(const Div& v, int x) { return (int)((__umulhi((uint32_t)x, v.m) + (uint32_t)x) >> v.s); }
-
 struct Args {
   Side q, k;
   int Hq, H;  // q heads, q + k heads
@@ -159,15 +153,9 @@ static cudaError_t launch(Args& a, bool half_layout, bool vec, bool copy_rest, c
   a.tok_blk = tb;
   const int64_t blocks = (a.tokens + tb - 1) / tb;
   if (blocks > 0x7fffffffll) return cudaErrorInvalidValue;
-  auto div = [](int64_t d) {
-    Div v{0, 0};
-    while ((1ll << v.s) < d) ++v.s;
-    v.m = (uint32_t)(((1ull << 32) * ((1ull << v.s) - (uint64_t)d)) / (uint64_t)d + 1);
-    return v;
-  };
-  a.by_units = div(a.units);
-  a.by_H = div(a.H);
-  a.by_half = div(a.half);
+  a.by_units = make_div(a.units);
+  a.by_H = make_div(a.H);
+  a.by_half = make_div(a.half);
   const int64_t per = (int64_t)tb * a.H * a.units;
   int64_t y = 592 / blocks;
   y = y < 1 ? 1 : y;
