@@ -263,13 +263,20 @@ def stream_ptr(device=None) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_autograd = None
+
+
 def wants_derivative(*tensors) -> bool:
     """Whether a gradient would be asked of any of the tensors (None among them), or one carries
     a forward-mode tangent: the ops have neither, and must not drop them."""
-    import torch
-    from torch.autograd import forward_ad
+    global _autograd
+    if _autograd is None:
+        import torch
+        from torch.autograd import forward_ad
 
-    if torch.is_grad_enabled():
+        _autograd = torch.is_grad_enabled, forward_ad
+    grad_enabled, forward_ad = _autograd
+    if grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
