@@ -677,7 +677,19 @@ def profile_cases(dev) -> dict:
             return lambda: masked_attn(q, k, v, window=(-1, 0), tensor_layout="NHD")
         return case
 
+    def masked_attn_capped(b, n, hq, hkv, d, left):  # capped scores: short prompts, or padded ones in a window
+        def case():
+            from quantfun2_b200.attention import masked_attn
+
+            q, k, v = rn(b, n, hq, d).to(bf), rn(b, n, hkv, d).to(bf), rn(b, n, hkv, d).to(bf)
+            ids = (torch.arange(n, device=dev)[None] < n - 100 * torch.arange(b, device=dev)[:, None]).int() - 1
+            return lambda: masked_attn(q, k, v, window=(left, 0), segment_ids=ids if left >= 0 else None, softcap=50.0,
+                                       tensor_layout="NHD")
+        return case
+
     return {"rotary": rotary, "masked_attn": masked_attn_case(8192), "masked_attn_single": masked_attn_case(1),
+            "masked_attn_small": masked_attn_capped(16, 512, 24, 8, 64, -1),
+            "masked_attn_wide": masked_attn_capped(4, 1000, 8, 4, 256, 511),
             "lumina_step": lumina_step, "flux_step": flux_step, "rope": rope, "qkv_norm_rope": qkv_norm_rope, "rmsnorm": rmsnorm, "softmax": softmax,
             "gate_residual": gate_residual, "ln_modulate": ln_modulate, "quantize_rows": quantize_rows,
             "codes_to_bf16": codes_to_bf16, "quantize_weight": quantize_weight, "copy_chunks": copy_chunks,

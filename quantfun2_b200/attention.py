@@ -427,7 +427,9 @@ def masked_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: tuple
     result, whatever its bits; a NaN or infinity in the values of a key that some queries see may
     reach others beside them (0 * NaN, as in a plain product).  Scores: s = sm_scale q.k (default D ** -0.5), then softcap > 0:
     softcap * tanh(s / softcap), then minus slopes[h] * |t - j| (fp32 [Hq]) or plus
-    bias_table[h, clamp(j - t, -R, R) + R] (fp32 [Hq, 2 R + 1], R <= 1024).  Inference only.
+    bias_table[h, clamp(j - t, -R, R) + R] (fp32 [Hq, 2 R + 1], R <= 1024).  The probabilities
+    are rounded to the operands' type before they weigh the values, their sum is taken before that.
+    int64 lengths, offsets and ids count in all their bits.  Inference only.
     `out` may be any strided view of q's shape with 16-byte aligned rows, q itself among them;
     where it overlaps an input in another way the result is made beside it and copied."""
     return _masked(q, None, None, k, v, window, prefix_lens, segment_ids, kv_lens, q_offset, softcap, slopes,

@@ -362,7 +362,10 @@ static int make_plan(Plan* p, int64_t B, int64_t Hq, int64_t Hkv, int64_t Sq, in
     // and launches the merge.  kDeep, one CTA per SM, takes less time over a tile than kSmall, two
     // per SM (1.2 against 1.9 us for 128 rows, 0.9 against 1.2 us for the four copies of up to 32),
     // and kSmall takes twice the items in a wave: 500 tokens of 24 / 8 heads of 128 9.9 us in kDeep
-    // and 13.7 us in kSmall, 64 single tokens on 4096 keys 176 and 162 us.
+    // and 13.7 us in kSmall, 64 single tokens on 4096 keys 176 and 162 us.  Where it misses most: a
+    // second wave of memory-bound tiles is priced too high, so that 16 single tokens on 8192 keys of
+    // 12 heads of 64 take one split (84 us in the sweep that it was fitted to, 71 with three), and
+    // 4 x 16 tokens on 1000 keys 18 % more than the best.
     const bool few = (int64_t)p->G * p->T <= 32;
     const double rows = (double)B * (double)Sq * (double)Hq;
     double best = 1e30, walk = 0.0;

@@ -1,7 +1,7 @@
 // Masked, capped and biased 16-bit attention (sm_100a): the kernel and its launcher,
 // compiled per head dim in masked_attn_d*.cu; the entry points are in masked_attn.cu.
 //
-//   s(i, j) = scale q_i.k_j;  s = cap tanh(s / cap);  s += -slope_h |t_i - j| or
+//   s(i, j) = scale q_i.k_j;  s = cap tanh(s / cap);  s -= slope_h |t_i - j| or
 //   s += table_h[clamp(j - t_i, -R, R)];  out_i = sum_seen e^s v_j / sum_seen e^s
 //
 // for the keys j that the query at position t_i sees (a band, a prefix, a length, an id);
@@ -61,7 +61,10 @@ using Int = std::integral_constant<int, N>;
 // NT = 2: three warpgroups, so that registers can move from the first (producer, products,
 // two idle warps) to the softmax ones: launched with 168 a thread (384 x 168 = 64512), then
 // 128 x 88 + 256 x 208 = 64512.  (88: with 56 the product warp kept its descriptors in local
-// memory.)  Two threads per row, exchanging maxima through shared memory, and a first part of
+// memory.)  The compiler reports 410 to 500 bytes of spill stores for these kernels, about 350 of
+// them with the products left out (the softmax warps, whose 128 scores are all in registers) and
+// 70 to 200 with the softmax left out; kDeep with capped or biased scores has 8 to 124, kSmall none.
+// Two threads per row, exchanging maxima through shared memory, and a first part of
 // the exponentials taken before the maximum is known were both slower (8192 x 8192, 24 heads of
 // 128: 734 us; 772; 773), as were 1/8 to 3/8 of the exponentials on the FMA pipe, and half key
 // tiles with products and barriers of their own (24 heads of 64: 684 us; 863).
@@ -721,7 +724,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
           all = all && r.x >= uid0 && r.y <= uid1;
           ids = A.k_ids + ((int64_t)b0 * A.nto + (t - A.ntp)) * kBlk;
         }
-        if (all && !decltype(looks)::value) return;
+        if (all && (!decltype(looks)::value || look == 0)) return;
         uint8_t* v = sR + ((2 * j + 1) % NS) * L::op;
         for (int r = lane; r < kBlk; r += 32) {
           const int p = p0 + r;
@@ -785,8 +788,8 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
         for (int t = 0; t < NT; ++t) issue_qk(t, t, 0);
         choose_look();
       }
-      // (the rare looks have a loop of their own: their registers in the one for all calls cost 3 to 6 %
-      // of the pair form's time)
+      // (kPair: the rare looks have a loop of their own; their registers in the one for all calls cost 3
+      // to 6 % of the time.  The other forms have registers left, and gain 1 % by the shorter code.)
       auto steps = [&](auto looks) {
         if constexpr (DB) {
           for (int j = 0; ok && j < n; ++j) {
@@ -825,7 +828,7 @@ __global__ void __launch_bounds__(threads(FORM == kPair ? 2 : 1), FORM == kSmall
           }
         }
       };
-      if (look == 0) steps(std::false_type{});
+      if (FORM == kPair && look == 0) steps(std::false_type{});
       else steps(std::true_type{});
       if (elect_one()) {
         if (!ok) fail(kDevTimeoutMma);
